@@ -353,6 +353,97 @@ n3d_status n3d_bench_layer_norm(int device, size_t rows, size_t cols, int iters,
  * device time the wait took, and the device stays usable for the next call. */
 n3d_status n3d_selftest_wait_timeout(int device, double limit_ms, double *waited_ms);
 
+/* ------------------------------------- training operators of an encoder block */
+/* What a fine-tuning step of an encoder block needs next to its linear layers: rotary
+ * positions, the residual add with the norms before and after a block, and attention
+ * with its gradient.  No counterpart in the reference, which only runs inference.
+ *
+ * These calls enqueue their work on `stream` (a cudaStream_t, NULL for the default
+ * stream) and return without waiting for it.  They allocate nothing, keep nothing
+ * between calls and may be captured into a CUDA graph, after the first call on each
+ * device, which does a one-time set-up.  The caller's current device is left as it was.
+ * Calls from several threads are independent; two calls may overlap on the GPU when
+ * they share no output and no workspace.  Results do not depend on timing: every sum is
+ * taken in a fixed order.  Arithmetic, row statistics and sums are fp32; each output is
+ * rounded once to its type.
+ *
+ * The kernels' bounded waits record a timeout instead of hanging.  The record is seen by
+ * the next of these calls on the device, and by n3d_train_status, which return
+ * N3D_ERR_TIMEOUT once and clear it. */
+
+typedef enum n3d_dtype { N3D_F32 = 0, N3D_BF16 = 1, N3D_F16 = 2 } n3d_dtype;
+
+/* A device tensor [seqs, rows, heads, head_dim]: element (s, r, h, d) is at
+ * d_data + s * seq_stride + r * row_stride + h * head_stride + d (strides in elements,
+ * at least 0 for inputs, so that a dimension may be broadcast; the elements of an
+ * output must not overlap).  The sizes besides `heads` are the call's. */
+typedef struct n3d_heads {
+    void *d_data;
+    size_t heads;
+    long long seq_stride, row_stride, head_stride;
+} n3d_heads;
+
+/* A device matrix of rows: element (r, c) is at d_data + r * row_stride + c. */
+typedef struct n3d_rows {
+    void *d_data;
+    long long row_stride;
+} n3d_rows;
+
+/* N3D_ERR_TIMEOUT if a wait of an earlier training operator on `device` gave up (and
+ * clears it), N3D_OK otherwise.  Only work that has finished is reported: synchronise
+ * the stream first. */
+n3d_status n3d_train_status(int device);
+
+/* Rotary positions.  The first rotary_dim elements of each head are pairs
+ * (a, b) = (x[i], x[i + rotary_dim/2]) in the half layout (the encoder's, as
+ * src/encoder.rs:281-296) or (x[2i], x[2i + 1]) in the interleaved one, turned by the
+ * angle position * f_i and multiplied by the attention factor m:
+ *   (a, b) -> m (a cos - b sin, b cos + a sin);
+ * the remaining elements are copied.  f_i = theta^(-2i/rotary_dim), scaled by
+ *   LINEAR  f_i / factor;
+ *   NTK     theta * factor^(rotary_dim / (rotary_dim - 2)) in theta's place;
+ *   YARN    f_i where a pair makes at least beta_fast turns over original_length,
+ *           f_i / factor where it makes at most beta_slow, a linear ramp over the pairs
+ *           between; m = 0.1 ln(factor) + 1.
+ * attention_factor other than 0 replaces m (1 but for YARN). */
+typedef enum n3d_rope_layout { N3D_ROPE_HALF = 0, N3D_ROPE_INTERLEAVED = 1 } n3d_rope_layout;
+typedef enum n3d_rope_scaling {
+    N3D_ROPE_PLAIN = 0,
+    N3D_ROPE_LINEAR = 1,
+    N3D_ROPE_NTK = 2,
+    N3D_ROPE_YARN = 3
+} n3d_rope_scaling;
+typedef struct n3d_rope_config {
+    size_t head_dim;   /* 2..256 */
+    size_t rotary_dim; /* even, 2..head_dim */
+    int layout;        /* n3d_rope_layout */
+    int scaling;       /* n3d_rope_scaling */
+    double theta;      /* > 1 */
+    double factor;     /* >= 1; used by the scalings */
+    double original_length, beta_fast, beta_slow; /* YARN */
+    double attention_factor;                      /* 0: the scaling's own */
+} n3d_rope_config;
+/* The rotation per position of each pair, as a 64-bit fraction of a turn: position
+ * times turns[i], modulo 2^64, is the exact phase at any position. */
+typedef struct n3d_rope_plan {
+    uint32_t head_dim, rotary_dim;
+    int layout;
+    float attention_factor;
+    uint64_t turns[128];
+} n3d_rope_plan;
+/* Host only: no GPU is needed. */
+n3d_status n3d_rope_plan_make(const n3d_rope_config *cfg, n3d_rope_plan *plan);
+
+/* y[t] = rotated x[t] for `count` (1 or 2: queries and keys) tensors of type `dtype`
+ * that share their positions, in one launch.  Row r of sequence s is at position
+ * d_positions[s * rows + r], or first_position + r when d_positions is NULL; positions
+ * may be negative.  transpose != 0 applies the transposed rotation, which is the
+ * gradient: x then holds dL/dy and y receives dL/dx.  y[t] may be x[t] itself (the same
+ * pointer and strides), and must not overlap it otherwise. */
+n3d_status n3d_rope(int device, const n3d_rope_plan *plan, int dtype, size_t seqs, size_t rows, size_t count,
+                    const n3d_heads *x, const n3d_heads *y, const int32_t *d_positions, long long first_position,
+                    int transpose, void *stream);
+
 /* ------------------------------------------------------------- profiling */
 
 /* Device time per kernel class of the launches n3d_run_* make while profiling

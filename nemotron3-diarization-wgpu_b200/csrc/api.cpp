@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../include/n3d.h"
+#include "api_guard.h"
 #include "model.h"
 
 struct n3d_model {
@@ -35,27 +36,14 @@ namespace {
 
 thread_local std::string g_last_error;
 
-template <class F>
-n3d_status guarded(F&& f) {
-    try {
-        f();
-        g_last_error.clear();
-        return N3D_OK;
-    } catch (const n3d::Error& e) {
-        g_last_error = e.what();
-        return (n3d_status)e.status;
-    } catch (const std::bad_alloc&) {
-        g_last_error = "out of host memory";
-        return N3D_ERR_GPU;
-    } catch (const std::exception& e) {
-        g_last_error = e.what();
-        return N3D_ERR_GPU;
-    }
-}
+}  // namespace
 
-void arg_check(bool ok, const char* what) {
-    if (!ok) throw n3d::Error(N3D_ERR_INVALID_ARGUMENT, what);
-}
+std::string& n3d::last_error() { return g_last_error; }
+
+namespace {
+
+using n3d::arg_check;
+using n3d::guarded;
 
 void fill_output(n3d_run_output* out, std::vector<float>& logits, const n3d::ClipPlan& p, size_t ns) {
     out->num_speakers = ns;

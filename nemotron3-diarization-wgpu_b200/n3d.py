@@ -77,6 +77,26 @@ class CacheConfig(C.Structure):
                 ("num_strong_boosted_frames", _sz), ("num_weak_boosted_frames", _sz)]
 
 
+class _Heads(C.Structure):
+    _fields_ = [("d_data", C.c_void_p), ("heads", _sz), ("seq_stride", C.c_longlong), ("row_stride", C.c_longlong),
+                ("head_stride", C.c_longlong)]
+
+
+class _Rows(C.Structure):
+    _fields_ = [("d_data", C.c_void_p), ("row_stride", C.c_longlong)]
+
+
+class _RopeConfig(C.Structure):
+    _fields_ = [("head_dim", _sz), ("rotary_dim", _sz), ("layout", C.c_int), ("scaling", C.c_int),
+                ("theta", C.c_double), ("factor", C.c_double), ("original_length", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("attention_factor", C.c_double)]
+
+
+class _RopePlan(C.Structure):
+    _fields_ = [("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32), ("layout", C.c_int),
+                ("attention_factor", C.c_float), ("turns", C.c_uint64 * 128)]
+
+
 class _KernelStats(C.Structure):
     _fields_ = [("name", C.c_char_p), ("launches", _sz), ("ms", C.c_double), ("flops", C.c_double),
                 ("bytes", C.c_double)]
@@ -173,6 +193,10 @@ def lib() -> C.CDLL:
         "n3d_bench_linear": ([C.c_int, _sz, _sz, _sz, C.c_int, C.POINTER(C.c_double)], C.c_int),
         "n3d_bench_attention": ([C.c_int, _sz, _sz, _sz, C.c_int, C.POINTER(C.c_double)], C.c_int),
         "n3d_bench_layer_norm": ([C.c_int, _sz, _sz, C.c_int, C.POINTER(C.c_double)], C.c_int),
+        "n3d_train_status": ([C.c_int], C.c_int),
+        "n3d_rope_plan_make": ([C.POINTER(_RopeConfig), C.POINTER(_RopePlan)], C.c_int),
+        "n3d_rope": ([C.c_int, C.POINTER(_RopePlan), C.c_int, _sz, _sz, _sz, C.POINTER(_Heads), C.POINTER(_Heads), vp,
+                      C.c_longlong, C.c_int, vp], C.c_int),
         "n3d_profile_enable": ([vp, C.c_int], C.c_int),
         "n3d_profile_read": ([vp, C.POINTER(_KernelStats), _sz], _sz),
         "n3d_step_timing_enable": ([vp, C.c_int], C.c_int),
@@ -595,3 +619,108 @@ def selftest_wait_timeout(device: int, limit_ms: float) -> tuple[int, str, float
     w = C.c_double()
     st = lib().n3d_selftest_wait_timeout(device, limit_ms, C.byref(w))
     return st, lib().n3d_last_error().decode(), w.value
+
+
+# ---- training operators of an encoder block
+#
+# Tensors are any objects with data_ptr(), shape, stride() and dtype, as torch's (which
+# this module does not import).  Work is enqueued on `stream` (a cudaStream_t as an int,
+# None for the default stream) and the calls return without waiting for it.
+
+DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def _bad(message: str) -> DiarizationError:
+    return DiarizationError(13, message)
+
+
+def _dtype(t) -> int:
+    name = str(t.dtype).rpartition(".")[2]
+    if name not in DTYPES:
+        raise _bad(f"dtype {name}: float32, bfloat16 or float16 is wanted")
+    return DTYPES[name]
+
+
+def _device(t) -> int:
+    d = t.device
+    if d.type != "cuda":
+        raise _bad("a tensor is not in device memory")
+    return d.index or 0
+
+
+def _heads(t, shape=None, dtype=None) -> _Heads:
+    """A [seqs, rows, heads, head_dim] tensor as n3d_heads; `shape` and `dtype` are what it must have."""
+    sh, st = t.shape, t.stride()
+    if len(sh) != 4:
+        raise _bad("a [seqs, rows, heads, head_dim] tensor is wanted")
+    if shape is not None and tuple(sh) != tuple(shape):
+        raise _bad(f"a tensor of shape {tuple(sh)} where {tuple(shape)} is wanted")
+    if dtype is not None and t.dtype != dtype:
+        raise _bad(f"a tensor of type {t.dtype} where {dtype} is wanted")
+    if st[3] != 1 and sh[3] > 1:
+        raise _bad("the elements of a head must be consecutive")
+    return _Heads(t.data_ptr(), sh[2], st[0], st[1], st[2])
+
+
+def _flat(t, count: int, dtype: str, device: int):
+    """The pointer of a contiguous tensor of `count` elements (None: NULL)."""
+    if t is None:
+        return None
+    if not str(t.dtype).endswith(dtype) or t.numel() != count or not t.is_contiguous() or _device(t) != device:
+        raise _bad(f"a contiguous {dtype} tensor of {count} elements on device {device} is wanted")
+    return t.data_ptr()
+
+
+def train_status(device: int = 0) -> None:
+    """Raises Timeout if a wait of an earlier training operator on `device` gave up (n3d_train_status)."""
+    _check(lib().n3d_train_status(device))
+
+
+class RopePlan:
+    """Rotation frequencies of rotary positions (n3d_rope_plan_make).  Host only."""
+
+    def __init__(self, head_dim: int, rotary_dim: int | None = None, layout: str = "half", theta: float = 10000.0,
+                 scaling: str = "none", factor: float = 1.0, original_length: float = 4096, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, attention_factor: float = 0.0):
+        if layout not in ROPE_LAYOUTS or scaling not in ROPE_SCALINGS:
+            raise _bad(f"unknown layout {layout} or scaling {scaling}")
+        self._p = _RopePlan()
+        cfg = _RopeConfig(head_dim, head_dim if rotary_dim is None else rotary_dim, ROPE_LAYOUTS[layout],
+                          ROPE_SCALINGS[scaling], theta, factor, original_length, beta_fast, beta_slow,
+                          attention_factor)
+        _check(lib().n3d_rope_plan_make(C.byref(cfg), C.byref(self._p)))
+
+    @property
+    def head_dim(self) -> int:
+        return self._p.head_dim
+
+    @property
+    def attention_factor(self) -> float:
+        return self._p.attention_factor
+
+    @property
+    def turns(self) -> list[int]:
+        """Turns per position of each pair, in units of 2^-64 of a turn."""
+        return list(self._p.turns[: self._p.rotary_dim // 2])
+
+
+def rope(plan: RopePlan, xs, ys, positions=None, first_position: int = 0, transpose: bool = False,
+         stream: int | None = None) -> None:
+    """Rotary positions of one or two tensors [seqs, rows, heads, head_dim] (queries and keys) into `ys`
+    (n3d_rope); `ys` may be `xs`.  `positions`: int32 [seqs, rows], or None for first_position + row.
+    transpose=True is the gradient: dL/dy -> dL/dx."""
+    n = len(xs)
+    if n not in (1, 2) or len(ys) != n:
+        raise _bad("rope: one or two tensors, and as many outputs, are wanted")
+    seqs, rows, _, hd = xs[0].shape
+    if hd != plan.head_dim:
+        raise _bad(f"rope: head_dim {hd}, the plan has {plan.head_dim}")
+    dt, device = xs[0].dtype, _device(xs[0])
+    x, y = (_Heads * 2)(), (_Heads * 2)()
+    for i in range(n):
+        x[i] = _heads(xs[i], (seqs, rows, xs[i].shape[2], hd), dt)
+        y[i] = _heads(ys[i], xs[i].shape, dt)
+    _check(lib().n3d_rope(device, C.byref(plan._p), _dtype(xs[0]), seqs, rows, n, x, y,
+                          _flat(positions, seqs * rows, "int32", device), first_position, int(transpose), stream))
