@@ -444,6 +444,45 @@ n3d_status n3d_rope(int device, const n3d_rope_plan *plan, int dtype, size_t seq
                     const n3d_heads *x, const n3d_heads *y, const int32_t *d_positions, long long first_position,
                     int transpose, void *stream);
 
+/* The boundary between two blocks of the residual stream, in one pass:
+ *   u = Norm_post(block)               (post_norm; N3D_NORM_NONE: u = block)
+ *   r = x + scale * gate * u           (the new residual stream; no gate: 1)
+ *   y = Norm_pre(r)                    (pre_norm; N3D_NORM_NONE: y is not written)
+ * with Norm LayerNorm (as tensor::layer_norm, src/tensor.rs:97-110) or RMS norm over the
+ * cols elements of a row, times a weight, plus a bias.  y is computed from r before its
+ * rounding.  The gate has one row of cols values for every rows_per_gate rows (all rows: a
+ * learned gate per channel; a sequence's rows: a conditioning gate; 1: a gate per row). */
+typedef enum n3d_norm { N3D_NORM_NONE = 0, N3D_NORM_LAYER = 1, N3D_NORM_RMS = 2 } n3d_norm;
+typedef struct n3d_residual_config {
+    size_t rows, cols;                 /* cols 1..8192 */
+    int residual_dtype, block_dtype;   /* of x, r, dr, dx; of block, y, dy, dblock: the same, or fp32 and 16 bits */
+    int post_norm, pre_norm;           /* n3d_norm */
+    float post_eps, pre_eps;           /* above 0 where the norm is used */
+    float scale;
+    size_t rows_per_gate;              /* 0: no gate */
+} n3d_residual_config;
+/* Weights, biases and the gate [ceil(rows / rows_per_gate), cols] are fp32 and contiguous;
+ * a NULL weight is 1, a NULL bias 0, both unused with N3D_NORM_NONE.  r may be x, and y
+ * may be block (the same pointer and stride); otherwise no output overlaps an input. */
+n3d_status n3d_residual_norm(int device, const n3d_residual_config *cfg, const n3d_rows *x, const n3d_rows *block,
+                             const float *d_post_w, const float *d_post_b, const float *d_gate,
+                             const float *d_pre_w, const float *d_pre_b, const n3d_rows *r, const n3d_rows *y,
+                             void *stream);
+/* Its gradient at the r and block of the forward call (row statistics are taken again
+ * from them): with dy = dL/dy and dr = dL/dr from the stream's later users (NULL: 0),
+ *   dx = dr + (Norm_pre)'^T dy,   dblock = (Norm_post)'^T (scale * gate * dx),
+ * and, where the pointers are not NULL, the fp32 gradients of the gate, the weights and
+ * the biases, overwritten.  dy is NULL with N3D_NORM_NONE (dr is then needed).  dx may be
+ * dr, and dblock may be dy or block.  The workspace, 16-byte aligned, holds partial sums
+ * (n3d_residual_norm_workspace bytes; the same for every GPU). */
+size_t n3d_residual_norm_workspace(size_t rows, size_t cols, size_t rows_per_gate);
+n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config *cfg, const n3d_rows *block, const n3d_rows *r,
+                                  const float *d_post_w, const float *d_post_b, const float *d_gate,
+                                  const float *d_pre_w, const n3d_rows *dy, const n3d_rows *dr, const n3d_rows *dx,
+                                  const n3d_rows *dblock, float *d_dgate, float *d_dpost_w, float *d_dpost_b,
+                                  float *d_dpre_w, float *d_dpre_b, void *d_workspace, size_t workspace_bytes,
+                                  void *stream);
+
 /* ------------------------------------------------------------- profiling */
 
 /* Device time per kernel class of the launches n3d_run_* make while profiling

@@ -1,0 +1,63 @@
+// Shared by the residual-norm kernels: rows spread over TPR threads, sums over a row.
+#pragma once
+
+#include "n3d_device.cuh"
+#include "train.h"
+#include "train_types.cuh"
+
+namespace n3d {
+
+// Columns of thread t of a row: EPT of them, in chunks of VEC consecutive ones; chunk k
+// starts at (k * TPR + t) * VEC, so that a warp's chunk is one run of memory.
+template <int VEC, int TPR>
+__device__ __forceinline__ int chunk_col(int k, int t) {
+    return (k * TPR + t) * VEC;
+}
+
+// VEC fp32 values (weights), or `other` for a null pointer.
+template <int VEC>
+__device__ __forceinline__ void load_weights(const float* p, int col, float other, float* v) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = other;
+        return;
+    }
+    if constexpr (VEC == 1) {
+        v[0] = __ldg(p + col);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(p + col + i));
+            v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+        }
+    }
+}
+
+// Sums of NV values over the TPR threads of a row, the same in every thread and taken in
+// a fixed order: a butterfly in each warp, then the warps' sums by another.  `buf` (one
+// per call site of a row, TPR / 32 * NV floats) may be written again once a later sum of
+// the row has been taken.  Threads of a row wait only for one another (named barrier
+// 1 + slot of the block).
+template <int TPR, int NV>
+__device__ __forceinline__ void row_sums(float (&v)[NV], float* buf, int slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < NV; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        const int lane = threadIdx.x & 31, warp = (threadIdx.x % TPR) >> 5;
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < NV; i++) buf[i * W + warp] = v[i];
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "n"(TPR) : "memory");
+#pragma unroll
+        for (int i = 0; i < NV; i++) v[i] = buf[i * W + lane % W];
+#pragma unroll
+        for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < NV; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+}
+
+}  // namespace n3d

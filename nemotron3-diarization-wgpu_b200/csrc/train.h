@@ -34,4 +34,31 @@ struct RopeArgs {
 };
 void launch_rope(cudaStream_t s, const RopeArgs& a, const n3d_rope_plan& plan, int dtype);
 
+// ---- residual_norm.cu, residual_norm_grad.cu
+struct ResidualArgs {
+    long long rows;
+    int cols;
+    int post, pre;  // n3d_norm
+    float post_eps, pre_eps, scale;
+    long long rows_per_gate;  // 0: no gate
+    const float *post_w, *post_b, *gate, *pre_w, *pre_b;
+    const void *x, *block, *r, *dy, *dr;
+    long long ld_x, ld_block, ld_r, ld_dy, ld_dr;
+    void *r_out, *y, *dx, *dblock;
+    long long ld_r_out, ld_y, ld_dx, ld_dblock;
+    float *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+    float* sums;        // [blocks][4][cols]: post weight and bias, pre weight and bias
+    float* gate_parts;  // [slots][2][cols]
+    int slots;          // row ranges of the gradient kernel
+    int wide;           // every row, weight and row stride is a whole number of 16-byte words
+};
+void launch_residual_norm(cudaStream_t s, const ResidualArgs& a, int residual_dtype, int block_dtype);
+// How the gradient kernel splits the rows: `slots` ranges (range i is rows
+// rows * i / slots ..), `blocks` thread blocks, `threads` per row.
+struct ResidualSplit {
+    int threads, per_block, slots, blocks;
+};
+ResidualSplit residual_split(long long rows, int cols, bool wide);
+void launch_residual_norm_grad(cudaStream_t s, const ResidualArgs& a, int residual_dtype, int block_dtype);
+
 }  // namespace n3d

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <initializer_list>
 #include <mutex>
 
 #include "api_guard.h"
@@ -85,6 +86,70 @@ void check_heads(const n3d_heads& t, size_t seqs, size_t rows, size_t dim, int d
             arg_check(st[i] >= span, "an output's elements overlap");
             span = st[i] * (n[i] - 1) + span;
         }
+}
+
+// One dimension of a row view: non-negative strides, representable offsets; the rows of
+// an output do not overlap.
+void check_rows(const n3d_rows& t, size_t rows, size_t cols, int dtype, bool distinct) {
+    arg_check(t.d_data || rows == 0, "null matrix");
+    arg_check(reinterpret_cast<uintptr_t>(t.d_data) % n3d::dtype_size(dtype) == 0, "matrix not aligned to its type");
+    arg_check(t.row_stride >= 0, "negative row stride");
+    if (rows > 1) {
+        arg_check(t.row_stride <= kMaxOffset / (long long)rows, "row stride beyond 2^60 elements");
+        arg_check(!distinct || t.row_stride >= (long long)cols, "an output's rows overlap");
+    }
+}
+bool wide_rows(const n3d_rows* t, int dtype) {
+    const int per = 16 / n3d::dtype_size(dtype);
+    return !t || (reinterpret_cast<uintptr_t>(t->d_data) % 16 == 0 && t->row_stride % per == 0);
+}
+bool wide_weights(std::initializer_list<const float*> ws) {
+    for (const float* w : ws)
+        if (reinterpret_cast<uintptr_t>(w) % 16) return false;
+    return true;
+}
+// `out` may be `in` itself (in place).
+void check_in_place(const n3d_rows& out, const n3d_rows& in, size_t rows, const char* what) {
+    if (out.d_data == in.d_data) arg_check(rows <= 1 || out.row_stride == in.row_stride, what);
+}
+
+void check_residual(const n3d_residual_config* cfg) {
+    arg_check(cfg != nullptr, "residual norm: null configuration");
+    arg_check(cfg->cols >= 1 && cfg->cols <= 8192, "residual norm: cols outside 1..8192");
+    arg_check(cfg->rows <= (size_t)INT_MAX, "residual norm: rows beyond 2^31");
+    check_dtype(cfg->residual_dtype);
+    check_dtype(cfg->block_dtype);
+    arg_check(cfg->residual_dtype == N3D_F32 || cfg->residual_dtype == cfg->block_dtype,
+              "residual norm: the residual stream has the block's type or fp32");
+    for (int n : {cfg->post_norm, cfg->pre_norm})
+        arg_check(n == N3D_NORM_NONE || n == N3D_NORM_LAYER || n == N3D_NORM_RMS, "residual norm: unknown norm");
+    arg_check(cfg->post_norm == N3D_NORM_NONE || cfg->post_eps > 0.0f, "residual norm: post_eps must be above 0");
+    arg_check(cfg->pre_norm == N3D_NORM_NONE || cfg->pre_eps > 0.0f, "residual norm: pre_eps must be above 0");
+}
+n3d::ResidualArgs residual_args(const n3d_residual_config& cfg) {
+    n3d::ResidualArgs a{};
+    a.rows = (long long)cfg.rows;
+    a.cols = (int)cfg.cols;
+    a.post = cfg.post_norm;
+    a.pre = cfg.pre_norm;
+    a.post_eps = cfg.post_eps;
+    a.pre_eps = cfg.pre_eps;
+    a.scale = cfg.scale;
+    a.rows_per_gate = (long long)std::min(cfg.rows_per_gate, std::max<size_t>(cfg.rows, 1));
+    return a;
+}
+struct ResidualWorkspace {
+    size_t sums, gate_parts;  // floats
+};
+ResidualWorkspace residual_workspace(size_t rows, size_t cols, bool gate) {
+    ResidualWorkspace w{0, 0};
+    for (bool wide : {false, true}) {
+        const n3d::ResidualSplit sp = n3d::residual_split((long long)rows, (int)cols, wide);
+        w.sums = std::max(w.sums, (size_t)sp.blocks * 4 * cols);
+        w.gate_parts = std::max(w.gate_parts, gate ? (size_t)sp.slots * 2 * cols : 0);
+    }
+    w.sums = (w.sums + 3) / 4 * 4;
+    return w;
 }
 
 n3d::HeadsView view(const n3d_heads& t) { return {t.d_data, t.seq_stride, t.row_stride, t.head_stride}; }
@@ -192,6 +257,99 @@ n3d_status n3d_rope(int device, const n3d_rope_plan* plan, int dtype, size_t seq
         DeviceGuard g(device);
         check_record(train_error(device));
         n3d::launch_rope((cudaStream_t)stream, a, *plan, dtype);
+    });
+}
+
+n3d_status n3d_residual_norm(int device, const n3d_residual_config* cfg, const n3d_rows* x, const n3d_rows* block,
+                             const float* d_post_w, const float* d_post_b, const float* d_gate, const float* d_pre_w,
+                             const float* d_pre_b, const n3d_rows* r, const n3d_rows* y, void* stream) {
+    return guarded([&] {
+        check_residual(cfg);
+        const bool pre = cfg->pre_norm != N3D_NORM_NONE;
+        arg_check(x && block && r && (y || !pre), "n3d_residual_norm: null argument");
+        arg_check(cfg->rows_per_gate == 0 || cfg->rows == 0 || d_gate, "n3d_residual_norm: null gate");
+        check_rows(*x, cfg->rows, cfg->cols, cfg->residual_dtype, false);
+        check_rows(*block, cfg->rows, cfg->cols, cfg->block_dtype, false);
+        check_rows(*r, cfg->rows, cfg->cols, cfg->residual_dtype, true);
+        if (pre) check_rows(*y, cfg->rows, cfg->cols, cfg->block_dtype, true);
+        check_in_place(*r, *x, cfg->rows, "n3d_residual_norm: in place, r and x must have the same stride");
+        if (pre) check_in_place(*y, *block, cfg->rows, "n3d_residual_norm: in place, y and block must have the same stride");
+        n3d::ResidualArgs a = residual_args(*cfg);
+        a.post_w = d_post_w, a.post_b = d_post_b, a.pre_w = d_pre_w, a.pre_b = d_pre_b;
+        a.gate = d_gate;
+        a.x = x->d_data, a.ld_x = x->row_stride;
+        a.block = block->d_data, a.ld_block = block->row_stride;
+        a.r_out = r->d_data, a.ld_r_out = r->row_stride;
+        if (pre) a.y = y->d_data, a.ld_y = y->row_stride;
+        a.wide = cfg->cols % 8 == 0 && wide_rows(x, cfg->residual_dtype) && wide_rows(r, cfg->residual_dtype) &&
+                 wide_rows(block, cfg->block_dtype) && wide_rows(pre ? y : nullptr, cfg->block_dtype) &&
+                 wide_weights({d_post_w, d_post_b, d_gate, d_pre_w, d_pre_b});
+        if (cfg->rows == 0) return;
+        DeviceGuard g(device);
+        check_record(train_error(device));
+        n3d::launch_residual_norm((cudaStream_t)stream, a, cfg->residual_dtype, cfg->block_dtype);
+    });
+}
+
+size_t n3d_residual_norm_workspace(size_t rows, size_t cols, size_t rows_per_gate) {
+    if (rows > (size_t)INT_MAX || cols < 1 || cols > 8192) return 0;
+    const ResidualWorkspace w = residual_workspace(rows, cols, rows_per_gate != 0);
+    return (w.sums + w.gate_parts) * sizeof(float);
+}
+
+n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config* cfg, const n3d_rows* block, const n3d_rows* r,
+                                  const float* d_post_w, const float* d_post_b, const float* d_gate,
+                                  const float* d_pre_w, const n3d_rows* dy, const n3d_rows* dr, const n3d_rows* dx,
+                                  const n3d_rows* dblock, float* d_dgate, float* d_dpost_w, float* d_dpost_b,
+                                  float* d_dpre_w, float* d_dpre_b, void* d_workspace, size_t workspace_bytes,
+                                  void* stream) {
+    return guarded([&] {
+        check_residual(cfg);
+        const bool pre = cfg->pre_norm != N3D_NORM_NONE, post = cfg->post_norm != N3D_NORM_NONE;
+        arg_check(block && dx && dblock && (!pre || (r && dy)) && (pre || dr), "n3d_residual_norm_grad: null argument");
+        arg_check(cfg->rows_per_gate == 0 || cfg->rows == 0 || d_gate, "n3d_residual_norm_grad: null gate");
+        arg_check(cfg->rows_per_gate != 0 || !d_dgate, "n3d_residual_norm_grad: the gradient of a gate that is not used");
+        arg_check(post || (!d_dpost_w && !d_dpost_b), "n3d_residual_norm_grad: gradients of a norm that is not used");
+        arg_check(pre || (!d_dpre_w && !d_dpre_b), "n3d_residual_norm_grad: gradients of a norm that is not used");
+        const size_t rows = cfg->rows, cols = cfg->cols;
+        const int rt = cfg->residual_dtype, bt = cfg->block_dtype;
+        check_rows(*block, rows, cols, bt, false);
+        if (pre) check_rows(*r, rows, cols, rt, false);
+        if (pre) check_rows(*dy, rows, cols, bt, false);
+        if (dr) check_rows(*dr, rows, cols, rt, false);
+        check_rows(*dx, rows, cols, rt, true);
+        check_rows(*dblock, rows, cols, bt, true);
+        const char* strides = "n3d_residual_norm_grad: in place, the strides must be the same";
+        if (dr) check_in_place(*dx, *dr, rows, strides);
+        if (pre) check_in_place(*dblock, *dy, rows, strides);
+        check_in_place(*dblock, *block, rows, strides);
+        const ResidualWorkspace w = residual_workspace(rows, cols, cfg->rows_per_gate != 0);
+        arg_check(workspace_bytes >= (w.sums + w.gate_parts) * sizeof(float) && d_workspace &&
+                      reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0,
+                  "n3d_residual_norm_grad: a 16-byte aligned workspace of n3d_residual_norm_workspace bytes is wanted");
+        DeviceGuard g(device);
+        check_record(train_error(device));
+        if (rows == 0) {  // sums over nothing
+            for (float* p : {d_dpost_w, d_dpost_b, d_dpre_w, d_dpre_b})
+                if (p) N3D_CUDA(cudaMemsetAsync(p, 0, cols * sizeof(float), (cudaStream_t)stream));
+            return;
+        }
+        n3d::ResidualArgs a = residual_args(*cfg);
+        a.post_w = d_post_w, a.post_b = d_post_b, a.pre_w = d_pre_w;
+        a.gate = d_gate;
+        a.block = block->d_data, a.ld_block = block->row_stride;
+        if (pre) a.r = r->d_data, a.ld_r = r->row_stride, a.dy = dy->d_data, a.ld_dy = dy->row_stride;
+        if (dr) a.dr = dr->d_data, a.ld_dr = dr->row_stride;
+        a.dx = dx->d_data, a.ld_dx = dx->row_stride;
+        a.dblock = dblock->d_data, a.ld_dblock = dblock->row_stride;
+        a.dgate = d_dgate, a.dpost_w = d_dpost_w, a.dpost_b = d_dpost_b, a.dpre_w = d_dpre_w, a.dpre_b = d_dpre_b;
+        a.sums = static_cast<float*>(d_workspace);
+        a.gate_parts = a.sums + w.sums;
+        a.wide = cols % 8 == 0 && wide_rows(block, bt) && wide_rows(dx, rt) && wide_rows(dblock, bt) &&
+                 wide_rows(pre ? r : nullptr, rt) && wide_rows(pre ? dy : nullptr, bt) && wide_rows(dr, rt) &&
+                 wide_weights({d_post_w, d_post_b, d_gate, d_pre_w, d_dgate});
+        a.slots = n3d::residual_split(a.rows, a.cols, a.wide).slots;
+        n3d::launch_residual_norm_grad((cudaStream_t)stream, a, rt, bt);
     });
 }
 

@@ -86,6 +86,12 @@ class _Rows(C.Structure):
     _fields_ = [("d_data", C.c_void_p), ("row_stride", C.c_longlong)]
 
 
+class _ResidualConfig(C.Structure):
+    _fields_ = [("rows", _sz), ("cols", _sz), ("residual_dtype", C.c_int), ("block_dtype", C.c_int),
+                ("post_norm", C.c_int), ("pre_norm", C.c_int), ("post_eps", C.c_float), ("pre_eps", C.c_float),
+                ("scale", C.c_float), ("rows_per_gate", _sz)]
+
+
 class _RopeConfig(C.Structure):
     _fields_ = [("head_dim", _sz), ("rotary_dim", _sz), ("layout", C.c_int), ("scaling", C.c_int),
                 ("theta", C.c_double), ("factor", C.c_double), ("original_length", C.c_double),
@@ -197,6 +203,12 @@ def lib() -> C.CDLL:
         "n3d_rope_plan_make": ([C.POINTER(_RopeConfig), C.POINTER(_RopePlan)], C.c_int),
         "n3d_rope": ([C.c_int, C.POINTER(_RopePlan), C.c_int, _sz, _sz, _sz, C.POINTER(_Heads), C.POINTER(_Heads), vp,
                       C.c_longlong, C.c_int, vp], C.c_int),
+        "n3d_residual_norm": ([C.c_int, C.POINTER(_ResidualConfig), C.POINTER(_Rows), C.POINTER(_Rows), vp, vp, vp, vp,
+                               vp, C.POINTER(_Rows), C.POINTER(_Rows), vp], C.c_int),
+        "n3d_residual_norm_workspace": ([_sz, _sz, _sz], _sz),
+        "n3d_residual_norm_grad": ([C.c_int, C.POINTER(_ResidualConfig), C.POINTER(_Rows), C.POINTER(_Rows), vp, vp, vp,
+                                    vp, C.POINTER(_Rows), C.POINTER(_Rows), C.POINTER(_Rows), C.POINTER(_Rows), vp, vp,
+                                    vp, vp, vp, vp, _sz, vp], C.c_int),
         "n3d_profile_enable": ([vp, C.c_int], C.c_int),
         "n3d_profile_read": ([vp, C.POINTER(_KernelStats), _sz], _sz),
         "n3d_step_timing_enable": ([vp, C.c_int], C.c_int),
@@ -724,3 +736,73 @@ def rope(plan: RopePlan, xs, ys, positions=None, first_position: int = 0, transp
         y[i] = _heads(ys[i], xs[i].shape, dt)
     _check(lib().n3d_rope(device, C.byref(plan._p), _dtype(xs[0]), seqs, rows, n, x, y,
                           _flat(positions, seqs * rows, "int32", device), first_position, int(transpose), stream))
+
+
+NORMS = {"none": 0, "layer": 1, "rms": 2}
+
+
+def _rows(t, shape, dtype=None):
+    """A [rows, cols] tensor as n3d_rows (None: NULL)."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape:
+        raise _bad(f"a matrix of shape {tuple(t.shape)} where {shape} is wanted")
+    if dtype is not None and t.dtype != dtype:
+        raise _bad(f"a matrix of type {t.dtype} where {dtype} is wanted")
+    st = t.stride()
+    if st[1] != 1 and shape[1] > 1:
+        raise _bad("the elements of a row must be consecutive")
+    return C.byref(_Rows(t.data_ptr(), st[0]))
+
+
+def _residual_config(residual, block, post, pre, eps, scale, gate, gate_rows):
+    if post not in NORMS or pre not in NORMS:
+        raise _bad(f"unknown norm {post} or {pre}")
+    if len(block.shape) != 2:
+        raise _bad("a [rows, cols] matrix is wanted")
+    rows, cols = block.shape
+    if gate is None:
+        gate_rows = 0
+    elif gate_rows < 1:
+        raise _bad("a gate needs gate_rows, the number of rows that share one of its rows")
+    return _ResidualConfig(rows, cols, _dtype(residual), _dtype(block), NORMS[post], NORMS[pre], eps, eps, scale,
+                           gate_rows)
+
+
+def residual_norm(x, block, r, y, post: str = "none", pre: str = "layer", eps: float = 1e-5, scale: float = 1.0,
+                  post_w=None, post_b=None, gate=None, gate_rows: int = 0, pre_w=None, pre_b=None,
+                  stream: int | None = None) -> None:
+    """r = x + scale * gate * Norm_post(block), y = Norm_pre(r) (n3d_residual_norm); norms are "none",
+    "layer" or "rms".  gate [ceil(rows / gate_rows), cols], weights and biases [cols]: fp32 or None.
+    r may be x, y may be block; y is None when pre is "none"."""
+    cfg = _residual_config(x, block, post, pre, eps, scale, gate, gate_rows)
+    sh, dev, cols = (cfg.rows, cfg.cols), _device(x), cfg.cols
+    gates = -(-cfg.rows // cfg.rows_per_gate) * cols if gate is not None else 0
+    _check(lib().n3d_residual_norm(
+        dev, C.byref(cfg), _rows(x, sh), _rows(block, sh), _flat(post_w, cols, "float32", dev),
+        _flat(post_b, cols, "float32", dev), _flat(gate, gates, "float32", dev), _flat(pre_w, cols, "float32", dev),
+        _flat(pre_b, cols, "float32", dev), _rows(r, sh, x.dtype), _rows(y, sh, block.dtype), stream))
+
+
+def residual_norm_workspace(rows: int, cols: int, gate_rows: int = 0) -> int:
+    """Bytes of workspace residual_norm_grad needs (n3d_residual_norm_workspace)."""
+    return lib().n3d_residual_norm_workspace(rows, cols, gate_rows)
+
+
+def residual_norm_grad(block, r, dy, dr, dx, dblock, post: str = "none", pre: str = "layer", eps: float = 1e-5,
+                       scale: float = 1.0, post_w=None, post_b=None, gate=None, gate_rows: int = 0, pre_w=None,
+                       pre_b=None, dgate=None, dpost_w=None, dpost_b=None, dpre_w=None, dpre_b=None, workspace=None,
+                       stream: int | None = None) -> None:
+    """The gradient of residual_norm (n3d_residual_norm_grad): dy and dr (or None) -> dx, dblock, and the
+    fp32 gradients that are not None.  `workspace`: a tensor of at least residual_norm_workspace bytes.
+    pre_b does not enter; it is accepted so that both calls take the same arguments."""
+    cfg = _residual_config(dx, block, post, pre, eps, scale, gate, gate_rows)
+    sh, dev, cols = (cfg.rows, cfg.cols), _device(dx), cfg.cols
+    gates = -(-cfg.rows // cfg.rows_per_gate) * cols if gate is not None else 0
+    w = [_flat(t, cols, "float32", dev) for t in (post_w, post_b, pre_w, dpost_w, dpost_b, dpre_w, dpre_b)]
+    _check(lib().n3d_residual_norm_grad(
+        dev, C.byref(cfg), _rows(block, sh), _rows(r, sh, dx.dtype), w[0], w[1], _flat(gate, gates, "float32", dev), w[2],
+        _rows(dy, sh, block.dtype), _rows(dr, sh, dx.dtype), _rows(dx, sh), _rows(dblock, sh, block.dtype),
+        _flat(dgate, gates, "float32", dev), w[3], w[4], w[5], w[6],
+        workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))

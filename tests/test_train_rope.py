@@ -13,6 +13,7 @@ import numpy as np
 import pytest
 
 import n3d
+from fake_tensor import FakeTensor
 
 ULP = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}  # half an ulp, relative
 
@@ -62,37 +63,6 @@ def test_plan_refusals(kw):
     with pytest.raises(n3d.DiarizationError) as e:
         n3d.RopePlan(**kw)
     assert e.value.kind == "InvalidArgument"
-
-
-class FakeTensor:
-    """Looks like a device tensor; its memory is never touched, since the calls are refused."""
-
-    def __init__(self, shape, stride=None, dtype="float32", ptr=1 << 20):
-        self.shape, self.dtype, self._p = tuple(shape), "torch." + dtype, ptr
-        if stride is None:
-            stride, n = [], 1
-            for s in reversed(self.shape):
-                stride.insert(0, n)
-                n *= s
-        self._s = tuple(stride)
-        self.device = type("Device", (), {"type": "cuda", "index": 0})()
-
-    def data_ptr(self):
-        return self._p
-
-    def stride(self):
-        return self._s
-
-    def numel(self):
-        return math.prod(self.shape)
-
-    def is_contiguous(self):
-        n = 1
-        for s, t in zip(reversed(self.shape), reversed(self._s)):
-            if s > 1 and t != n:
-                return False
-            n *= s
-        return True
 
 
 @pytest.mark.parametrize("x,y", [
