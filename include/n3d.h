@@ -483,6 +483,44 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config *cfg, co
                                   float *d_dpre_w, float *d_dpre_b, void *d_workspace, size_t workspace_bytes,
                                   void *stream);
 
+/* Attention for training.  For sequence b, query head h and its key head
+ * h / (q heads / k heads), query row i sees key row j when
+ *   i < q_len[b],  j < k_len[b]  and  -left <= j - (i + q_offset) <= right
+ * (a negative left or right is no limit; right = 0 with q_offset = k_rows - q_rows is
+ * causal attention), and
+ *   S = scale q.k,  lse = ln sum_j exp S,  out = sum_j exp(S - lse) v.
+ * A row that sees no key has out = 0 and lse = -inf, and no gradient passes it.  Rows at
+ * or past q_len and k_len are not read: they may hold anything.  q_len and k_len are
+ * int32 [seqs] device arrays, values outside 0..rows are clamped; NULL means all rows.
+ *
+ * bf16 and fp16 products run on the tensor cores with probabilities and their gradients
+ * rounded to the type before the second product (sums stay fp32); fp32 tensors keep fp32
+ * accuracy. */
+typedef struct n3d_attn_config {
+    size_t seqs, q_rows, k_rows;
+    size_t head_dim; /* 64 or 128 */
+    int dtype;       /* n3d_dtype, of every tensor */
+    float scale;     /* 0: head_dim^-1/2 */
+    long long left, right, q_offset; /* at most 2^30 in magnitude */
+} n3d_attn_config;
+/* Bytes of workspace, 16-byte aligned, that forward (backward = 0) or backward needs; it
+ * may be 0.  Nothing in it has to survive from one call to the next. */
+size_t n3d_attention_workspace(const n3d_attn_config *cfg, size_t q_heads, size_t k_heads, int backward);
+/* out, and the row statistics lse [seqs, q heads, q_rows] (fp32, contiguous; may be NULL
+ * when no gradient is wanted). */
+n3d_status n3d_attention_forward(int device, const n3d_attn_config *cfg, const n3d_heads *q, const n3d_heads *k,
+                                 const n3d_heads *v, const int32_t *d_q_len, const int32_t *d_k_len,
+                                 const n3d_heads *out, float *d_lse, void *d_workspace, size_t workspace_bytes,
+                                 void *stream);
+/* dq, dk and dv for dout = dL/dout, from the out and lse of the forward call; the
+ * probabilities are computed again.  Gradients of shared key heads are summed over their
+ * query heads.  Rows without gradient are written as zeros. */
+n3d_status n3d_attention_backward(int device, const n3d_attn_config *cfg, const n3d_heads *q, const n3d_heads *k,
+                                  const n3d_heads *v, const n3d_heads *out, const float *d_lse, const n3d_heads *dout,
+                                  const int32_t *d_q_len, const int32_t *d_k_len, const n3d_heads *dq,
+                                  const n3d_heads *dk, const n3d_heads *dv, void *d_workspace, size_t workspace_bytes,
+                                  void *stream);
+
 /* ------------------------------------------------------------- profiling */
 
 /* Device time per kernel class of the launches n3d_run_* make while profiling

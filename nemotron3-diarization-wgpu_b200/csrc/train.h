@@ -61,4 +61,45 @@ struct ResidualSplit {
 ResidualSplit residual_split(long long rows, int cols, bool wide);
 void launch_residual_norm_grad(cudaStream_t s, const ResidualArgs& a, int residual_dtype, int block_dtype);
 
+// ---- attention_train.cu, attention_train_tc.cu
+struct AttnArgs {
+    HeadsView q, k, v, o, dout, dq, dk, dv;
+    float* lse;         // [seqs, q_heads, q_rows], null: not wanted (forward)
+    float* row_dot;     // workspace [seqs, q_heads, q_rows]: dout . out
+    int seqs, q_rows, k_rows, q_heads, k_heads, head_dim;
+    float scale;
+    int left, right, offset;      // kNoLimit where unlimited
+    const int32_t *q_len, *k_len;  // null: all rows
+};
+constexpr int kNoLimit = 1 << 30;
+
+// The rows of one sequence and which keys a query row sees.
+struct AttnMask {
+    int q_len, k_len, left, right, offset;
+#ifdef __CUDACC__
+    __device__ __forceinline__ AttnMask(const AttnArgs& a, int seq)
+        : q_len(a.q_len ? min(max(a.q_len[seq], 0), a.q_rows) : a.q_rows),
+          k_len(a.k_len ? min(max(a.k_len[seq], 0), a.k_rows) : a.k_rows),
+          left(a.left),
+          right(a.right),
+          offset(a.offset) {}
+    // key rows [first, last) of query row i, empty when last <= first
+    __device__ __forceinline__ int first_key(int i) const {
+        return left >= kNoLimit ? 0 : (int)max(0LL, (long long)i + offset - left);
+    }
+    __device__ __forceinline__ int last_key(int i) const {
+        return right >= kNoLimit ? k_len : (int)max(0LL, min((long long)k_len, (long long)i + offset + right + 1));
+    }
+    // query rows [first, last) that see key row j
+    __device__ __forceinline__ int first_query(int j) const {
+        return right >= kNoLimit ? 0 : (int)max(0LL, (long long)j - offset - right);
+    }
+    __device__ __forceinline__ int last_query(int j) const {
+        return left >= kNoLimit ? q_len : (int)max(0LL, min((long long)q_len, (long long)j - offset + left + 1));
+    }
+#endif
+};
+void launch_attention_forward(cudaStream_t s, const AttnArgs& a, int dtype);
+void launch_attention_backward(cudaStream_t s, const AttnArgs& a, int dtype);
+
 }  // namespace n3d

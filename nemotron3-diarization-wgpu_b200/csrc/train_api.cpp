@@ -154,6 +154,43 @@ ResidualWorkspace residual_workspace(size_t rows, size_t cols, bool gate) {
 
 n3d::HeadsView view(const n3d_heads& t) { return {t.d_data, t.seq_stride, t.row_stride, t.head_stride}; }
 
+void check_attn(const n3d_attn_config* cfg) {
+    arg_check(cfg != nullptr, "attention: null configuration");
+    arg_check(cfg->head_dim == 64 || cfg->head_dim == 128, "attention: head_dim must be 64 or 128");
+    check_dtype(cfg->dtype);
+    arg_check(cfg->seqs <= (size_t)INT_MAX && cfg->q_rows <= (size_t)1 << 30 && cfg->k_rows <= (size_t)1 << 30,
+              "attention: seqs beyond 2^31 or rows beyond 2^30");
+    arg_check(std::isfinite(cfg->scale), "attention: scale is not finite");
+    arg_check(cfg->left <= n3d::kNoLimit && cfg->right <= n3d::kNoLimit && cfg->q_offset <= n3d::kNoLimit &&
+                  cfg->q_offset >= -n3d::kNoLimit,
+              "attention: left, right or q_offset beyond 2^30");
+}
+// The tensors every attention call has; fills their views.
+n3d::AttnArgs attn_args(const n3d_attn_config& cfg, const n3d_heads* q, const n3d_heads* k, const n3d_heads* v,
+                        const n3d_heads* out, bool out_written, const int32_t* q_len, const int32_t* k_len) {
+    arg_check(q && k && v && out, "attention: null argument");
+    check_heads(*q, cfg.seqs, cfg.q_rows, cfg.head_dim, cfg.dtype, false);
+    check_heads(*k, cfg.seqs, cfg.k_rows, cfg.head_dim, cfg.dtype, false);
+    check_heads(*v, cfg.seqs, cfg.k_rows, cfg.head_dim, cfg.dtype, false);
+    check_heads(*out, cfg.seqs, cfg.q_rows, cfg.head_dim, cfg.dtype, out_written);
+    arg_check(k->heads == v->heads && q->heads == out->heads, "attention: q and out, k and v must have the same heads");
+    arg_check(q->heads % k->heads == 0, "attention: the query heads must be a multiple of the key heads");
+    n3d::AttnArgs a{};
+    a.q = view(*q), a.k = view(*k), a.v = view(*v), a.o = view(*out);
+    a.seqs = (int)cfg.seqs, a.q_rows = (int)cfg.q_rows, a.k_rows = (int)cfg.k_rows;
+    a.q_heads = (int)q->heads, a.k_heads = (int)k->heads, a.head_dim = (int)cfg.head_dim;
+    a.scale = cfg.scale != 0.0f ? cfg.scale : (float)(1.0 / std::sqrt((double)cfg.head_dim));
+    a.left = cfg.left < 0 ? n3d::kNoLimit : (int)cfg.left;
+    a.right = cfg.right < 0 ? n3d::kNoLimit : (int)cfg.right;
+    a.offset = (int)cfg.q_offset;
+    a.q_len = q_len, a.k_len = k_len;
+    return a;
+}
+void check_workspace(size_t need, const void* p, size_t bytes) {
+    arg_check(need == 0 || (p && bytes >= need && reinterpret_cast<uintptr_t>(p) % 16 == 0),
+              "attention: a 16-byte aligned workspace of n3d_attention_workspace bytes is wanted");
+}
+
 void check_sizes(size_t seqs, size_t rows) {
     arg_check(seqs <= (size_t)INT_MAX && rows <= (size_t)INT_MAX, "seqs or rows beyond 2^31");
 }
@@ -350,6 +387,55 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config* cfg, co
                  wide_weights({d_post_w, d_post_b, d_gate, d_pre_w, d_dgate});
         a.slots = n3d::residual_split(a.rows, a.cols, a.wide).slots;
         n3d::launch_residual_norm_grad((cudaStream_t)stream, a, rt, bt);
+    });
+}
+
+size_t n3d_attention_workspace(const n3d_attn_config* cfg, size_t q_heads, size_t k_heads, int backward) {
+    if (!cfg || q_heads > 65535 || k_heads > 65535 || cfg->seqs > (size_t)INT_MAX || cfg->q_rows > (size_t)1 << 30)
+        return 0;
+    return backward ? cfg->seqs * q_heads * cfg->q_rows * sizeof(float) : 0;
+}
+
+n3d_status n3d_attention_forward(int device, const n3d_attn_config* cfg, const n3d_heads* q, const n3d_heads* k,
+                                 const n3d_heads* v, const int32_t* d_q_len, const int32_t* d_k_len,
+                                 const n3d_heads* out, float* d_lse, void* d_workspace, size_t workspace_bytes,
+                                 void* stream) {
+    return guarded([&] {
+        check_attn(cfg);
+        n3d::AttnArgs a = attn_args(*cfg, q, k, v, out, true, d_q_len, d_k_len);
+        check_workspace(n3d_attention_workspace(cfg, q->heads, k->heads, 0), d_workspace, workspace_bytes);
+        a.lse = d_lse;
+        if (cfg->seqs == 0 || cfg->q_rows == 0) return;
+        DeviceGuard g(device);
+        check_record(train_error(device));
+        n3d::launch_attention_forward((cudaStream_t)stream, a, cfg->dtype);
+    });
+}
+
+n3d_status n3d_attention_backward(int device, const n3d_attn_config* cfg, const n3d_heads* q, const n3d_heads* k,
+                                  const n3d_heads* v, const n3d_heads* out, const float* d_lse, const n3d_heads* dout,
+                                  const int32_t* d_q_len, const int32_t* d_k_len, const n3d_heads* dq,
+                                  const n3d_heads* dk, const n3d_heads* dv, void* d_workspace, size_t workspace_bytes,
+                                  void* stream) {
+    return guarded([&] {
+        check_attn(cfg);
+        n3d::AttnArgs a = attn_args(*cfg, q, k, v, out, false, d_q_len, d_k_len);
+        arg_check(dout && dq && dk && dv, "n3d_attention_backward: null argument");
+        arg_check(d_lse || cfg->seqs == 0 || cfg->q_rows == 0, "n3d_attention_backward: null lse");
+        check_heads(*dout, cfg->seqs, cfg->q_rows, cfg->head_dim, cfg->dtype, false);
+        check_heads(*dq, cfg->seqs, cfg->q_rows, cfg->head_dim, cfg->dtype, true);
+        check_heads(*dk, cfg->seqs, cfg->k_rows, cfg->head_dim, cfg->dtype, true);
+        check_heads(*dv, cfg->seqs, cfg->k_rows, cfg->head_dim, cfg->dtype, true);
+        arg_check(dout->heads == q->heads && dq->heads == q->heads && dk->heads == k->heads && dv->heads == k->heads,
+                  "n3d_attention_backward: a gradient has other heads than its tensor");
+        check_workspace(n3d_attention_workspace(cfg, q->heads, k->heads, 1), d_workspace, workspace_bytes);
+        a.dout = view(*dout), a.dq = view(*dq), a.dk = view(*dk), a.dv = view(*dv);
+        a.lse = const_cast<float*>(d_lse);
+        a.row_dot = static_cast<float*>(d_workspace);
+        if (cfg->seqs == 0) return;
+        DeviceGuard g(device);
+        check_record(train_error(device));
+        n3d::launch_attention_backward((cudaStream_t)stream, a, cfg->dtype);
     });
 }
 

@@ -92,6 +92,11 @@ class _ResidualConfig(C.Structure):
                 ("scale", C.c_float), ("rows_per_gate", _sz)]
 
 
+class _AttnConfig(C.Structure):
+    _fields_ = [("seqs", _sz), ("q_rows", _sz), ("k_rows", _sz), ("head_dim", _sz), ("dtype", C.c_int),
+                ("scale", C.c_float), ("left", C.c_longlong), ("right", C.c_longlong), ("q_offset", C.c_longlong)]
+
+
 class _RopeConfig(C.Structure):
     _fields_ = [("head_dim", _sz), ("rotary_dim", _sz), ("layout", C.c_int), ("scaling", C.c_int),
                 ("theta", C.c_double), ("factor", C.c_double), ("original_length", C.c_double),
@@ -209,6 +214,11 @@ def lib() -> C.CDLL:
         "n3d_residual_norm_grad": ([C.c_int, C.POINTER(_ResidualConfig), C.POINTER(_Rows), C.POINTER(_Rows), vp, vp, vp,
                                     vp, C.POINTER(_Rows), C.POINTER(_Rows), C.POINTER(_Rows), C.POINTER(_Rows), vp, vp,
                                     vp, vp, vp, vp, _sz, vp], C.c_int),
+        "n3d_attention_workspace": ([C.POINTER(_AttnConfig), _sz, _sz, C.c_int], _sz),
+        "n3d_attention_forward": ([C.c_int, C.POINTER(_AttnConfig)] + [C.POINTER(_Heads)] * 3 + [vp, vp]
+                                  + [C.POINTER(_Heads), vp, vp, _sz, vp], C.c_int),
+        "n3d_attention_backward": ([C.c_int, C.POINTER(_AttnConfig)] + [C.POINTER(_Heads)] * 4 + [vp, C.POINTER(_Heads)]
+                                   + [vp, vp] + [C.POINTER(_Heads)] * 3 + [vp, _sz, vp], C.c_int),
         "n3d_profile_enable": ([vp, C.c_int], C.c_int),
         "n3d_profile_read": ([vp, C.POINTER(_KernelStats), _sz], _sz),
         "n3d_step_timing_enable": ([vp, C.c_int], C.c_int),
@@ -804,5 +814,49 @@ def residual_norm_grad(block, r, dy, dr, dx, dblock, post: str = "none", pre: st
         dev, C.byref(cfg), _rows(block, sh), _rows(r, sh, dx.dtype), w[0], w[1], _flat(gate, gates, "float32", dev), w[2],
         _rows(dy, sh, block.dtype), _rows(dr, sh, dx.dtype), _rows(dx, sh), _rows(dblock, sh, block.dtype),
         _flat(dgate, gates, "float32", dev), w[3], w[4], w[5], w[6],
+        workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))
+
+
+def _attn_config(q, k, scale, left, right, q_offset) -> _AttnConfig:
+    if len(q.shape) != 4 or len(k.shape) != 4:
+        raise _bad("a [seqs, rows, heads, head_dim] tensor is wanted")
+    return _AttnConfig(q.shape[0], q.shape[1], k.shape[1], q.shape[3], _dtype(q), scale, left, right, q_offset)
+
+
+def attention_workspace(q, k, backward: bool = True) -> int:
+    """Bytes of workspace attention_forward (backward False) or both calls (True) need for tensors like q
+    and k (n3d_attention_workspace)."""
+    cfg = _attn_config(q, k, 0.0, -1, -1, 0)
+    need = [lib().n3d_attention_workspace(C.byref(cfg), q.shape[2], k.shape[2], b) for b in (0, 1)]
+    return max(need) if backward else need[0]
+
+
+def attention_forward(q, k, v, out, lse=None, q_len=None, k_len=None, scale: float = 0.0, left: int = -1,
+                      right: int = -1, q_offset: int = 0, workspace=None, stream: int | None = None) -> None:
+    """Attention of q [seqs, q rows, q heads, head_dim] over k, v [seqs, k rows, k heads, head_dim] into out, with
+    the rows' log-sum-exp in lse [seqs, q heads, q rows] (fp32) for the gradient (n3d_attention_forward).
+    q_len, k_len: int32 [seqs]; left, right: the window around key row i + q_offset, negative for no limit."""
+    cfg, dev = _attn_config(q, k, scale, left, right, q_offset), _device(q)
+    b, nq, hq, hd = q.shape
+    kv = (b, k.shape[1], k.shape[2], hd)
+    _check(lib().n3d_attention_forward(
+        dev, C.byref(cfg), _heads(q), _heads(k, kv, q.dtype), _heads(v, kv, q.dtype), _flat(q_len, b, "int32", dev),
+        _flat(k_len, b, "int32", dev), _heads(out, q.shape, q.dtype), _flat(lse, b * hq * nq, "float32", dev),
+        workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))
+
+
+def attention_backward(q, k, v, out, lse, dout, dq, dk, dv, q_len=None, k_len=None, scale: float = 0.0, left: int = -1,
+                       right: int = -1, q_offset: int = 0, workspace=None, stream: int | None = None) -> None:
+    """The gradient of attention_forward from its out and lse: dout -> dq, dk, dv (n3d_attention_backward).
+    `workspace`: a tensor of at least attention_workspace bytes."""
+    cfg, dev = _attn_config(q, k, scale, left, right, q_offset), _device(q)
+    b, nq, hq, hd = q.shape
+    dt, kv = q.dtype, (b, k.shape[1], k.shape[2], hd)
+    _check(lib().n3d_attention_backward(
+        dev, C.byref(cfg), _heads(q), _heads(k, kv, dt), _heads(v, kv, dt), _heads(out, q.shape, dt),
+        _flat(lse, b * hq * nq, "float32", dev), _heads(dout, q.shape, dt), _flat(q_len, b, "int32", dev),
+        _flat(k_len, b, "int32", dev), _heads(dq, q.shape, dt), _heads(dk, kv, dt), _heads(dv, kv, dt),
         workspace.data_ptr() if workspace is not None else None,
         workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))
