@@ -291,6 +291,7 @@ void launch_dim(cudaStream_t s, const AttnArgs& a, bool backward) {
     a.head_dim == 64 ? launch_modes<T, 64>(s, a, backward) : launch_modes<T, 128>(s, a, backward);
 }
 void launch_type(cudaStream_t s, const AttnArgs& a, int dtype, bool backward) {
+    if (attention_tc_fits(a, dtype, backward)) return launch_attention_train_tc(s, a, dtype, backward);
     if (dtype == N3D_F32)
         launch_dim<float>(s, a, backward);
     else if (dtype == N3D_BF16)

@@ -1,0 +1,707 @@
+// Attention with its gradient on the sm_100a tensor cores (tcgen05, kind::f16) for bf16
+// and fp16 tensors (n3d_attention_forward, _backward); the formulas are those of
+// attention_train.cu, and so are the three passes from one body:
+//   forward  rows = queries, columns = keys:  T1 = q k^T;                  out += P v
+//   dq       rows = queries, columns = keys:  T1 = q k^T, T2 = dout v^T;   dq += dS k
+//   dkv      rows = keys, columns = queries:  T1 = k q^T, T2 = v dout^T;   dk += dS^T q, dv += P^T dout
+//
+// A block owns 128 rows (TMEM lanes, one softmax thread each) and walks blocks of 64
+// columns.  Both operands of T1 and T2 are K-major tiles in shared memory; the weights (P,
+// dS) go back to TMEM as the 16-bit A operand of the second product, over the scores they
+// came from, and its B operand is the same column tile read with the token index as K
+// (MN-major), so no tile is stored twice or transposed.  Nothing of size rows x columns
+// leaves the SM.
+//   warp 0      TMA: the row tiles once, the column tiles through a ring of stages
+//   warp 1      TMEM owner; issues every MMA: T of block g + NBUF once the second product of
+//               block g, which reads the weights in the same columns, has completed
+//   warps 2..   softmax groups of 4 warps, one thread per row; group g % NWG works on block g
+// head_dim 64: one group and two blocks per SM, which interleave (256 TMEM columns each);
+// head_dim 128: one block per SM with two groups on alternating column blocks (forward:
+// each with its own running maximum, sum and accumulator, joined at the end).
+//
+// dq and dkv both recompute T1 and T2: seven products where a kernel that adds dq
+// atomically needs five, but each sum is taken in one accumulator in a fixed order, and
+// no fp32 copy of dq passes through memory.  dq runs first and leaves -lse log2 e and -D
+// of each row for dkv, where they belong to columns and come through the ring.
+//
+// fp16: P is kept times 2^7 (forward, P <= 2^8 there) or 2^10 (dkv), and dS times 2^3 /
+// |dout row| (dq) or over the largest |dout row| of the head group (dkv), as powers of
+// two, so that small weights and gradients keep fp16's precision; |dS| <= 2 P |dout row|
+// |v row| then stays inside fp16 while |v row| < 4096.
+//
+// Rows past a sequence's length: TMA fills what lies past the tensor with zeros, and the
+// MMA warp overwrites what lies past the length with zeros before a tile is used, so
+// nothing that stands there enters a product.  Pairs that the mask hides are cleared by a
+// select.  Every wait is bounded; an expired wait records its site and the block returns.
+// Each barrier is waited for at most one phase behind (argued at the waits).
+
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "n3d_device.cuh"
+#include "train.h"
+#include "train_types.cuh"
+
+namespace n3d {
+
+namespace {
+
+enum Mode { FORWARD, GRAD_Q, GRAD_KV };
+constexpr int ROWS = 128, COLS = 64;
+constexpr int BOX = 64 * 128;  // a TMA box: 64 rows of 64 elements
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float RESCALE_LOG2 = 8.0f;  // forward: raise the running maximum when exponents would exceed 2^8
+constexpr int DEV_TIMEOUT_ATTN_TRAIN = 7;
+
+template <int HD, int MODE>
+struct Cfg {
+    static constexpr bool GRAD = MODE != FORWARD;
+    static constexpr int NWG = HD == 64 ? 1 : 2;                          // softmax groups
+    static constexpr int NBUF = HD == 64 && GRAD ? 1 : 2;                 // score buffers, a multiple of NWG
+    static constexpr int THREADS = 64 + 128 * NWG, PER_SM = HD == 64 ? 2 : 1;
+    static constexpr int RTILE = ROWS * HD * 2, CTILE = COLS * HD * 2;    // bytes
+    static constexpr int STATS = MODE == GRAD_KV ? 512 : 0;               // 64 x (-lse log2 e), 64 x (-D)
+    static constexpr int STAGE = 2 * CTILE + 1024 * (STATS > 0), NST = 4;
+    static constexpr int ROW_BYTES = (GRAD ? 2 : 1) * RTILE;
+    // barriers and the TMEM slot, the groups' row statistics, and slack to align the tiles to 1024 bytes
+    static constexpr int SMEM = ROW_BYTES + NST * STAGE + 256 + (NWG > 1 ? 4 * 128 * 4 : 64) + 1024;
+    static constexpr uint32_t TBUF = GRAD ? 128 : 64;                     // TMEM columns of a score buffer
+    static constexpr uint32_t ACC = NBUF * TBUF;                          // first accumulator
+    static constexpr int NACC = MODE == FORWARD ? NWG : MODE == GRAD_Q ? 1 : 2;
+    static constexpr uint32_t TMEM_COLS = HD == 64 ? 256 : 512;
+    static_assert(ACC + NACC * HD <= TMEM_COLS, "TMEM");
+    static_assert(NBUF % NWG == 0, "a score buffer belongs to one softmax group");
+    static_assert(SMEM * PER_SM <= 227 * 1024, "shared memory");
+};
+
+// Instruction descriptor of kind::f16 with fp32 accumulators, M = 128; B K-major, or
+// MN-major (token index as K); A negated for a negative score scale.
+template <class T>
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn, bool negate_a = false) {
+    const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(negate_a) << 13) |
+           (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// Descriptor of an MN-major B tile: boxes of 64 d-elements (128-byte swizzled rows, one
+// row per token); 8-token groups 1024 B apart (SBO), boxes BOX apart (LBO).
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(BOX >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int d, int row, int head,
+                                            int seq) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+            "r"(smem_u32(dst)),
+        "l"(map), "r"(smem_u32(bar)), "r"(d), "r"(row), "r"(head), "r"(seq)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int d, int row, int head,
+                                             int seq) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(map),
+                 "r"(d), "r"(row), "r"(head), "r"(seq), "r"(smem_u32(src))
+                 : "memory");
+}
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned).
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, int bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 16 TMEM columns of this thread's lane from 32-bit words; completes with tmem_wait_st().
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^-floor(log2 x) for a positive normal x, 1 otherwise
+__device__ __forceinline__ float inverse_power(float x) {
+    const int e = (__float_as_int(x) >> 23) & 255;
+    return x > 0.0f && e > 0 && e < 254 ? __int_as_float((254 - e) << 23) : 1.0f;
+}
+
+struct TcMaps {
+    CUtensorMap q, k, v, dout;       // loads, 64-row boxes
+    CUtensorMap out, dq, dk, dv;     // stores, 32-row boxes
+};
+struct TcArgs {
+    AttnArgs a;
+    int tiles;         // row tiles of a head
+    float k2, factor;  // |scale| log2 e; the scale of dq and dk
+    int negate;        // scale < 0
+    float* stats;      // [seqs * q_heads][q tiles][2][-lse log2 e: 64 | -D: 64]
+    float* norms;      // [seqs * q_heads][q tiles]: the largest |dout row|
+    int q_tiles;
+};
+
+template <class T, int HD, int MODE>
+__global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
+    attention_train_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs args) {
+    using C = Cfg<HD, MODE>;
+    constexpr bool F16 = std::is_same<T, __half>::value;
+    constexpr int NWG = C::NWG, NBUF = C::NBUF, NST = C::NST;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* rows1 = smem;              // q, q, k: HD / 64 boxes of [128 rows x 128 B]
+    uint8_t* rows2 = smem + C::RTILE;   // -, dout, v
+    uint8_t* ring = smem + C::ROW_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NST * C::STAGE);
+    uint64_t* r_full = bars;               // 1: the row tiles landed
+    uint64_t* c_full = bars + 1;           // NST: the column tiles of block g landed (stage g % NST)
+    uint64_t* c_empty = c_full + NST;      // NST: block g's second product completed
+    uint64_t* t_full = c_empty + NST;      // NBUF: T of block g completed (buffer g % NBUF)
+    uint64_t* p_full = t_full + NBUF;      // NBUF: weights of block g written (4 warps)
+    uint64_t* acc_done = p_full + NBUF;    // NBUF: second product of block g completed
+    uint64_t* all_done = acc_done + NBUF;  // 1: the last one completed
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+    float* join = reinterpret_cast<float*>(bars + 32);  // forward with two groups: [2][128] maxima; then sums
+    static_assert(1 + 2 * NST + 3 * NBUF + 2 <= 32, "barriers and the TMEM slot fill at most 256 bytes");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0 && lane == 0) {
+        mbar_init(r_full, 1);
+        for (int i = 0; i < NST; i++) mbar_init(&c_full[i], 1), mbar_init(&c_empty[i], 1);
+        for (int i = 0; i < NBUF; i++) mbar_init(&t_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&acc_done[i], 1);
+        mbar_init(all_done, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    griddep_wait();
+    griddep_launch_dependents();
+
+    // ---- this block's rows and the column blocks they see
+    const AttnArgs& a = args.a;
+    int* const err = a.err;
+    const int heads = MODE == GRAD_KV ? a.k_heads : a.q_heads, group = a.q_heads / a.k_heads;
+    const int sh = blockIdx.x / args.tiles, head = sh % heads, seq = sh / heads;
+    const int order = blockIdx.x - sh * args.tiles;
+    // queries: the last tiles see the most keys of a causal mask, so they go first
+    const int r0 = (MODE == GRAD_KV ? order : args.tiles - 1 - order) * ROWS;
+    const AttnMask mask(a, seq);
+    const int row_len = MODE == GRAD_KV ? mask.k_len : mask.q_len, col_len = MODE == GRAD_KV ? mask.q_len : mask.k_len;
+    const int row_cap = MODE == GRAD_KV ? a.k_rows : a.q_rows, col_cap = MODE == GRAD_KV ? a.q_rows : a.k_rows;
+    auto first_col = [&](int r) { return MODE == GRAD_KV ? mask.first_query(r) : mask.first_key(r); };
+    auto last_col = [&](int r) { return MODE == GRAD_KV ? mask.last_query(r) : mask.last_key(r); };
+    const int r_last = min(r0 + ROWS, row_len) - 1;
+    int c_begin = 0, per_head = 0;  // first column block, blocks of one column head
+    if (r_last >= r0) {
+        const int lo = first_col(r0), hi = last_col(r_last);
+        if (hi > lo) c_begin = lo / COLS, per_head = (hi + COLS - 1) / COLS - c_begin;
+    }
+    const int nblk = per_head * (MODE == GRAD_KV ? group : 1);
+    auto col0 = [&](int g) { return (c_begin + (MODE == GRAD_KV ? g % per_head : g)) * COLS; };
+    auto col_head = [&](int g) { return MODE == GRAD_KV ? head * group + g / per_head : head / group; };
+
+    if (warp == 0) {
+        if (lane == 0 && nblk > 0) {
+            const CUtensorMap* rm1 = MODE == GRAD_KV ? &maps.k : &maps.q;
+            const CUtensorMap* rm2 = MODE == GRAD_KV ? &maps.v : &maps.dout;
+            const CUtensorMap* cm1 = MODE == GRAD_KV ? &maps.q : &maps.k;
+            const CUtensorMap* cm2 = MODE == GRAD_KV ? &maps.dout : &maps.v;
+            mbar_arrive_expect_tx(r_full, C::ROW_BYTES);
+#pragma unroll
+            for (int i = 0; i < HD / 64; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {  // 64 rows each
+                    const int o = (2 * i + h) * BOX;
+                    tma_load_4d(rows1 + o, rm1, r_full, 64 * i, r0 + 64 * h, head, seq);
+                    if (C::GRAD) tma_load_4d(rows2 + o, rm2, r_full, 64 * i, r0 + 64 * h, head, seq);
+                }
+            int g = 0;
+            for (; g < nblk; g++) {
+                // the stage's previous block (phase g / NST - 1; the one after it needs this load)
+                if (g >= NST && !mbar_wait(&c_empty[g % NST], (g / NST - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN)) break;
+                uint8_t* st = ring + (g % NST) * C::STAGE;
+                uint64_t* bar = &c_full[g % NST];
+                const int c0 = col0(g), ch = col_head(g);
+                mbar_arrive_expect_tx(bar, 2 * C::CTILE + C::STATS);
+#pragma unroll
+                for (int i = 0; i < HD / 64; i++) {
+                    tma_load_4d(st + i * BOX, cm1, bar, 64 * i, c0, ch, seq);
+                    tma_load_4d(st + C::CTILE + i * BOX, cm2, bar, 64 * i, c0, ch, seq);
+                }
+                if (MODE == GRAD_KV)
+                    bulk_load(st + 2 * C::CTILE,
+                              args.stats + (((long long)seq * a.q_heads + ch) * args.q_tiles * 2 + c0 / COLS) * 128,
+                              C::STATS, bar);
+            }
+            // every load has landed before the block may exit (already true unless a wait expired)
+            mbar_wait(r_full, 0, err, DEV_TIMEOUT_ATTN_TRAIN);
+            for (int x = max(0, g - NST); x < g; x++)
+                mbar_wait(&c_full[x % NST], (x / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN);
+        }
+    } else if (warp == 1) {
+        // zeros over rows [from, n) of a tile (boxes of `box_rows` rows)
+        auto clear = [&](uint8_t* tile, int from, int n) {
+            for (int i = 0; i < HD / 64; i++)
+                for (int x = from * 8 + lane; x < n * 8; x += 32)
+                    *reinterpret_cast<uint4*>(tile + i * n * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+        };
+        const uint32_t t_desc = idesc<T>(COLS, false, false), t_neg = idesc<T>(COLS, false, true);
+        constexpr uint32_t acc_desc = idesc<T>(HD, true);
+        bool ok = nblk > 0;
+        if (ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait(r_full, 0, err, DEV_TIMEOUT_ATTN_TRAIN));
+            if (ok && r0 + ROWS > row_len && row_len < row_cap) {
+                clear(rows1, max(row_len - r0, 0), ROWS);
+                if (C::GRAD) clear(rows2, max(row_len - r0, 0), ROWS);
+                fence_async_smem();
+                __syncwarp();
+            }
+        }
+        auto issue_t = [&](int g) {
+            // the column tiles of block g (phase g / NST; the next needs this block's second product)
+            ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            if (!ok) return;
+            uint8_t* st = ring + (g % NST) * C::STAGE;
+            const int c0 = col0(g);
+            if (c0 + COLS > col_len && col_len < col_cap) {
+                clear(st, col_len - c0, COLS);
+                clear(st + C::CTILE, col_len - c0, COLS);
+                fence_async_smem();
+                __syncwarp();
+            }
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
+                const uint32_t t = tmem + (g % NBUF) * C::TBUF;
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; kk++) {
+                    const uint32_t ro = (kk / 4) * 2 * BOX + (kk % 4) * 32, co = (kk / 4) * BOX + (kk % 4) * 32;
+                    umma_f16(t, desc_k_sw128(r1 + ro), desc_k_sw128(b + co), args.negate ? t_neg : t_desc, kk != 0);
+                }
+                if (C::GRAD) {
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; kk++) {
+                        const uint32_t ro = (kk / 4) * 2 * BOX + (kk % 4) * 32, co = (kk / 4) * BOX + (kk % 4) * 32;
+                        umma_f16(t + 64, desc_k_sw128(r2 + ro), desc_k_sw128(b + C::CTILE + co), t_desc, kk != 0);
+                    }
+                }
+                umma_commit(&t_full[g % NBUF]);
+            }
+            __syncwarp();
+        };
+        for (int g = 0; ok && g < min(NBUF, nblk); g++) issue_t(g);
+        for (int g = 0; ok && g < nblk; g++) {
+            // the weights of block g (phase g / NBUF; the next needs T of block g + NBUF, issued below)
+            ok = __all_sync(0xffffffffu, mbar_wait(&p_full[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t b = smem_u32(ring + (g % NST) * C::STAGE);
+                const uint32_t t = tmem + (g % NBUF) * C::TBUF;
+                // forward: P v (tile 2); gradients: dS k or dS^T q (tile 1), and P^T dout (tile 2)
+                const uint32_t acc = tmem + C::ACC + (MODE == FORWARD ? (g % NWG) * HD : 0);
+                const uint32_t first = MODE == FORWARD ? g < NWG : g == 0;
+#pragma unroll
+                for (int kk = 0; kk < COLS / 16; kk++)
+                    umma_f16_ts(acc, t + (C::GRAD ? 64 : 0) + 8 * kk,
+                                desc_mn_sw128(b + (MODE == FORWARD ? C::CTILE : 0) + kk * 2048), acc_desc,
+                                kk != 0 || !first);
+                if (MODE == GRAD_KV) {
+#pragma unroll
+                    for (int kk = 0; kk < COLS / 16; kk++)
+                        umma_f16_ts(acc + HD, t + 8 * kk, desc_mn_sw128(b + C::CTILE + kk * 2048), acc_desc,
+                                    kk != 0 || !first);
+                }
+                umma_commit(&acc_done[g % NBUF]);
+                umma_commit(&c_empty[g % NST]);
+                if (g == nblk - 1) umma_commit(all_done);
+            }
+            __syncwarp();
+            if (g + NBUF < nblk) {
+                // T of block g + NBUF overwrites the weights of block g (phase g / NBUF; the next
+                // needs that T)
+                ok = __all_sync(0xffffffffu,
+                                mbar_wait(&acc_done[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                if (ok) issue_t(g + NBUF);
+            }
+        }
+    } else {
+        // ---- softmax: group wg, TMEM lane quadrant warp % 4, one row per thread
+        const int wg = (warp - 2) / 4, qd = warp & 3, r = qd * 32 + lane, row = r0 + r;
+        const uint32_t lb = tmem + (static_cast<uint32_t>(qd * 32) << 16);
+        const bool live = row < row_len;
+        const int lo = first_col(row), hi = last_col(row);
+        const int full_lo = r_last >= r0 ? first_col(r_last) : 0, full_hi = r_last >= r0 ? last_col(r0) : 0;
+        const float k2 = args.k2;
+        bool ok = true;
+
+        // dq: this row's -lse log2 e, -D and fp16 scale; dkv: the fp16 scale of the head group
+        float nlse = 0.0f, ndot = 0.0f, ds_scale = 1.0f;
+        if (MODE == GRAD_Q) {
+            const long long sqh = (long long)seq * a.q_heads + head;
+            float norm2 = 0.0f;
+            nlse = -INFINITY;
+            if (live) {
+                const T* o = static_cast<const T*>(a.o.p) + seq * a.o.seq + head * a.o.head + (long long)row * a.o.row;
+                const T* d =
+                    static_cast<const T*>(a.dout.p) + seq * a.dout.seq + head * a.dout.head + (long long)row * a.dout.row;
+                float dot = 0.0f;
+#pragma unroll 4
+                for (int c = 0; c < HD; c += 8) {
+                    Vec<T, 8> vo, vd;
+                    vo.load(o + c);
+                    vd.load(d + c);
+                    float x[8], y[8];
+                    vo.get(x);
+                    vd.get(y);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) dot += x[i] * y[i], norm2 += y[i] * y[i];
+                }
+                ndot = -dot;
+                const float l = a.lse[sqh * a.q_rows + row];
+                if (l != -INFINITY) nlse = -l * LOG2E;
+            }
+            const float norm = sqrtf(norm2);
+            if (F16) ds_scale = 8.0f * inverse_power(norm);
+            if (wg == 0) {
+                float* st = args.stats + ((sqh * args.q_tiles + r0 / ROWS) * 2 + r / 64) * 128 + r % 64;
+                st[0] = nlse;
+                st[64] = ndot;
+                if (F16) {
+                    float m = norm;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    if (lane == 0) join[qd] = m;
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    if (r == 0)
+                        args.norms[sqh * args.q_tiles + r0 / ROWS] = fmaxf(fmaxf(join[0], join[1]), fmaxf(join[2], join[3]));
+                }
+            }
+        }
+        if (MODE == GRAD_KV && F16) {
+            float m = 0.0f;
+            const float* n = args.norms + ((long long)seq * a.q_heads + head * group) * args.q_tiles;
+            for (int i = lane; i < group * args.q_tiles; i += 32) m = fmaxf(m, n[i]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            ds_scale = 8.0f * inverse_power(m);
+        }
+        constexpr float P_LOG2 = !F16 ? 0.0f : MODE == FORWARD ? 7.0f : MODE == GRAD_KV ? 10.0f : 0.0f;
+
+        float m = -INFINITY, l = 0.0f;  // forward: running maximum (raw scores) and sum (times 2^P_LOG2)
+        for (int g = wg; g < nblk; g += NWG) {
+            const int buf = g % NBUF, c0 = col0(g);
+            const uint32_t t = lb + buf * C::TBUF;
+            const bool full = c0 >= full_lo && c0 + COLS <= full_hi;
+            // T of block g (phase g / NBUF of its buffer: the next needs this block's weights).  After an
+            // expired wait the loop keeps running (results unused).
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(&t_full[buf], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            tc_fence_after();
+            if constexpr (MODE == FORWARD) {
+                float s[64];
+                tmem_ld32(t, s);
+                tmem_ld32(t + 32, s + 32);
+                if (!full) {
+#pragma unroll
+                    for (int c = 0; c < 64; c++)
+                        if (c0 + c < lo || c0 + c >= hi) s[c] = -INFINITY;
+                }
+                float mx[8];
+#pragma unroll
+                for (int c = 0; c < 8; c++) mx[c] = fmaxf(s[c], s[c + 8]);
+#pragma unroll
+                for (int c = 16; c < 64; c += 16)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) mx[i] = max3f(mx[i], s[c + i], s[c + 8 + i]);
+                const float mb = max3f(max3f(mx[0], mx[1], mx[2]), max3f(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+                // (an unseen block leaves mb = -inf: no raise, and the exponents below stay -inf)
+                const bool raise = mb > m && (mb - m) * k2 > RESCALE_LOG2;
+                const float corr = raise ? ex2_approx((m - mb) * k2) : 1.0f;  // 0 from m = -inf
+                if (raise) m = mb;
+                const float off = m == -INFINITY ? 0.0f : P_LOG2 - m * k2;
+                const uint64_t k22 = pack2(k2, k2), off2 = pack2(off, off);
+                uint64_t sum2[4] = {0, 0, 0, 0};
+                uint32_t w[32];
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    float x, y;
+                    unpack2(fma2(pack2(s[c], s[c + 1]), k22, off2), x, y);
+                    x = ex2_approx(x);
+                    y = ex2_approx(y);
+                    sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], pack2(x, y));
+                    w[c / 2] = pack_pair<T>(x, y);
+                }
+                float sa, sb;
+                unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sa, sb);
+                l = l * corr + (sa + sb);
+                if (g >= NWG && __any_sync(0xffffffffu, raise)) {
+                    // this group's previous product (its phase: the buffer's next product needs P of
+                    // this or a later block of the group)
+                    ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_done[(g - NWG) % NBUF], ((g - NWG) / NBUF) & 1, err,
+                                                                 DEV_TIMEOUT_ATTN_TRAIN));
+                    tc_fence_after();
+                    const uint32_t acc = lb + C::ACC + wg * HD;
+                    const uint64_t c2 = pack2(corr, corr);
+#pragma unroll 1
+                    for (int cb = 0; cb < HD; cb += 16) {
+                        float o[16];
+                        uint32_t u[16];
+                        tmem_ld16(acc + cb, o);
+#pragma unroll
+                        for (int d = 0; d < 16; d += 2) {
+                            unpack2(mul2(pack2(o[d], o[d + 1]), c2), o[d], o[d + 1]);
+                            u[d] = __float_as_uint(o[d]), u[d + 1] = __float_as_uint(o[d + 1]);
+                        }
+                        tmem_st16(acc + cb, u);
+                    }
+                }
+                tmem_st16(t, w);
+                tmem_st16(t + 16, w + 16);
+            } else {
+                const float4* st = reinterpret_cast<const float4*>(ring + (g % NST) * C::STAGE + 2 * C::CTILE);
+                const uint64_t k22 = pack2(k2, k2);
+                if (MODE == GRAD_KV)  // the statistics came by bulk copy: this thread's own wait makes them visible
+                    ok = __all_sync(0xffffffffu,
+                                    ok && mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+#pragma unroll
+                for (int h = 0; h < 2; h++) {  // 32 columns: weights h go over scores that are read already
+                    float s[32], u[32];
+                    tmem_ld32(t + 32 * h, s);
+                    tmem_ld32(t + 64 + 32 * h, u);
+                    uint32_t pw[16], dw[16];
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
+                        if (MODE == GRAD_KV) {
+                            nl = st[8 * h + c / 4];
+                            nd = st[16 + 8 * h + c / 4];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const uint64_t n2 = e == 0 ? pack2(nl.x, nl.y) : pack2(nl.z, nl.w);
+                            const uint64_t d2 = e == 0 ? pack2(nd.x, nd.y) : pack2(nd.z, nd.w);
+                            float x, y;
+                            unpack2(fma2(pack2(s[c + e], s[c + e + 1]), k22, n2), x, y);
+                            if (!full) {
+                                const int cc = c0 + 32 * h + c + e;
+                                if (cc < lo || cc >= hi) x = -INFINITY;
+                                if (cc + 1 < lo || cc + 1 >= hi) y = -INFINITY;
+                            }
+                            const bool sx = x != -INFINITY, sy = y != -INFINITY;
+                            x = ex2_approx(x);
+                            y = ex2_approx(y);
+                            uint64_t p2 = pack2(x, y);
+                            if (F16 && MODE == GRAD_Q) p2 = mul2(p2, pack2(ds_scale, ds_scale));
+                            uint64_t g2 = mul2(p2, add2(pack2(u[c + e], u[c + e + 1]), d2));
+                            if (F16 && MODE == GRAD_KV) {
+                                g2 = mul2(g2, pack2(ds_scale, ds_scale));
+                                x *= 1024.0f;
+                                y *= 1024.0f;
+                            }
+                            float gx, gy;
+                            unpack2(g2, gx, gy);
+                            if (!full) {
+                                if (!sx) gx = 0.0f;
+                                if (!sy) gy = 0.0f;
+                            }
+                            if (MODE == GRAD_KV) pw[(c + e) / 2] = pack_pair<T>(x, y);
+                            dw[(c + e) / 2] = pack_pair<T>(gx, gy);
+                        }
+                    }
+                    if (MODE == GRAD_KV) tmem_st16(t + 16 * h, pw);
+                    tmem_st16(t + 64 + 16 * h, dw);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[buf]);
+        }
+
+        // ---- the accumulators, once every product has completed
+        if (nblk > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(all_done, 0, err, DEV_TIMEOUT_ATTN_TRAIN));
+        tc_fence_after();
+        float f0 = 0.0f, f1 = 0.0f;  // what the accumulator(s) are multiplied by
+        if (MODE == FORWARD) {
+            float lse;
+            if (NWG == 1) {
+                f0 = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN;
+                lse = l == 0.0f ? -INFINITY : (m * k2 + log2f(l) - P_LOG2) * LN2;
+            } else {
+                join[wg * 128 + r] = m;
+                join[256 + wg * 128 + r] = l;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float m0 = join[r], m1 = join[128 + r], l0 = join[256 + r], l1 = join[256 + 128 + r];
+                const float mm = fmaxf(m0, m1);
+                // a group that saw nothing has m = -inf and l = 0
+                const float e0 = l0 == 0.0f ? 0.0f : ex2_approx((m0 - mm) * k2);
+                const float e1 = l1 == 0.0f ? 0.0f : ex2_approx((m1 - mm) * k2);
+                const float sum = l0 * e0 + l1 * e1;
+                const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : NAN;
+                f0 = e0 * inv;
+                f1 = nblk > 1 ? e1 * inv : 0.0f;
+                lse = sum == 0.0f ? -INFINITY : (mm * k2 + log2f(sum) - P_LOG2) * LN2;
+            }
+            if (a.lse && wg == 0 && row < a.q_rows)
+                a.lse[((long long)seq * a.q_heads + head) * a.q_rows + row] = live ? lse : -INFINITY;
+        } else {
+            f0 = args.factor;
+            if (F16) f0 /= ds_scale;
+        }
+        // 64 columns of one accumulator (plus those of a second one) to a row's 128 bytes of staging
+        auto stage_box = [&](uint32_t acc, float f, uint32_t acc2, float g2, uint8_t* box) {
+#pragma unroll 1
+            for (int cb = 0; cb < 64; cb += 16) {
+                float o[16], o2[16];
+                if (nblk > 0) tmem_ld16(acc + cb, o);
+                if (acc2 && nblk > 1) tmem_ld16(acc2 + cb, o2);
+                uint32_t w[8];
+#pragma unroll
+                for (int d = 0; d < 16; d += 2) {
+                    float x = 0.0f, y = 0.0f;
+                    if (live && nblk > 0) {
+                        x = o[d] * f, y = o[d + 1] * f;
+                        if (acc2 && nblk > 1) x += o2[d] * g2, y += o2[d + 1] * g2;
+                    }
+                    w[d / 2] = pack_pair<T>(x, y);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    *reinterpret_cast<uint4*>(box + r * 128 + (((cb / 8 + i) ^ (r & 7)) << 4)) =
+                        make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            }
+        };
+        auto send_box = [&](const CUtensorMap* map, uint8_t* box, int d) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && r0 + qd * 32 < row_cap) {
+                tma_store_4d(map, box + qd * 32 * 128, d, r0 + qd * 32, head, seq);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        };
+        // the row tiles are no longer read: they hold the staging, a box of 128 rows each
+        const uint32_t acc = lb + C::ACC;
+        if constexpr (MODE == FORWARD) {
+            if (NWG == 1) {
+                stage_box(acc, f0, 0, 0.0f, rows1);
+                send_box(&maps.out, rows1, 0);
+            } else {
+                stage_box(acc + 64 * wg, f0, acc + HD + 64 * wg, f1, rows1 + wg * ROWS * 128);
+                send_box(&maps.out, rows1 + wg * ROWS * 128, 64 * wg);
+            }
+        } else if constexpr (MODE == GRAD_Q) {
+            stage_box(acc + 64 * wg, f0, 0, 0.0f, rows1 + wg * ROWS * 128);
+            send_box(&maps.dq, rows1 + wg * ROWS * 128, 64 * wg);
+        } else {
+            const float fv = F16 ? 1.0f / 1024.0f : 1.0f;
+            if (NWG == 1 || wg == 0) {
+#pragma unroll 1
+                for (int i = 0; i < HD / 64; i++) {
+                    stage_box(acc + 64 * i, f0, 0, 0.0f, rows1 + i * ROWS * 128);
+                    send_box(&maps.dk, rows1 + i * ROWS * 128, 64 * i);
+                }
+            }
+            if (NWG == 1 || wg == 1) {
+#pragma unroll 1
+                for (int i = 0; i < HD / 64; i++) {
+                    stage_box(acc + HD + 64 * i, fv, 0, 0.0f, rows2 + i * ROWS * 128);
+                    send_box(&maps.dv, rows2 + i * ROWS * 128, 64 * i);
+                }
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // staging read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
+}
+
+template <class T, int HD, int MODE>
+void launch(cudaStream_t s, const AttnArgs& a) {
+    using C = Cfg<HD, MODE>;
+    static std::atomic<unsigned long long> attr{0};
+    once_per_device(attr, [] {
+        N3D_CUDA(cudaFuncSetAttribute(attention_train_tc_kernel<T, HD, MODE>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    });
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    const int rows = MODE == GRAD_KV ? a.k_rows : a.q_rows, heads = MODE == GRAD_KV ? a.k_heads : a.q_heads;
+    TcArgs t{};
+    t.a = a;
+    t.tiles = (rows + ROWS - 1) / ROWS;
+    const long long blocks = (long long)t.tiles * heads * a.seqs;
+    if (blocks > INT_MAX) throw Error(13, "attention: more than 2^31 tiles");
+    if (blocks == 0) return;
+    auto map = [&](const HeadsView& v, int n, int h, int box) {
+        return make_heads_map(v.p, bf16, a.seqs, n, h, HD, v.seq, v.row, v.head, box);
+    };
+    TcMaps m{};
+    // a tensor without rows is never loaded: any valid map stands in for its own
+    const HeadsView& any = MODE == GRAD_KV ? a.k : a.q;
+    const CUtensorMap stand_in = map(any, rows, heads, 64);
+    m.q = a.q_rows ? map(a.q, a.q_rows, a.q_heads, 64) : stand_in;
+    m.k = a.k_rows ? map(a.k, a.k_rows, a.k_heads, 64) : stand_in;
+    m.v = a.k_rows ? map(a.v, a.k_rows, a.k_heads, 64) : stand_in;
+    if (MODE != FORWARD) m.dout = a.q_rows ? map(a.dout, a.q_rows, a.q_heads, 64) : stand_in;
+    if (MODE == FORWARD) m.out = map(a.o, a.q_rows, a.q_heads, 32);
+    if (MODE == GRAD_Q) m.dq = map(a.dq, a.q_rows, a.q_heads, 32);
+    if (MODE == GRAD_KV) {
+        m.dk = map(a.dk, a.k_rows, a.k_heads, 32);
+        m.dv = map(a.dv, a.k_rows, a.k_heads, 32);
+    }
+    t.k2 = fabsf(a.scale) * LOG2E;
+    t.factor = a.scale;
+    t.negate = a.scale < 0.0f;
+    t.q_tiles = (a.q_rows + ROWS - 1) / ROWS;
+    t.stats = a.row_dot;
+    t.norms = a.row_dot + (size_t)a.seqs * a.q_heads * t.q_tiles * 256;
+    launch_pdl(attention_train_tc_kernel<T, HD, MODE>, dim3((unsigned)blocks), dim3(C::THREADS), C::SMEM, s, m, t);
+}
+
+template <class T, int HD>
+void launch_modes(cudaStream_t s, const AttnArgs& a, bool backward) {
+    if (!backward) return launch<T, HD, FORWARD>(s, a);
+    launch<T, HD, GRAD_Q>(s, a);
+    launch<T, HD, GRAD_KV>(s, a);
+}
+template <class T>
+void launch_dim(cudaStream_t s, const AttnArgs& a, bool backward) {
+    a.head_dim == 64 ? launch_modes<T, 64>(s, a, backward) : launch_modes<T, 128>(s, a, backward);
+}
+
+// Whole 16-byte words, and strides that a tensor map can hold (above 0, below 2^40 bytes).
+bool tma_view(const HeadsView& v, long long seqs, long long rows, long long heads) {
+    if (rows == 0) return true;
+    auto fits = [](long long st, long long n) { return n <= 1 || (st > 0 && st % 8 == 0 && st < (1LL << 39)); };
+    return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && fits(v.seq, seqs) && fits(v.row, rows) && fits(v.head, heads);
+}
+
+}  // namespace
+
+bool attention_tc_fits(const AttnArgs& a, int dtype, bool backward) {
+    if (dtype == N3D_F32) return false;
+    auto q_side = [&](const HeadsView& v) { return tma_view(v, a.seqs, a.q_rows, a.q_heads); };
+    auto k_side = [&](const HeadsView& v) { return tma_view(v, a.seqs, a.k_rows, a.k_heads); };
+    const bool f = q_side(a.q) && q_side(a.o) && k_side(a.k) && k_side(a.v);
+    return f && (!backward || (q_side(a.dout) && q_side(a.dq) && k_side(a.dk) && k_side(a.dv)));
+}
+
+void launch_attention_train_tc(cudaStream_t s, const AttnArgs& a, int dtype, bool backward) {
+    dtype == N3D_BF16 ? launch_dim<__nv_bfloat16>(s, a, backward) : launch_dim<__half>(s, a, backward);
+}
+
+}  // namespace n3d

@@ -956,6 +956,24 @@ CUtensorMap make_f16_map(const void* p, long long rows, long long cols, long lon
     return cached_map(p, MAP_F16, rows, cols, ld, box_cols, box_rows, swizzle);
 }
 
+CUtensorMap make_heads_map(const void* p, bool bf16, long long seqs, long long rows, long long heads, int hd,
+                           long long seq_stride, long long row_stride, long long head_stride, int box_rows) {
+    CUtensorMap m;
+    const long long n[3] = {rows, heads, seqs}, st[3] = {row_stride, head_stride, seq_stride};
+    cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd)}, strides[3];
+    for (int i = 0; i < 3; i++) {
+        dims[i + 1] = static_cast<cuuint64_t>(n[i]);
+        strides[i] = static_cast<cuuint64_t>(n[i] > 1 ? st[i] : hd) * 2;  // the stride of a single index is not used
+    }
+    cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
+    CUresult r = encode_fn()(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                             const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw Error(9, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+    return m;
+}
+
 // A plain fp32 output (EPI_STORE without a reduce) whose rows start on 16-byte
 // boundaries leaves through the TMA epilogue: 32 x 32 boxes staged in shared memory,
 // instead of each thread writing its own row.  The values are the same either way.

@@ -157,6 +157,12 @@ CUtensorMap make_store_map_f16(const void* p, long long rows, long long cols, lo
 CUtensorMap make_f16_map(const void* p, long long rows, long long cols, long long ld, int box_cols, int box_rows,
                          bool swizzle);
 
+// 4-D map over a bf16 or fp16 tensor [seqs, rows, heads, hd] (strides in elements, whole
+// 16-byte words; p 16-byte aligned): coordinates (d, row, head, seq), box 64 x box_rows x
+// 1 x 1 with the 128-byte swizzle.  Rows past the end read zeros and are not stored.
+CUtensorMap make_heads_map(const void* p, bool bf16, long long seqs, long long rows, long long heads, int hd,
+                           long long seq_stride, long long row_stride, long long head_stride, int box_rows);
+
 // C[M, N] = A[M, K] * B[N, K]^T with the fp16 split on tcgen05 (gemm.cu).  K % 32 == 0
 // (k-blocks of 64; a last half block reads zeros past K).  `kb_per_tap` > 0 turns on
 // the shifted-row (implicit k=3 conv) mode: k-block kb (of 64) reads A at column

@@ -65,7 +65,8 @@ void launch_residual_norm_grad(cudaStream_t s, const ResidualArgs& a, int residu
 struct AttnArgs {
     HeadsView q, k, v, o, dout, dq, dk, dv;
     float* lse;         // [seqs, q_heads, q_rows], null: not wanted (forward)
-    float* row_dot;     // workspace [seqs, q_heads, q_rows]: dout . out
+    float* row_dot;     // workspace of attn_workspace_floats(): row statistics of the gradient
+    int* err;           // where an expired wait records its site
     int seqs, q_rows, k_rows, q_heads, k_heads, head_dim;
     float scale;
     int left, right, offset;      // kNoLimit where unlimited
@@ -99,6 +100,16 @@ struct AttnMask {
     }
 #endif
 };
+// Workspace of the gradient: on the fp32 units dout . out of each row; on the tensor cores
+// two blocks of 128 floats for every 128 query rows of a head (row statistics of 64 rows
+// each) and one float (the largest |dout row| of the 128).
+inline size_t attn_workspace_floats(size_t seqs, size_t q_heads, size_t q_rows) {
+    return seqs * q_heads * ((q_rows + 127) / 128) * (2 * 128 + 1);
+}
+// attention_train_tc.cu: whether the call's tensors fit TMA (16-bit types, whole 16-byte
+// words, no broadcast dimension), and the launches.
+bool attention_tc_fits(const AttnArgs& a, int dtype, bool backward);
+void launch_attention_train_tc(cudaStream_t s, const AttnArgs& a, int dtype, bool backward);
 void launch_attention_forward(cudaStream_t s, const AttnArgs& a, int dtype);
 void launch_attention_backward(cudaStream_t s, const AttnArgs& a, int dtype);
 

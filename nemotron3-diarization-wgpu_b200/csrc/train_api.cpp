@@ -393,7 +393,7 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config* cfg, co
 size_t n3d_attention_workspace(const n3d_attn_config* cfg, size_t q_heads, size_t k_heads, int backward) {
     if (!cfg || q_heads > 65535 || k_heads > 65535 || cfg->seqs > (size_t)INT_MAX || cfg->q_rows > (size_t)1 << 30)
         return 0;
-    return backward ? cfg->seqs * q_heads * cfg->q_rows * sizeof(float) : 0;
+    return backward ? n3d::attn_workspace_floats(cfg->seqs, q_heads, cfg->q_rows) * sizeof(float) : 0;
 }
 
 n3d_status n3d_attention_forward(int device, const n3d_attn_config* cfg, const n3d_heads* q, const n3d_heads* k,
@@ -407,7 +407,8 @@ n3d_status n3d_attention_forward(int device, const n3d_attn_config* cfg, const n
         a.lse = d_lse;
         if (cfg->seqs == 0 || cfg->q_rows == 0) return;
         DeviceGuard g(device);
-        check_record(train_error(device));
+        a.err = train_error(device);
+        check_record(a.err);
         n3d::launch_attention_forward((cudaStream_t)stream, a, cfg->dtype);
     });
 }
@@ -434,7 +435,8 @@ n3d_status n3d_attention_backward(int device, const n3d_attn_config* cfg, const 
         a.row_dot = static_cast<float*>(d_workspace);
         if (cfg->seqs == 0) return;
         DeviceGuard g(device);
-        check_record(train_error(device));
+        a.err = train_error(device);
+        check_record(a.err);
         n3d::launch_attention_backward((cudaStream_t)stream, a, cfg->dtype);
     });
 }
