@@ -145,6 +145,8 @@ struct TcMaps {
 struct TcArgs {
     AttnArgs a;
     int tiles;         // row tiles of a head
+    int run;           // heads whose tiles are interleaved
+    int ascending;     // which end of a one-sided window is open: 1 if keys before the query
     float k2, factor;  // |scale| log2 e; the scale of dq and dk
     int negate;        // scale < 0
     float* stats;      // [seqs * q_heads][q tiles][2][-lse log2 e: 64 | -D: 64]
@@ -195,10 +197,15 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
     const AttnArgs& a = args.a;
     int* const err = a.err;
     const int heads = MODE == GRAD_KV ? a.k_heads : a.q_heads, group = a.q_heads / a.k_heads;
-    const int sh = blockIdx.x / args.tiles, head = sh % heads, seq = sh / heads;
-    const int order = blockIdx.x - sh * args.tiles;
-    // queries: the last tiles see the most keys of a causal mask, so they go first
-    const int r0 = (MODE == GRAD_KV ? order : args.tiles - 1 - order) * ROWS;
+    // Heads in runs of args.run: within a run the same tile of every head, then the next tile.
+    // Under a one-sided window the tiles with the most columns go first (the last query tiles see
+    // the most keys, the first key tiles the most queries), so that the blocks that finish
+    // last are short.  Without one the run is 1: the tiles of a head, which read the same columns,
+    // are neighbours.
+    const int run0 = blockIdx.x / (args.run * args.tiles) * args.run, in_run = blockIdx.x - run0 * args.tiles;
+    const int width = min(args.run, heads * a.seqs - run0), order = in_run / width;
+    const int sh = run0 + in_run - order * width, head = sh % heads, seq = sh / heads;
+    const int r0 = ((MODE == GRAD_KV) == args.ascending ? order : args.tiles - 1 - order) * ROWS;
     const AttnMask mask(a, seq);
     const int row_len = MODE == GRAD_KV ? mask.k_len : mask.q_len, col_len = MODE == GRAD_KV ? mask.q_len : mask.k_len;
     const int row_cap = MODE == GRAD_KV ? a.k_rows : a.q_rows, col_cap = MODE == GRAD_KV ? a.q_rows : a.k_rows;
@@ -284,7 +291,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 __syncwarp();
             }
             tc_fence_after();
-            if (lane == 0) {
+            if (elect_one()) {
                 const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
                 const uint32_t t = tmem + (g % NBUF) * C::TBUF;
 #pragma unroll
@@ -309,7 +316,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
             ok = __all_sync(0xffffffffu, mbar_wait(&p_full[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
+            if (elect_one()) {
                 const uint32_t b = smem_u32(ring + (g % NST) * C::STAGE);
                 const uint32_t t = tmem + (g % NBUF) * C::TBUF;
                 // forward: P v (tile 2); gradients: dS k or dS^T q (tile 1), and P^T dout (tile 2)
@@ -473,58 +480,53 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 tmem_st16(t + 16, w + 16);
             } else {
                 const float4* st = reinterpret_cast<const float4*>(ring + (g % NST) * C::STAGE + 2 * C::CTILE);
-                const uint64_t k22 = pack2(k2, k2);
+                const uint64_t k22 = pack2(k2, k2), scale2 = pack2(ds_scale, ds_scale);
                 if (MODE == GRAD_KV)  // the statistics came by bulk copy: this thread's own wait makes them visible
                     ok = __all_sync(0xffffffffu,
                                     ok && mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                auto weights = [&](auto masked) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {  // 32 columns: weights h go over scores that are read already
-                    float s[32], u[32];
-                    tmem_ld32(t + 32 * h, s);
-                    tmem_ld32(t + 64 + 32 * h, u);
-                    uint32_t pw[16], dw[16];
+                    for (int h = 0; h < 2; h++) {  // 32 columns: weights h go over scores that are read already
+                        float s[32], u[32];
+                        tmem_ld32(t + 32 * h, s);
+                        tmem_ld32(t + 64 + 32 * h, u);
+                        uint32_t pw[16], dw[16];
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
-                        if (MODE == GRAD_KV) {
-                            nl = st[8 * h + c / 4];
-                            nd = st[16 + 8 * h + c / 4];
-                        }
+                        for (int c = 0; c < 32; c += 4) {
+                            float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
+                            if (MODE == GRAD_KV) {
+                                nl = st[8 * h + c / 4];
+                                nd = st[16 + 8 * h + c / 4];
+                            }
 #pragma unroll
-                        for (int e = 0; e < 4; e += 2) {
-                            const uint64_t n2 = e == 0 ? pack2(nl.x, nl.y) : pack2(nl.z, nl.w);
-                            const uint64_t d2 = e == 0 ? pack2(nd.x, nd.y) : pack2(nd.z, nd.w);
-                            float x, y;
-                            unpack2(fma2(pack2(s[c + e], s[c + e + 1]), k22, n2), x, y);
-                            if (!full) {
+                            for (int e = 0; e < 4; e += 2) {
+                                const uint64_t n2 = e == 0 ? pack2(nl.x, nl.y) : pack2(nl.z, nl.w);
+                                const uint64_t d2 = e == 0 ? pack2(nd.x, nd.y) : pack2(nd.z, nd.w);
                                 const int cc = c0 + 32 * h + c + e;
-                                if (cc < lo || cc >= hi) x = -INFINITY;
-                                if (cc + 1 < lo || cc + 1 >= hi) y = -INFINITY;
+                                float x, y, gx, gy;
+                                unpack2(fma2(pack2(s[c + e], s[c + e + 1]), k22, n2), x, y);
+                                x = ex2_approx(x);
+                                y = ex2_approx(y);
+                                if (masked && (cc < lo || cc >= hi)) x = 0.0f;
+                                if (masked && (cc + 1 < lo || cc + 1 >= hi)) y = 0.0f;
+                                uint64_t g2 = mul2(pack2(x, y), add2(pack2(u[c + e], u[c + e + 1]), d2));
+                                if (F16) g2 = mul2(g2, scale2);
+                                unpack2(g2, gx, gy);
+                                if (masked && x == 0.0f) gx = 0.0f;
+                                if (masked && y == 0.0f) gy = 0.0f;
+                                if (MODE == GRAD_KV)
+                                    pw[(c + e) / 2] = F16 ? pack_pair<T>(x * 1024.0f, y * 1024.0f) : pack_pair<T>(x, y);
+                                dw[(c + e) / 2] = pack_pair<T>(gx, gy);
                             }
-                            const bool sx = x != -INFINITY, sy = y != -INFINITY;
-                            x = ex2_approx(x);
-                            y = ex2_approx(y);
-                            uint64_t p2 = pack2(x, y);
-                            if (F16 && MODE == GRAD_Q) p2 = mul2(p2, pack2(ds_scale, ds_scale));
-                            uint64_t g2 = mul2(p2, add2(pack2(u[c + e], u[c + e + 1]), d2));
-                            if (F16 && MODE == GRAD_KV) {
-                                g2 = mul2(g2, pack2(ds_scale, ds_scale));
-                                x *= 1024.0f;
-                                y *= 1024.0f;
-                            }
-                            float gx, gy;
-                            unpack2(g2, gx, gy);
-                            if (!full) {
-                                if (!sx) gx = 0.0f;
-                                if (!sy) gy = 0.0f;
-                            }
-                            if (MODE == GRAD_KV) pw[(c + e) / 2] = pack_pair<T>(x, y);
-                            dw[(c + e) / 2] = pack_pair<T>(gx, gy);
                         }
+                        if (MODE == GRAD_KV) tmem_st16(t + 16 * h, pw);
+                        tmem_st16(t + 64 + 16 * h, dw);
                     }
-                    if (MODE == GRAD_KV) tmem_st16(t + 16 * h, pw);
-                    tmem_st16(t + 64 + 16 * h, dw);
-                }
+                };
+                if (full)
+                    weights(std::false_type());
+                else
+                    weights(std::true_type());
             }
             tmem_wait_st();
             tc_fence_before();
@@ -663,6 +665,9 @@ void launch(cudaStream_t s, const AttnArgs& a) {
         m.dk = map(a.dk, a.k_rows, a.k_heads, 32);
         m.dv = map(a.dv, a.k_rows, a.k_heads, 32);
     }
+    const bool before = a.left >= kNoLimit, after = a.right >= kNoLimit;
+    t.run = before != after ? (int)std::min<long long>((long long)heads * a.seqs, 32) : 1;
+    t.ascending = before;
     t.k2 = fabsf(a.scale) * LOG2E;
     t.factor = a.scale;
     t.negate = a.scale < 0.0f;

@@ -119,6 +119,18 @@ __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
+// True in one thread of the (converged) warp, always the same one.  A branch on it lets the
+// compiler keep the operands of tcgen05 instructions in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(pred));
+    return pred != 0;
+}
+
 // Shared-memory matrix descriptor for a K-major tile written by TMA with the
 // 128-byte swizzle: rows of 128 B, 8-row atoms 1024 B apart (SBO), leading
 // offset unused (1), descriptor version 1, layout SWIZZLE_128B (2).

@@ -18,6 +18,7 @@ import ctypes as C
 import os
 import weakref
 import re
+import struct
 import subprocess
 from dataclasses import dataclass
 
@@ -75,26 +76,6 @@ class CacheConfig(C.Structure):
                 ("num_silence_frames", _sz), ("score_threshold", C.c_float), ("latest_frames_score_boost", C.c_float),
                 ("num_speakers", _sz), ("subsampling_factor", _sz), ("min_positive_scores", _sz),
                 ("num_strong_boosted_frames", _sz), ("num_weak_boosted_frames", _sz)]
-
-
-class _Heads(C.Structure):
-    _fields_ = [("d_data", C.c_void_p), ("heads", _sz), ("seq_stride", C.c_longlong), ("row_stride", C.c_longlong),
-                ("head_stride", C.c_longlong)]
-
-
-class _Rows(C.Structure):
-    _fields_ = [("d_data", C.c_void_p), ("row_stride", C.c_longlong)]
-
-
-class _ResidualConfig(C.Structure):
-    _fields_ = [("rows", _sz), ("cols", _sz), ("residual_dtype", C.c_int), ("block_dtype", C.c_int),
-                ("post_norm", C.c_int), ("pre_norm", C.c_int), ("post_eps", C.c_float), ("pre_eps", C.c_float),
-                ("scale", C.c_float), ("rows_per_gate", _sz)]
-
-
-class _AttnConfig(C.Structure):
-    _fields_ = [("seqs", _sz), ("q_rows", _sz), ("k_rows", _sz), ("head_dim", _sz), ("dtype", C.c_int),
-                ("scale", C.c_float), ("left", C.c_longlong), ("right", C.c_longlong), ("q_offset", C.c_longlong)]
 
 
 class _RopeConfig(C.Structure):
@@ -206,19 +187,13 @@ def lib() -> C.CDLL:
         "n3d_bench_layer_norm": ([C.c_int, _sz, _sz, C.c_int, C.POINTER(C.c_double)], C.c_int),
         "n3d_train_status": ([C.c_int], C.c_int),
         "n3d_rope_plan_make": ([C.POINTER(_RopeConfig), C.POINTER(_RopePlan)], C.c_int),
-        "n3d_rope": ([C.c_int, C.POINTER(_RopePlan), C.c_int, _sz, _sz, _sz, C.POINTER(_Heads), C.POINTER(_Heads), vp,
-                      C.c_longlong, C.c_int, vp], C.c_int),
-        "n3d_residual_norm": ([C.c_int, C.POINTER(_ResidualConfig), C.POINTER(_Rows), C.POINTER(_Rows), vp, vp, vp, vp,
-                               vp, C.POINTER(_Rows), C.POINTER(_Rows), vp], C.c_int),
+        "n3d_rope": ([C.c_int, vp, C.c_int, _sz, _sz, _sz, vp, vp, vp, C.c_longlong, C.c_int, vp], C.c_int),
+        "n3d_residual_norm": ([C.c_int] + [vp] * 11, C.c_int),
         "n3d_residual_norm_workspace": ([_sz, _sz, _sz], _sz),
-        "n3d_residual_norm_grad": ([C.c_int, C.POINTER(_ResidualConfig), C.POINTER(_Rows), C.POINTER(_Rows), vp, vp, vp,
-                                    vp, C.POINTER(_Rows), C.POINTER(_Rows), C.POINTER(_Rows), C.POINTER(_Rows), vp, vp,
-                                    vp, vp, vp, vp, _sz, vp], C.c_int),
-        "n3d_attention_workspace": ([C.POINTER(_AttnConfig), _sz, _sz, C.c_int], _sz),
-        "n3d_attention_forward": ([C.c_int, C.POINTER(_AttnConfig)] + [C.POINTER(_Heads)] * 3 + [vp, vp]
-                                  + [C.POINTER(_Heads), vp, vp, _sz, vp], C.c_int),
-        "n3d_attention_backward": ([C.c_int, C.POINTER(_AttnConfig)] + [C.POINTER(_Heads)] * 4 + [vp, C.POINTER(_Heads)]
-                                   + [vp, vp] + [C.POINTER(_Heads)] * 3 + [vp, _sz, vp], C.c_int),
+        "n3d_residual_norm_grad": ([C.c_int] + [vp] * 17 + [_sz, vp], C.c_int),
+        "n3d_attention_workspace": ([vp, _sz, _sz, C.c_int], _sz),
+        "n3d_attention_forward": ([C.c_int] + [vp] * 9 + [_sz, vp], C.c_int),
+        "n3d_attention_backward": ([C.c_int] + [vp] * 13 + [_sz, vp], C.c_int),
         "n3d_profile_enable": ([vp, C.c_int], C.c_int),
         "n3d_profile_read": ([vp, C.POINTER(_KernelStats), _sz], _sz),
         "n3d_step_timing_enable": ([vp, C.c_int], C.c_int),
@@ -645,54 +620,79 @@ def selftest_wait_timeout(device: int, limit_ms: float) -> tuple[int, str, float
 
 # ---- training operators of an encoder block
 #
-# Tensors are any objects with data_ptr(), shape, stride() and dtype, as torch's (which
-# this module does not import).  Work is enqueued on `stream` (a cudaStream_t as an int,
-# None for the default stream) and the calls return without waiting for it.
+# Tensors are any objects with data_ptr(), shape, stride(), dtype, numel(), is_contiguous()
+# and get_device(), as torch's (which this module does not import).  Work is enqueued on
+# `stream` (a cudaStream_t as an int, None for the default stream) and the calls return
+# without waiting for it.  Small calls cost what this file costs: the C structures are
+# packed as bytes, in one step for all tensors of a call, rather than built field by field.
 
 DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
 ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+NORMS = {"none": 0, "layer": 1, "rms": 2}
+
+_pack_heads = struct.Struct("PNqqq").pack           # n3d_heads
+_pack_heads2 = struct.Struct("PNqqqPNqqq").pack     # n3d_heads[2]
+_pack_rows = struct.Struct("Pq").pack               # n3d_rows
+_pack_residual = struct.Struct("NNiiiifff4xN").pack  # n3d_residual_config
+_pack_attn = struct.Struct("NNNNif qqq").pack       # n3d_attn_config
+_dtype_codes: dict = {}                             # a library's dtype object -> n3d_dtype
 
 
 def _bad(message: str) -> DiarizationError:
     return DiarizationError(13, message)
 
 
-def _dtype(t) -> int:
-    name = str(t.dtype).rpartition(".")[2]
-    if name not in DTYPES:
-        raise _bad(f"dtype {name}: float32, bfloat16 or float16 is wanted")
-    return DTYPES[name]
+def _dtype(dtype) -> int:
+    code = _dtype_codes.get(dtype)
+    if code is None:
+        name = str(dtype).rpartition(".")[2]
+        if name not in DTYPES:
+            raise _bad(f"dtype {name}: float32, bfloat16 or float16 is wanted")
+        code = _dtype_codes[dtype] = DTYPES[name]
+    return code
 
 
 def _device(t) -> int:
-    d = t.device
-    if d.type != "cuda":
+    d = t.get_device()
+    if d < 0:
         raise _bad("a tensor is not in device memory")
-    return d.index or 0
+    return d
 
 
-def _heads(t, shape=None, dtype=None) -> _Heads:
-    """A [seqs, rows, heads, head_dim] tensor as n3d_heads; `shape` and `dtype` are what it must have."""
-    sh, st = t.shape, t.stride()
-    if len(sh) != 4:
+def _heads(t, seqs, rows, heads, hd, dtype, device):
+    """The fields of n3d_heads of a [seqs, rows, heads, hd] tensor (heads None: any)."""
+    if len(t.shape) != 4:
         raise _bad("a [seqs, rows, heads, head_dim] tensor is wanted")
-    if shape is not None and tuple(sh) != tuple(shape):
-        raise _bad(f"a tensor of shape {tuple(sh)} where {tuple(shape)} is wanted")
-    if dtype is not None and t.dtype != dtype:
+    s, r, h, d = t.shape
+    a, b, c, e = t.stride()
+    if s != seqs or r != rows or d != hd or (h != heads and heads is not None):
+        raise _bad(f"a tensor of shape {tuple(t.shape)} where {(seqs, rows, heads, hd)} is wanted")
+    if t.dtype != dtype:
         raise _bad(f"a tensor of type {t.dtype} where {dtype} is wanted")
-    if st[3] != 1 and sh[3] > 1:
+    if e != 1 and d > 1:
         raise _bad("the elements of a head must be consecutive")
-    return _Heads(t.data_ptr(), sh[2], st[0], st[1], st[2])
+    if t.get_device() != device:
+        raise _bad("the tensors are not all on one device")
+    return t.data_ptr(), h, a, b, c
 
 
 def _flat(t, count: int, dtype: str, device: int):
     """The pointer of a contiguous tensor of `count` elements (None: NULL)."""
     if t is None:
         return None
-    if not str(t.dtype).endswith(dtype) or t.numel() != count or not t.is_contiguous() or _device(t) != device:
+    if t.numel() != count or not t.is_contiguous() or t.get_device() != device or str(t.dtype).rpartition(".")[2] != dtype:
         raise _bad(f"a contiguous {dtype} tensor of {count} elements on device {device} is wanted")
     return t.data_ptr()
+
+
+def _space(t, device: int):
+    """Pointer and bytes of a workspace tensor (None: nothing)."""
+    if t is None:
+        return None, 0
+    if t.get_device() != device or not t.is_contiguous():
+        raise _bad("a contiguous workspace on the tensors' device is wanted")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 def train_status(device: int = 0) -> None:
@@ -713,10 +713,8 @@ class RopePlan:
                           ROPE_SCALINGS[scaling], theta, factor, original_length, beta_fast, beta_slow,
                           attention_factor)
         _check(lib().n3d_rope_plan_make(C.byref(cfg), C.byref(self._p)))
-
-    @property
-    def head_dim(self) -> int:
-        return self._p.head_dim
+        self._at = C.addressof(self._p)
+        self.head_dim = head_dim
 
     @property
     def attention_factor(self) -> float:
@@ -734,49 +732,56 @@ def rope(plan: RopePlan, xs, ys, positions=None, first_position: int = 0, transp
     (n3d_rope); `ys` may be `xs`.  `positions`: int32 [seqs, rows], or None for first_position + row.
     transpose=True is the gradient: dL/dy -> dL/dx."""
     n = len(xs)
-    if n not in (1, 2) or len(ys) != n:
-        raise _bad("rope: one or two tensors, and as many outputs, are wanted")
-    seqs, rows, _, hd = xs[0].shape
+    if n not in (1, 2) or len(ys) != n or len(xs[0].shape) != 4:
+        raise _bad("rope: one or two [seqs, rows, heads, head_dim] tensors, and as many outputs, are wanted")
+    seqs, rows, heads, hd = xs[0].shape
     if hd != plan.head_dim:
         raise _bad(f"rope: head_dim {hd}, the plan has {plan.head_dim}")
-    dt, device = xs[0].dtype, _device(xs[0])
-    x, y = (_Heads * 2)(), (_Heads * 2)()
-    for i in range(n):
-        x[i] = _heads(xs[i], (seqs, rows, xs[i].shape[2], hd), dt)
-        y[i] = _heads(ys[i], xs[i].shape, dt)
-    _check(lib().n3d_rope(device, C.byref(plan._p), _dtype(xs[0]), seqs, rows, n, x, y,
-                          _flat(positions, seqs * rows, "int32", device), first_position, int(transpose), stream))
+    dt, dev = xs[0].dtype, _device(xs[0])
+    x = _heads(xs[0], seqs, rows, heads, hd, dt, dev)
+    y = _heads(ys[0], seqs, rows, heads, hd, dt, dev)
+    if n == 2:
+        x1 = _heads(xs[1], seqs, rows, None, hd, dt, dev)
+        x, y = _pack_heads2(*x, *x1), _pack_heads2(*y, *_heads(ys[1], seqs, rows, x1[1], hd, dt, dev))
+    else:
+        x, y = _pack_heads(*x), _pack_heads(*y)
+    st = (_lib or lib()).n3d_rope(dev, plan._at, _dtype(dt), seqs, rows, n, x, y,
+                                  _flat(positions, seqs * rows, "int32", dev), first_position, transpose, stream)
+    if st:
+        _check(st)
 
 
-NORMS = {"none": 0, "layer": 1, "rms": 2}
-
-
-def _rows(t, shape, dtype=None):
+def _matrix(t, rows, cols, dtype, device):
     """A [rows, cols] tensor as n3d_rows (None: NULL)."""
     if t is None:
         return None
-    if tuple(t.shape) != shape:
-        raise _bad(f"a matrix of shape {tuple(t.shape)} where {shape} is wanted")
-    if dtype is not None and t.dtype != dtype:
+    if tuple(t.shape) != (rows, cols):
+        raise _bad(f"a matrix of shape {tuple(t.shape)} where {(rows, cols)} is wanted")
+    if t.dtype != dtype:
         raise _bad(f"a matrix of type {t.dtype} where {dtype} is wanted")
-    st = t.stride()
-    if st[1] != 1 and shape[1] > 1:
+    a, b = t.stride()
+    if b != 1 and cols > 1:
         raise _bad("the elements of a row must be consecutive")
-    return C.byref(_Rows(t.data_ptr(), st[0]))
+    if t.get_device() != device:
+        raise _bad("the tensors are not all on one device")
+    return _pack_rows(t.data_ptr(), a)
 
 
 def _residual_config(residual, block, post, pre, eps, scale, gate, gate_rows):
+    """(n3d_residual_config, rows, cols, values of the gate)"""
     if post not in NORMS or pre not in NORMS:
         raise _bad(f"unknown norm {post} or {pre}")
     if len(block.shape) != 2:
         raise _bad("a [rows, cols] matrix is wanted")
     rows, cols = block.shape
     if gate is None:
-        gate_rows = 0
+        gate_rows = gates = 0
     elif gate_rows < 1:
         raise _bad("a gate needs gate_rows, the number of rows that share one of its rows")
-    return _ResidualConfig(rows, cols, _dtype(residual), _dtype(block), NORMS[post], NORMS[pre], eps, eps, scale,
-                           gate_rows)
+    else:
+        gates = -(-rows // gate_rows) * cols
+    return _pack_residual(rows, cols, _dtype(residual.dtype), _dtype(block.dtype), NORMS[post], NORMS[pre], eps, eps,
+                          scale, gate_rows), rows, cols, gates
 
 
 def residual_norm(x, block, r, y, post: str = "none", pre: str = "layer", eps: float = 1e-5, scale: float = 1.0,
@@ -785,18 +790,20 @@ def residual_norm(x, block, r, y, post: str = "none", pre: str = "layer", eps: f
     """r = x + scale * gate * Norm_post(block), y = Norm_pre(r) (n3d_residual_norm); norms are "none",
     "layer" or "rms".  gate [ceil(rows / gate_rows), cols], weights and biases [cols]: fp32 or None.
     r may be x, y may be block; y is None when pre is "none"."""
-    cfg = _residual_config(x, block, post, pre, eps, scale, gate, gate_rows)
-    sh, dev, cols = (cfg.rows, cfg.cols), _device(x), cfg.cols
-    gates = -(-cfg.rows // cfg.rows_per_gate) * cols if gate is not None else 0
-    _check(lib().n3d_residual_norm(
-        dev, C.byref(cfg), _rows(x, sh), _rows(block, sh), _flat(post_w, cols, "float32", dev),
-        _flat(post_b, cols, "float32", dev), _flat(gate, gates, "float32", dev), _flat(pre_w, cols, "float32", dev),
-        _flat(pre_b, cols, "float32", dev), _rows(r, sh, x.dtype), _rows(y, sh, block.dtype), stream))
+    cfg, rows, cols, gates = _residual_config(x, block, post, pre, eps, scale, gate, gate_rows)
+    dev, rt, bt = _device(x), x.dtype, block.dtype
+    st = (_lib or lib()).n3d_residual_norm(
+        dev, cfg, _matrix(x, rows, cols, rt, dev), _matrix(block, rows, cols, bt, dev),
+        _flat(post_w, cols, "float32", dev), _flat(post_b, cols, "float32", dev), _flat(gate, gates, "float32", dev),
+        _flat(pre_w, cols, "float32", dev), _flat(pre_b, cols, "float32", dev), _matrix(r, rows, cols, rt, dev),
+        _matrix(y, rows, cols, bt, dev), stream)
+    if st:
+        _check(st)
 
 
 def residual_norm_workspace(rows: int, cols: int, gate_rows: int = 0) -> int:
     """Bytes of workspace residual_norm_grad needs (n3d_residual_norm_workspace)."""
-    return lib().n3d_residual_norm_workspace(rows, cols, gate_rows)
+    return (_lib or lib()).n3d_residual_norm_workspace(rows, cols, gate_rows)
 
 
 def residual_norm_grad(block, r, dy, dr, dx, dblock, post: str = "none", pre: str = "layer", eps: float = 1e-5,
@@ -806,30 +813,34 @@ def residual_norm_grad(block, r, dy, dr, dx, dblock, post: str = "none", pre: st
     """The gradient of residual_norm (n3d_residual_norm_grad): dy and dr (or None) -> dx, dblock, and the
     fp32 gradients that are not None.  `workspace`: a tensor of at least residual_norm_workspace bytes.
     pre_b does not enter; it is accepted so that both calls take the same arguments."""
-    cfg = _residual_config(dx, block, post, pre, eps, scale, gate, gate_rows)
-    sh, dev, cols = (cfg.rows, cfg.cols), _device(dx), cfg.cols
-    gates = -(-cfg.rows // cfg.rows_per_gate) * cols if gate is not None else 0
-    w = [_flat(t, cols, "float32", dev) for t in (post_w, post_b, pre_w, dpost_w, dpost_b, dpre_w, dpre_b)]
-    _check(lib().n3d_residual_norm_grad(
-        dev, C.byref(cfg), _rows(block, sh), _rows(r, sh, dx.dtype), w[0], w[1], _flat(gate, gates, "float32", dev), w[2],
-        _rows(dy, sh, block.dtype), _rows(dr, sh, dx.dtype), _rows(dx, sh), _rows(dblock, sh, block.dtype),
-        _flat(dgate, gates, "float32", dev), w[3], w[4], w[5], w[6],
-        workspace.data_ptr() if workspace is not None else None,
-        workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))
+    cfg, rows, cols, gates = _residual_config(dx, block, post, pre, eps, scale, gate, gate_rows)
+    dev, rt, bt = _device(dx), dx.dtype, block.dtype
+    f = "float32"
+    st = (_lib or lib()).n3d_residual_norm_grad(
+        dev, cfg, _matrix(block, rows, cols, bt, dev), _matrix(r, rows, cols, rt, dev), _flat(post_w, cols, f, dev),
+        _flat(post_b, cols, f, dev), _flat(gate, gates, f, dev), _flat(pre_w, cols, f, dev),
+        _matrix(dy, rows, cols, bt, dev), _matrix(dr, rows, cols, rt, dev), _matrix(dx, rows, cols, rt, dev),
+        _matrix(dblock, rows, cols, bt, dev), _flat(dgate, gates, f, dev), _flat(dpost_w, cols, f, dev),
+        _flat(dpost_b, cols, f, dev), _flat(dpre_w, cols, f, dev), _flat(dpre_b, cols, f, dev), *_space(workspace, dev),
+        stream)
+    if st:
+        _check(st)
 
 
-def _attn_config(q, k, scale, left, right, q_offset) -> _AttnConfig:
+def _attn_config(q, k, scale, left, right, q_offset) -> bytes:
     if len(q.shape) != 4 or len(k.shape) != 4:
         raise _bad("a [seqs, rows, heads, head_dim] tensor is wanted")
-    return _AttnConfig(q.shape[0], q.shape[1], k.shape[1], q.shape[3], _dtype(q), scale, left, right, q_offset)
+    b, n, _, hd = q.shape
+    return _pack_attn(b, n, k.shape[1], hd, _dtype(q.dtype), scale, left, right, q_offset)
 
 
 def attention_workspace(q, k, backward: bool = True) -> int:
     """Bytes of workspace attention_forward (backward False) or both calls (True) need for tensors like q
     and k (n3d_attention_workspace)."""
     cfg = _attn_config(q, k, 0.0, -1, -1, 0)
-    need = [lib().n3d_attention_workspace(C.byref(cfg), q.shape[2], k.shape[2], b) for b in (0, 1)]
-    return max(need) if backward else need[0]
+    size = (_lib or lib()).n3d_attention_workspace
+    need = size(cfg, q.shape[2], k.shape[2], 0)
+    return max(need, size(cfg, q.shape[2], k.shape[2], 1)) if backward else need
 
 
 def attention_forward(q, k, v, out, lse=None, q_len=None, k_len=None, scale: float = 0.0, left: int = -1,
@@ -837,26 +848,32 @@ def attention_forward(q, k, v, out, lse=None, q_len=None, k_len=None, scale: flo
     """Attention of q [seqs, q rows, q heads, head_dim] over k, v [seqs, k rows, k heads, head_dim] into out, with
     the rows' log-sum-exp in lse [seqs, q heads, q rows] (fp32) for the gradient (n3d_attention_forward).
     q_len, k_len: int32 [seqs]; left, right: the window around key row i + q_offset, negative for no limit."""
-    cfg, dev = _attn_config(q, k, scale, left, right, q_offset), _device(q)
+    cfg = _attn_config(q, k, scale, left, right, q_offset)
+    dev, dt = _device(q), q.dtype
     b, nq, hq, hd = q.shape
-    kv = (b, k.shape[1], k.shape[2], hd)
-    _check(lib().n3d_attention_forward(
-        dev, C.byref(cfg), _heads(q), _heads(k, kv, q.dtype), _heads(v, kv, q.dtype), _flat(q_len, b, "int32", dev),
-        _flat(k_len, b, "int32", dev), _heads(out, q.shape, q.dtype), _flat(lse, b * hq * nq, "float32", dev),
-        workspace.data_ptr() if workspace is not None else None,
-        workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))
+    _, nk, hk, _ = k.shape
+    st = (_lib or lib()).n3d_attention_forward(
+        dev, cfg, _pack_heads(*_heads(q, b, nq, hq, hd, dt, dev)), _pack_heads(*_heads(k, b, nk, hk, hd, dt, dev)),
+        _pack_heads(*_heads(v, b, nk, hk, hd, dt, dev)), _flat(q_len, b, "int32", dev), _flat(k_len, b, "int32", dev),
+        _pack_heads(*_heads(out, b, nq, hq, hd, dt, dev)), _flat(lse, b * hq * nq, "float32", dev),
+        *_space(workspace, dev), stream)
+    if st:
+        _check(st)
 
 
 def attention_backward(q, k, v, out, lse, dout, dq, dk, dv, q_len=None, k_len=None, scale: float = 0.0, left: int = -1,
                        right: int = -1, q_offset: int = 0, workspace=None, stream: int | None = None) -> None:
     """The gradient of attention_forward from its out and lse: dout -> dq, dk, dv (n3d_attention_backward).
     `workspace`: a tensor of at least attention_workspace bytes."""
-    cfg, dev = _attn_config(q, k, scale, left, right, q_offset), _device(q)
+    cfg = _attn_config(q, k, scale, left, right, q_offset)
+    dev, dt = _device(q), q.dtype
     b, nq, hq, hd = q.shape
-    dt, kv = q.dtype, (b, k.shape[1], k.shape[2], hd)
-    _check(lib().n3d_attention_backward(
-        dev, C.byref(cfg), _heads(q), _heads(k, kv, dt), _heads(v, kv, dt), _heads(out, q.shape, dt),
-        _flat(lse, b * hq * nq, "float32", dev), _heads(dout, q.shape, dt), _flat(q_len, b, "int32", dev),
-        _flat(k_len, b, "int32", dev), _heads(dq, q.shape, dt), _heads(dk, kv, dt), _heads(dv, kv, dt),
-        workspace.data_ptr() if workspace is not None else None,
-        workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))
+    _, nk, hk, _ = k.shape
+    qs = [_pack_heads(*_heads(t, b, nq, hq, hd, dt, dev)) for t in (q, out, dout, dq)]
+    ks = [_pack_heads(*_heads(t, b, nk, hk, hd, dt, dev)) for t in (k, v, dk, dv)]
+    st = (_lib or lib()).n3d_attention_backward(
+        dev, cfg, qs[0], ks[0], ks[1], qs[1], _flat(lse, b * hq * nq, "float32", dev), qs[2],
+        _flat(q_len, b, "int32", dev), _flat(k_len, b, "int32", dev), qs[3], ks[2], ks[3], *_space(workspace, dev),
+        stream)
+    if st:
+        _check(st)

@@ -14,7 +14,12 @@ class FakeTensor:
                 stride.insert(0, n)
                 n *= s
         self._s = tuple(stride)
-        self.device = type("Device", (), {"type": "cuda", "index": 0})()
+
+    def get_device(self):
+        return 0
+
+    def element_size(self):
+        return {"float64": 8, "float32": 4, "int32": 4, "int64": 8, "uint8": 1}.get(self.dtype[6:], 2)
 
     def data_ptr(self):
         return self._p

@@ -12,7 +12,6 @@ sum |dout v|, dS by P (2 d |dP - D| + eD + err(dP)) + h |dS| (fp16: + 2^-24 max|
 gradients by the sums of these against |k|, |q| and |dout|, plus 16 e of the sums of
 magnitudes and their own rounding."""
 
-import ctypes as C
 import math
 
 import numpy as np
@@ -111,7 +110,6 @@ def _call(q=None, k=None, v=None, out=None, backward=False, space=1 << 20, **kw)
     if not backward:
         return n3d.attention_forward(q, k, v, out, kw.pop("lse", None), **kw)
     work = FakeTensor((space,), dtype="uint8", ptr=10 << 20)
-    work.element_size = lambda: 1
     g = {n: FakeTensor(t.shape, ptr=p << 20) for n, t, p in (("dout", q, 5), ("dq", q, 6), ("dk", k, 7), ("dv", k, 8))}
     g.update({n: kw.pop(n) for n in list(g) if n in kw})
     lse = kw.pop("lse", FakeTensor((2, 4, 5), ptr=9 << 20))
@@ -150,8 +148,8 @@ def test_null_arguments():
     L = n3d.lib()
     assert n3d.STATUS[L.n3d_attention_forward(0, None, None, None, None, None, None, None, None, None, 0, None)] == \
         "InvalidArgument"
-    cfg = n3d._AttnConfig(1, 1, 1, 64, 0, 0.0, -1, -1, 0)
-    assert n3d.STATUS[L.n3d_attention_forward(0, C.byref(cfg), None, None, None, None, None, None, None, None, 0,
+    cfg = n3d._pack_attn(1, 1, 1, 64, 0, 0.0, -1, -1, 0)
+    assert n3d.STATUS[L.n3d_attention_forward(0, cfg, None, None, None, None, None, None, None, None, 0,
                                               None)] == "InvalidArgument"
     assert L.n3d_attention_workspace(None, 1, 1, 1) == 0
 

@@ -11,7 +11,6 @@ are within 150 e: 350 e times the sum of the terms' magnitudes.  Outputs of 16 b
 rounded once more: half an ulp (2^-8 of bf16, 2^-11 of fp16, whose subnormals end at
 2^-24)."""
 
-import ctypes as C
 import math
 
 import numpy as np
@@ -55,7 +54,6 @@ def _backward(rows=4, cols=64, space=1 << 30, **kw):
     a = {n: FakeTensor((rows, cols), ptr=next(at)) for n in ("block", "r", "dy", "dr", "dx", "dblock")}
     a.update(kw)
     work = FakeTensor((space,), dtype="uint8", ptr=a.pop("work_ptr", next(at)))
-    work.element_size = lambda: 1
     n3d.residual_norm_grad(workspace=work, **a)
 
 
@@ -74,8 +72,8 @@ def test_gradient_refusals(kw):
 def test_null_configuration():
     L = n3d.lib()
     assert n3d.STATUS[L.n3d_residual_norm(0, None, *[None] * 9, None)] == "InvalidArgument"
-    cfg = n3d._ResidualConfig(4, 64, 0, 0, 0, 1, 1e-5, 1e-5, 1.0, 0)
-    assert n3d.STATUS[L.n3d_residual_norm(0, C.byref(cfg), *[None] * 9, None)] == "InvalidArgument"
+    cfg = n3d._pack_residual(4, 64, 0, 0, 0, 1, 1e-5, 1e-5, 1.0, 0)
+    assert n3d.STATUS[L.n3d_residual_norm(0, cfg, *[None] * 9, None)] == "InvalidArgument"
 
 
 def test_workspace_sizes():
