@@ -12,9 +12,13 @@
 // (MN-major), so no tile is stored twice or transposed.  Nothing of size rows x columns
 // leaves the SM.
 //   warp 0      TMA: the row tiles once, the column tiles through a ring of stages
-//   warp 1      TMEM owner; issues every MMA: T of block g + NBUF once the second product of
-//               block g, which reads the weights in the same columns, has completed
-//   warps 2..   softmax groups of 4 warps, one thread per row; group g % NWG works on block g
+//   warp 1      TMEM owner; issues T of block g once the second products of block g - NBUF, which read
+//               the weights in the same columns, have completed
+//   warp 2      issues the second products (with both kinds on one thread, which issues an MMA of 64
+//               columns every ~55 clocks, that thread was the bottleneck; a thread for each of the
+//               four products of dkv gains nothing more: the MMAs then wait for one another)
+//   warps 3..   softmax groups of 4 warps, one thread per row; NWG blocks are in work at a time, the
+//               SPLIT groups of a block take 64 / SPLIT of its columns each
 // head_dim 64: one group and two blocks per SM, which interleave (256 TMEM columns each);
 // head_dim 128: one block per SM with two groups on alternating column blocks (forward:
 // each with its own running maximum, sum and accumulator, joined at the end).
@@ -30,7 +34,7 @@
 // |v row| then stays inside fp16 while |v row| < 4096.
 //
 // Rows past a sequence's length: TMA fills what lies past the tensor with zeros, and the
-// MMA warp overwrites what lies past the length with zeros before a tile is used, so
+// T warp overwrites what lies past the length with zeros before a tile is used, so
 // nothing that stands there enters a product.  Pairs that the mask hides are cleared by a
 // select.  Every wait is bounded; an expired wait records its site and the block returns.
 // Each barrier is waited for at most one phase behind (argued at the waits).
@@ -57,22 +61,26 @@ constexpr int DEV_TIMEOUT_ATTN_TRAIN = 7;
 template <int HD, int MODE>
 struct Cfg {
     static constexpr bool GRAD = MODE != FORWARD;
-    static constexpr int NWG = HD == 64 ? 1 : 2;                          // softmax groups
-    static constexpr int NBUF = HD == 64 && GRAD ? 1 : 2;                 // score buffers, a multiple of NWG
-    static constexpr int THREADS = 64 + 128 * NWG, PER_SM = HD == 64 ? 2 : 1;
+    static constexpr int NWG = HD == 64 ? 1 : 2;            // column blocks in softmax at a time
+    static constexpr int SPLIT = GRAD && HD == 64 ? 2 : 1;   // groups of 4 warps that share a block's columns
+    static constexpr int CHUNK = 16;                        // columns a thread has in registers at a time (gradients)
+    static constexpr int GROUPS = NWG * SPLIT;
+    static constexpr int NBUF = MODE == FORWARD ? 2 : NWG;  // score buffers
+    static constexpr int SOFTMAX = 3;                       // first softmax warp
+    static constexpr int THREADS = 32 * SOFTMAX + 128 * GROUPS, PER_SM = HD == 128 ? 1 : 2;
     static constexpr int RTILE = ROWS * HD * 2, CTILE = COLS * HD * 2;    // bytes
     static constexpr int STATS = MODE == GRAD_KV ? 512 : 0;               // 64 x (-lse log2 e), 64 x (-D)
     static constexpr int STAGE = 2 * CTILE + 1024 * (STATS > 0), NST = 4;
     static constexpr int ROW_BYTES = (GRAD ? 2 : 1) * RTILE;
     // barriers and the TMEM slot, the groups' row statistics, and slack to align the tiles to 1024 bytes
-    static constexpr int SMEM = ROW_BYTES + NST * STAGE + 256 + (NWG > 1 ? 4 * 128 * 4 : 64) + 1024;
+    static constexpr int SMEM = ROW_BYTES + NST * STAGE + 256 + (MODE == FORWARD && NWG > 1 ? 4 * 128 * 4 : 64) + 1024;
     static constexpr uint32_t TBUF = GRAD ? 128 : 64;                     // TMEM columns of a score buffer
     static constexpr uint32_t ACC = NBUF * TBUF;                          // first accumulator
     static constexpr int NACC = MODE == FORWARD ? NWG : MODE == GRAD_Q ? 1 : 2;
-    static constexpr uint32_t TMEM_COLS = HD == 64 ? 256 : 512;
-    static_assert(ACC + NACC * HD <= TMEM_COLS, "TMEM");
-    static_assert(NBUF % NWG == 0, "a score buffer belongs to one softmax group");
-    static_assert(SMEM * PER_SM <= 227 * 1024, "shared memory");
+    static constexpr uint32_t TMEM_COLS = HD == 128 ? 512 : 256;
+    static_assert(COLS / SPLIT % CHUNK == 0, "whole chunks");
+    static_assert(ACC + NACC * HD <= TMEM_COLS && PER_SM * TMEM_COLS <= 512, "TMEM");
+    static_assert((SMEM + 1024) * PER_SM <= 228 * 1024, "shared memory");
 };
 
 // Instruction descriptor of kind::f16 with fp32 accumulators, M = 128; B K-major, or
@@ -126,6 +134,55 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t* v) {
+    static_assert(N == 8 || N == 16, "8 or 16 columns");
+    N == 8 ? tmem_st8(taddr, v) : tmem_st16(taddr, v);
+}
+// N columns at each of two places of this thread's lane: both loads, one wait.
+template <int N>
+__device__ __forceinline__ void tmem_ld_pair(uint32_t a, uint32_t b, float* x, float* y) {
+    static_assert(N == 16 || N == 32, "16 or 32 columns");
+    uint32_t r[2 * N];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        if constexpr (N == 16)
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                : "=r"(r[N * h + 0]), "=r"(r[N * h + 1]), "=r"(r[N * h + 2]), "=r"(r[N * h + 3]), "=r"(r[N * h + 4]),
+                  "=r"(r[N * h + 5]), "=r"(r[N * h + 6]), "=r"(r[N * h + 7]), "=r"(r[N * h + 8]), "=r"(r[N * h + 9]),
+                  "=r"(r[N * h + 10]), "=r"(r[N * h + 11]), "=r"(r[N * h + 12]), "=r"(r[N * h + 13]),
+                  "=r"(r[N * h + 14]), "=r"(r[N * h + 15])
+                : "r"(h ? b : a));
+        else
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                : "=r"(r[N * h + 0]), "=r"(r[N * h + 1]), "=r"(r[N * h + 2]), "=r"(r[N * h + 3]), "=r"(r[N * h + 4]),
+                  "=r"(r[N * h + 5]), "=r"(r[N * h + 6]), "=r"(r[N * h + 7]), "=r"(r[N * h + 8]), "=r"(r[N * h + 9]),
+                  "=r"(r[N * h + 10]), "=r"(r[N * h + 11]), "=r"(r[N * h + 12]), "=r"(r[N * h + 13]),
+                  "=r"(r[N * h + 14]), "=r"(r[N * h + 15]), "=r"(r[N * h + 16]), "=r"(r[N * h + 17]),
+                  "=r"(r[N * h + 18]), "=r"(r[N * h + 19]), "=r"(r[N * h + 20]), "=r"(r[N * h + 21]),
+                  "=r"(r[N * h + 22]), "=r"(r[N * h + 23]), "=r"(r[N * h + 24]), "=r"(r[N * h + 25]),
+                  "=r"(r[N * h + 26]), "=r"(r[N * h + 27]), "=r"(r[N * h + 28]), "=r"(r[N * h + 29]),
+                  "=r"(r[N * h + 30]), "=r"(r[N * h + 31])
+                : "r"(h ? b : a));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    reg_fence16(r);
+    reg_fence16(r + 16);
+    if constexpr (N == 32) {
+        reg_fence16(r + 32);
+        reg_fence16(r + 48);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = __uint_as_float(r[i]), y[i] = __uint_as_float(r[N + i]);
 }
 __device__ __forceinline__ float max3f(float a, float b, float c) {
     float r;
@@ -181,7 +238,8 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
     if (warp == 0 && lane == 0) {
         mbar_init(r_full, 1);
         for (int i = 0; i < NST; i++) mbar_init(&c_full[i], 1), mbar_init(&c_empty[i], 1);
-        for (int i = 0; i < NBUF; i++) mbar_init(&t_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&acc_done[i], 1);
+        for (int i = 0; i < NBUF; i++)
+            mbar_init(&t_full[i], 1), mbar_init(&p_full[i], 4 * C::SPLIT), mbar_init(&acc_done[i], 1);
         mbar_init(all_done, 1);
         mbar_fence_init();
     }
@@ -260,14 +318,14 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 mbar_wait(&c_full[x % NST], (x / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN);
         }
     } else if (warp == 1) {
-        // zeros over rows [from, n) of a tile (boxes of `box_rows` rows)
+        // ---- T1, T2
+        // zeros over rows [from, n) of a tile (boxes of n rows)
         auto clear = [&](uint8_t* tile, int from, int n) {
             for (int i = 0; i < HD / 64; i++)
                 for (int x = from * 8 + lane; x < n * 8; x += 32)
                     *reinterpret_cast<uint4*>(tile + i * n * 128 + x * 16) = make_uint4(0, 0, 0, 0);
         };
         const uint32_t t_desc = idesc<T>(COLS, false, false), t_neg = idesc<T>(COLS, false, true);
-        constexpr uint32_t acc_desc = idesc<T>(HD, true);
         bool ok = nblk > 0;
         if (ok) {
             ok = __all_sync(0xffffffffu, mbar_wait(r_full, 0, err, DEV_TIMEOUT_ATTN_TRAIN));
@@ -278,10 +336,10 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 __syncwarp();
             }
         }
-        auto issue_t = [&](int g) {
+        for (int g = 0; ok && g < nblk; g++) {
             // the column tiles of block g (phase g / NST; the next needs this block's second product)
             ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-            if (!ok) return;
+            if (!ok) break;
             uint8_t* st = ring + (g % NST) * C::STAGE;
             const int c0 = col0(g);
             if (c0 + COLS > col_len && col_len < col_cap) {
@@ -290,6 +348,10 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 fence_async_smem();
                 __syncwarp();
             }
+            // T of block g overwrites the weights of block g - NBUF, which its second products have read
+            // (phase g / NBUF - 1; the next needs this T)
+            if (g >= NBUF) ok = __all_sync(0xffffffffu, mbar_wait(&acc_done[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
@@ -309,28 +371,34 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 umma_commit(&t_full[g % NBUF]);
             }
             __syncwarp();
-        };
-        for (int g = 0; ok && g < min(NBUF, nblk); g++) issue_t(g);
+        }
+    } else if (warp == 2) {
+        // ---- second products: P v (forward); dS k, or dS^T q and P^T dout
+        constexpr uint32_t acc_desc = idesc<T>(HD, true);
+        // where the weights of columns 16 kk.. are: each group's over its own scores
+        auto weight_col = [](int kk) { return C::SPLIT == 1 ? 8 * kk : 32 * (kk / 2) + 8 * (kk % 2); };
+        bool ok = true;
         for (int g = 0; ok && g < nblk; g++) {
-            // the weights of block g (phase g / NBUF; the next needs T of block g + NBUF, issued below)
-            ok = __all_sync(0xffffffffu, mbar_wait(&p_full[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            // the column tiles (as above) and the weights of block g (phase g / NBUF; the next needs T of
+            // block g + NBUF, hence this product)
+            ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN) &&
+                                             mbar_wait(&p_full[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t b = smem_u32(ring + (g % NST) * C::STAGE);
                 const uint32_t t = tmem + (g % NBUF) * C::TBUF;
-                // forward: P v (tile 2); gradients: dS k or dS^T q (tile 1), and P^T dout (tile 2)
                 const uint32_t acc = tmem + C::ACC + (MODE == FORWARD ? (g % NWG) * HD : 0);
                 const uint32_t first = MODE == FORWARD ? g < NWG : g == 0;
 #pragma unroll
                 for (int kk = 0; kk < COLS / 16; kk++)
-                    umma_f16_ts(acc, t + (C::GRAD ? 64 : 0) + 8 * kk,
+                    umma_f16_ts(acc, t + (C::GRAD ? 64 : 0) + weight_col(kk),
                                 desc_mn_sw128(b + (MODE == FORWARD ? C::CTILE : 0) + kk * 2048), acc_desc,
                                 kk != 0 || !first);
                 if (MODE == GRAD_KV) {
 #pragma unroll
                     for (int kk = 0; kk < COLS / 16; kk++)
-                        umma_f16_ts(acc + HD, t + 8 * kk, desc_mn_sw128(b + C::CTILE + kk * 2048), acc_desc,
+                        umma_f16_ts(acc + HD, t + weight_col(kk), desc_mn_sw128(b + C::CTILE + kk * 2048), acc_desc,
                                     kk != 0 || !first);
                 }
                 umma_commit(&acc_done[g % NBUF]);
@@ -338,17 +406,11 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 if (g == nblk - 1) umma_commit(all_done);
             }
             __syncwarp();
-            if (g + NBUF < nblk) {
-                // T of block g + NBUF overwrites the weights of block g (phase g / NBUF; the next
-                // needs that T)
-                ok = __all_sync(0xffffffffu,
-                                mbar_wait(&acc_done[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-                if (ok) issue_t(g + NBUF);
-            }
         }
     } else {
         // ---- softmax: group wg, TMEM lane quadrant warp % 4, one row per thread
-        const int wg = (warp - 2) / 4, qd = warp & 3, r = qd * 32 + lane, row = r0 + r;
+        const int grp = (warp - C::SOFTMAX) / 4, wg = grp / C::SPLIT, part = grp % C::SPLIT;
+        const int qd = warp & 3, r = qd * 32 + lane, row = r0 + r;
         const uint32_t lb = tmem + (static_cast<uint32_t>(qd * 32) << 16);
         const bool live = row < row_len;
         const int lo = first_col(row), hi = last_col(row);
@@ -384,7 +446,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
             }
             const float norm = sqrtf(norm2);
             if (F16) ds_scale = 8.0f * inverse_power(norm);
-            if (wg == 0) {
+            if (grp == 0) {
                 float* st = args.stats + ((sqh * args.q_tiles + r0 / ROWS) * 2 + r / 64) * 128 + r % 64;
                 st[0] = nlse;
                 st[64] = ndot;
@@ -485,24 +547,27 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                     ok = __all_sync(0xffffffffu,
                                     ok && mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
                 auto weights = [&](auto masked) {
+                    constexpr int N = COLS / C::SPLIT, CH = C::CHUNK;  // this group's columns, and how many at a time
+                    const uint32_t t1 = t + N * part, t2 = t1 + 64;
+                    const int cp = c0 + N * part;
+                    const float4* sp = st + N / 4 * part;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {  // 32 columns: weights h go over scores that are read already
-                        float s[32], u[32];
-                        tmem_ld32(t + 32 * h, s);
-                        tmem_ld32(t + 64 + 32 * h, u);
-                        uint32_t pw[16], dw[16];
+                    for (int h = 0; h < N; h += CH) {  // the weights go over scores that are read already
+                        float s[CH], u[CH];
+                        tmem_ld_pair<CH>(t1 + h, t2 + h, s, u);
+                        uint32_t pw[CH / 2], dw[CH / 2];
 #pragma unroll
-                        for (int c = 0; c < 32; c += 4) {
+                        for (int c = 0; c < CH; c += 4) {
                             float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
                             if (MODE == GRAD_KV) {
-                                nl = st[8 * h + c / 4];
-                                nd = st[16 + 8 * h + c / 4];
+                                nl = sp[(h + c) / 4];
+                                nd = sp[16 + (h + c) / 4];
                             }
 #pragma unroll
                             for (int e = 0; e < 4; e += 2) {
                                 const uint64_t n2 = e == 0 ? pack2(nl.x, nl.y) : pack2(nl.z, nl.w);
                                 const uint64_t d2 = e == 0 ? pack2(nd.x, nd.y) : pack2(nd.z, nd.w);
-                                const int cc = c0 + 32 * h + c + e;
+                                const int cc = cp + h + c + e;
                                 float x, y, gx, gy;
                                 unpack2(fma2(pack2(s[c + e], s[c + e + 1]), k22, n2), x, y);
                                 x = ex2_approx(x);
@@ -519,8 +584,8 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                                 dw[(c + e) / 2] = pack_pair<T>(gx, gy);
                             }
                         }
-                        if (MODE == GRAD_KV) tmem_st16(t + 16 * h, pw);
-                        tmem_st16(t + 64 + 16 * h, dw);
+                        if (MODE == GRAD_KV) tmem_st<CH / 2>(t1 + h / 2, pw);
+                        tmem_st<CH / 2>(t2 + h / 2, dw);
                     }
                 };
                 if (full)
@@ -605,24 +670,14 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 stage_box(acc + 64 * wg, f0, acc + HD + 64 * wg, f1, rows1 + wg * ROWS * 128);
                 send_box(&maps.out, rows1 + wg * ROWS * 128, 64 * wg);
             }
-        } else if constexpr (MODE == GRAD_Q) {
-            stage_box(acc + 64 * wg, f0, 0, 0.0f, rows1 + wg * ROWS * 128);
-            send_box(&maps.dq, rows1 + wg * ROWS * 128, 64 * wg);
         } else {
+            constexpr int PER = HD / 64, BOXES = MODE == GRAD_Q ? PER : 2 * PER;  // dq, or dk then dv
             const float fv = F16 ? 1.0f / 1024.0f : 1.0f;
-            if (NWG == 1 || wg == 0) {
 #pragma unroll 1
-                for (int i = 0; i < HD / 64; i++) {
-                    stage_box(acc + 64 * i, f0, 0, 0.0f, rows1 + i * ROWS * 128);
-                    send_box(&maps.dk, rows1 + i * ROWS * 128, 64 * i);
-                }
-            }
-            if (NWG == 1 || wg == 1) {
-#pragma unroll 1
-                for (int i = 0; i < HD / 64; i++) {
-                    stage_box(acc + HD + 64 * i, fv, 0, 0.0f, rows2 + i * ROWS * 128);
-                    send_box(&maps.dv, rows2 + i * ROWS * 128, 64 * i);
-                }
+            for (int i = grp; i < BOXES; i += C::GROUPS) {
+                uint8_t* box = rows1 + i * ROWS * 128;
+                stage_box(acc + 64 * i, i < PER ? f0 : fv, 0, 0.0f, box);
+                send_box(MODE == GRAD_Q ? &maps.dq : i < PER ? &maps.dk : &maps.dv, box, 64 * (i % PER));
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // staging read
