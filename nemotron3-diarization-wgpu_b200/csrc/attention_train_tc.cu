@@ -58,29 +58,36 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float RESCALE_LOG2 = 8.0f;  // forward: raise the running maximum when exponents would exceed 2^8
 constexpr int DEV_TIMEOUT_ATTN_TRAIN = 7;
 
-template <int HD, int MODE>
+// PARTS: 1 for 16-bit tensors, 2 for fp32 tensors as fp16 pairs h + l.
+template <int HD, int MODE, int PARTS>
 struct Cfg {
     static constexpr bool GRAD = MODE != FORWARD;
-    static constexpr int NWG = HD == 64 ? 1 : 2;            // column blocks in softmax at a time
-    static constexpr int SPLIT = GRAD && HD == 64 ? 2 : 1;   // groups of 4 warps that share a block's columns
+    static constexpr bool SMALL = HD == 64 && PARTS == 1;   // two blocks fit an SM
+    static constexpr int NWG = SMALL ? 1 : 2;               // column blocks in softmax at a time
+    static constexpr int SPLIT = GRAD && SMALL ? 2 : 1;     // groups of 4 warps that share a block's columns
     static constexpr int CHUNK = 16;                        // columns a thread has in registers at a time (gradients)
     static constexpr int GROUPS = NWG * SPLIT;
     static constexpr int NBUF = MODE == FORWARD ? 2 : NWG;  // score buffers
     static constexpr int SOFTMAX = 3;                       // first softmax warp
-    static constexpr int THREADS = 32 * SOFTMAX + 128 * GROUPS, PER_SM = HD == 128 ? 1 : 2;
-    static constexpr int RTILE = ROWS * HD * 2, CTILE = COLS * HD * 2;    // bytes
+    static constexpr int THREADS = 32 * SOFTMAX + 128 * GROUPS, PER_SM = SMALL ? 2 : 1;
+    static constexpr int RTILE = ROWS * HD * 2 * PARTS, CTILE = COLS * HD * 2 * PARTS;  // bytes
     static constexpr int STATS = MODE == GRAD_KV ? 512 : 0;               // 64 x (-lse log2 e), 64 x (-D)
-    static constexpr int STAGE = 2 * CTILE + 1024 * (STATS > 0), NST = 4;
+    static constexpr int STAT_LD = PARTS == 1 ? 128 : kSplitStat;         // floats of a block of 64 rows
+    static constexpr int STAGE = 2 * CTILE + 1024 * (STATS > 0);
     static constexpr int ROW_BYTES = (GRAD ? 2 : 1) * RTILE;
     // barriers and the TMEM slot, the groups' row statistics, and slack to align the tiles to 1024 bytes
-    static constexpr int SMEM = ROW_BYTES + NST * STAGE + 256 + (MODE == FORWARD && NWG > 1 ? 4 * 128 * 4 : 64) + 1024;
+    static constexpr int REST = 256 + (MODE == FORWARD && NWG > 1 ? 4 * 128 * 4 : 64) + 1024;
+    static constexpr int ROOM = 226 * 1024 / PER_SM - ROW_BYTES - REST;
+    static constexpr int NST = ROOM / STAGE > 4 ? 4 : ROOM / STAGE;
+    static constexpr int SMEM = ROW_BYTES + NST * STAGE + REST;
     static constexpr uint32_t TBUF = GRAD ? 128 : 64;                     // TMEM columns of a score buffer
     static constexpr uint32_t ACC = NBUF * TBUF;                          // first accumulator
     static constexpr int NACC = MODE == FORWARD ? NWG : MODE == GRAD_Q ? 1 : 2;
-    static constexpr uint32_t TMEM_COLS = HD == 128 ? 512 : 256;
+    static constexpr uint32_t TMEM_COLS = SMALL ? 256 : 512;
     static_assert(COLS / SPLIT % CHUNK == 0, "whole chunks");
+    static_assert(NBUF % NWG == 0, "a score buffer belongs to one softmax group");
     static_assert(ACC + NACC * HD <= TMEM_COLS && PER_SM * TMEM_COLS <= 512, "TMEM");
-    static_assert((SMEM + 1024) * PER_SM <= 228 * 1024, "shared memory");
+    static_assert(NST >= 1 && (SMEM + 1024) * PER_SM <= 228 * 1024, "shared memory");
 };
 
 // Instruction descriptor of kind::f16 with fp32 accumulators, M = 128; B K-major, or
@@ -195,6 +202,13 @@ __device__ __forceinline__ float inverse_power(float x) {
     return x > 0.0f && e > 0 && e < 254 ? __int_as_float((254 - e) << 23) : 1.0f;
 }
 
+// Pairs: the power of two that keeps |dS| times it within 2^15, from |dS| <= 2 |dout row| |v row| and
+// |v row| <= sqrt(head_dim) max|v|.
+template <int HD>
+__device__ __forceinline__ float pair_ds_scale(float norm, float v_max) {
+    return 0.5f * split_scale_of(norm * v_max * (HD == 64 ? 8.0f : 11.3137085f));
+}
+
 struct TcMaps {
     CUtensorMap q, k, v, dout;       // loads, 64-row boxes
     CUtensorMap out, dq, dk, dv;     // stores, 32-row boxes
@@ -206,16 +220,19 @@ struct TcArgs {
     int ascending;     // which end of a one-sided window is open: 1 if keys before the query
     float k2, factor;  // |scale| log2 e; the scale of dq and dk
     int negate;        // scale < 0
-    float* stats;      // [seqs * q_heads][q tiles][2][-lse log2 e: 64 | -D: 64]
-    float* norms;      // [seqs * q_heads][q tiles]: the largest |dout row|
+    float* stats;      // [seqs * q_heads][q tiles][2][-lse log2 e: 64 | -D: 64 (| pairs: |dout row|: 64)]
+    float* norms;      // [seqs * q_heads][q tiles]: the largest |dout row|; pairs: [seqs * q_heads]
+    const float* maxima;  // pairs: the largest |q|, |k|, |v|, |dout|
     int q_tiles;
 };
 
-template <class T, int HD, int MODE>
-__global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
+// T: the type of the MMA operands; tensors are of type T (PARTS 1) or fp32 (PARTS 2, T = fp16).
+template <class T, int HD, int MODE, int PARTS>
+__global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, PARTS>::PER_SM)
     attention_train_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs args) {
-    using C = Cfg<HD, MODE>;
-    constexpr bool F16 = std::is_same<T, __half>::value;
+    using C = Cfg<HD, MODE, PARTS>;
+    constexpr bool F16 = std::is_same<T, __half>::value, PAIR = PARTS == 2;
+    constexpr int RPART = ROWS * HD * 2, CPART = COLS * HD * 2;  // bytes of one part of a tile
     constexpr int NWG = C::NWG, NBUF = C::NBUF, NST = C::NST;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -286,13 +303,14 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
             const CUtensorMap* cm1 = MODE == GRAD_KV ? &maps.q : &maps.k;
             const CUtensorMap* cm2 = MODE == GRAD_KV ? &maps.dout : &maps.v;
             mbar_arrive_expect_tx(r_full, C::ROW_BYTES);
+            // part p of a pair is the maps' sequence p * seqs + seq
 #pragma unroll
-            for (int i = 0; i < HD / 64; i++)
+            for (int i = 0; i < PARTS * HD / 64; i++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {  // 64 rows each
-                    const int o = (2 * i + h) * BOX;
-                    tma_load_4d(rows1 + o, rm1, r_full, 64 * i, r0 + 64 * h, head, seq);
-                    if (C::GRAD) tma_load_4d(rows2 + o, rm2, r_full, 64 * i, r0 + 64 * h, head, seq);
+                    const int o = (2 * i + h) * BOX, d = i % (HD / 64) * 64, sq = i / (HD / 64) * a.seqs + seq;
+                    tma_load_4d(rows1 + o, rm1, r_full, d, r0 + 64 * h, head, sq);
+                    if (C::GRAD) tma_load_4d(rows2 + o, rm2, r_full, d, r0 + 64 * h, head, sq);
                 }
             int g = 0;
             for (; g < nblk; g++) {
@@ -303,13 +321,14 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 const int c0 = col0(g), ch = col_head(g);
                 mbar_arrive_expect_tx(bar, 2 * C::CTILE + C::STATS);
 #pragma unroll
-                for (int i = 0; i < HD / 64; i++) {
-                    tma_load_4d(st + i * BOX, cm1, bar, 64 * i, c0, ch, seq);
-                    tma_load_4d(st + C::CTILE + i * BOX, cm2, bar, 64 * i, c0, ch, seq);
+                for (int i = 0; i < PARTS * HD / 64; i++) {
+                    const int d = i % (HD / 64) * 64, sq = i / (HD / 64) * a.seqs + seq;
+                    tma_load_4d(st + i * BOX, cm1, bar, d, c0, ch, sq);
+                    tma_load_4d(st + C::CTILE + i * BOX, cm2, bar, d, c0, ch, sq);
                 }
                 if (MODE == GRAD_KV)
                     bulk_load(st + 2 * C::CTILE,
-                              args.stats + (((long long)seq * a.q_heads + ch) * args.q_tiles * 2 + c0 / COLS) * 128,
+                              args.stats + (((long long)seq * a.q_heads + ch) * args.q_tiles * 2 + c0 / COLS) * C::STAT_LD,
                               C::STATS, bar);
             }
             // every load has landed before the block may exit (already true unless a wait expired)
@@ -319,7 +338,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
         }
     } else if (warp == 1) {
         // ---- T1, T2
-        // zeros over rows [from, n) of a tile (boxes of n rows)
+        // zeros over rows [from, n) of a tile (boxes of n rows); pairs come with zeros there
         auto clear = [&](uint8_t* tile, int from, int n) {
             for (int i = 0; i < HD / 64; i++)
                 for (int x = from * 8 + lane; x < n * 8; x += 32)
@@ -329,7 +348,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
         bool ok = nblk > 0;
         if (ok) {
             ok = __all_sync(0xffffffffu, mbar_wait(r_full, 0, err, DEV_TIMEOUT_ATTN_TRAIN));
-            if (ok && r0 + ROWS > row_len && row_len < row_cap) {
+            if (!PAIR && ok && r0 + ROWS > row_len && row_len < row_cap) {
                 clear(rows1, max(row_len - r0, 0), ROWS);
                 if (C::GRAD) clear(rows2, max(row_len - r0, 0), ROWS);
                 fence_async_smem();
@@ -342,7 +361,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
             if (!ok) break;
             uint8_t* st = ring + (g % NST) * C::STAGE;
             const int c0 = col0(g);
-            if (c0 + COLS > col_len && col_len < col_cap) {
+            if (!PAIR && c0 + COLS > col_len && col_len < col_cap) {
                 clear(st, col_len - c0, COLS);
                 clear(st + C::CTILE, col_len - c0, COLS);
                 fence_async_smem();
@@ -350,24 +369,28 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
             }
             // T of block g overwrites the weights of block g - NBUF, which its second products have read
             // (phase g / NBUF - 1; the next needs this T)
-            if (g >= NBUF) ok = __all_sync(0xffffffffu, mbar_wait(&acc_done[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            if (g >= NBUF)
+                ok = __all_sync(0xffffffffu,
+                                mbar_wait(&acc_done[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
                 const uint32_t t = tmem + (g % NBUF) * C::TBUF;
+                // pairs: l h + h l + h h, the dropped l l is 2^-22 of the product
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; kk++) {
-                    const uint32_t ro = (kk / 4) * 2 * BOX + (kk % 4) * 32, co = (kk / 4) * BOX + (kk % 4) * 32;
-                    umma_f16(t, desc_k_sw128(r1 + ro), desc_k_sw128(b + co), args.negate ? t_neg : t_desc, kk != 0);
-                }
-                if (C::GRAD) {
+                for (int i = 0; i < (C::GRAD ? 2 : 1); i++)
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; kk++) {
-                        const uint32_t ro = (kk / 4) * 2 * BOX + (kk % 4) * 32, co = (kk / 4) * BOX + (kk % 4) * 32;
-                        umma_f16(t + 64, desc_k_sw128(r2 + ro), desc_k_sw128(b + C::CTILE + co), t_desc, kk != 0);
-                    }
-                }
+                    for (int kk = 0; kk < HD / 16; kk++)
+#pragma unroll
+                        for (int c = 0; c < (PAIR ? 3 : 1); c++) {
+                            const uint32_t ro = (i ? r2 : r1) + (PAIR && c == 0 ? RPART : 0) + (kk / 4) * 2 * BOX +
+                                                (kk % 4) * 32;
+                            const uint32_t co = b + i * C::CTILE + (PAIR && c == 1 ? CPART : 0) + (kk / 4) * BOX +
+                                                (kk % 4) * 32;
+                            umma_f16(t + 64 * i, desc_k_sw128(ro), desc_k_sw128(co),
+                                     i == 0 && args.negate ? t_neg : t_desc, kk + c != 0);
+                        }
                 umma_commit(&t_full[g % NBUF]);
             }
             __syncwarp();
@@ -375,8 +398,9 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
     } else if (warp == 2) {
         // ---- second products: P v (forward); dS k, or dS^T q and P^T dout
         constexpr uint32_t acc_desc = idesc<T>(HD, true);
-        // where the weights of columns 16 kk.. are: each group's over its own scores
-        auto weight_col = [](int kk) { return C::SPLIT == 1 ? 8 * kk : 32 * (kk / 2) + 8 * (kk % 2); };
+        // where the weights of columns 16 kk.. are: each group's over its own scores, a pair's h and l
+        // side by side
+        auto weight_col = [](int kk) { return PAIR ? 16 * kk : C::SPLIT == 1 ? 8 * kk : 32 * (kk / 2) + 8 * (kk % 2); };
         bool ok = true;
         for (int g = 0; ok && g < nblk; g++) {
             // the column tiles (as above) and the weights of block g (phase g / NBUF; the next needs T of
@@ -390,17 +414,17 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 const uint32_t t = tmem + (g % NBUF) * C::TBUF;
                 const uint32_t acc = tmem + C::ACC + (MODE == FORWARD ? (g % NWG) * HD : 0);
                 const uint32_t first = MODE == FORWARD ? g < NWG : g == 0;
-#pragma unroll
-                for (int kk = 0; kk < COLS / 16; kk++)
-                    umma_f16_ts(acc, t + (C::GRAD ? 64 : 0) + weight_col(kk),
-                                desc_mn_sw128(b + (MODE == FORWARD ? C::CTILE : 0) + kk * 2048), acc_desc,
-                                kk != 0 || !first);
-                if (MODE == GRAD_KV) {
+                auto second = [&](uint32_t d, uint32_t weights, uint32_t tile) {
 #pragma unroll
                     for (int kk = 0; kk < COLS / 16; kk++)
-                        umma_f16_ts(acc + HD, t + weight_col(kk), desc_mn_sw128(b + C::CTILE + kk * 2048), acc_desc,
-                                    kk != 0 || !first);
-                }
+#pragma unroll
+                        for (int c = 0; c < (PAIR ? 3 : 1); c++)
+                            umma_f16_ts(d, weights + weight_col(kk) + (PAIR && c == 0 ? 8 : 0),
+                                        desc_mn_sw128(tile + (PAIR && c == 1 ? CPART : 0) + kk * 2048), acc_desc,
+                                        kk + c != 0 || !first);
+                };
+                second(acc, t + (C::GRAD ? 64 : 0), b + (MODE == FORWARD ? C::CTILE : 0));
+                if (MODE == GRAD_KV) second(acc + HD, t, b + C::CTILE);
                 umma_commit(&acc_done[g % NBUF]);
                 umma_commit(&c_empty[g % NST]);
                 if (g == nblk - 1) umma_commit(all_done);
@@ -415,12 +439,28 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
         const bool live = row < row_len;
         const int lo = first_col(row), hi = last_col(row);
         const int full_lo = r_last >= r0 ? first_col(r_last) : 0, full_hi = r_last >= r0 ? last_col(r0) : 0;
-        const float k2 = args.k2;
+        // pairs: the powers of two that q, k, v and dout were multiplied by
+        float s_q = 1.0f, s_k = 1.0f, s_v = 1.0f, s_do = 1.0f, v_max = 0.0f;
+        if (PAIR) {
+            s_q = split_scale_of(args.maxima[0]);
+            s_k = split_scale_of(args.maxima[1]);
+            v_max = args.maxima[2];
+            s_v = split_scale_of(v_max);
+            if (C::GRAD) s_do = split_scale_of(args.maxima[3]);
+        }
+        const float k2 = PAIR ? args.k2 / s_q / s_k : args.k2;
+        const float dp_unit = PAIR ? 1.0f / s_do / s_v : 1.0f;  // T2 times this is dP
         bool ok = true;
 
         // dq: this row's -lse log2 e, -D and fp16 scale; dkv: the fp16 scale of the head group
         float nlse = 0.0f, ndot = 0.0f, ds_scale = 1.0f;
-        if (MODE == GRAD_Q) {
+        if (MODE == GRAD_Q && PAIR) {
+            const float* st =
+                args.stats + ((((long long)seq * a.q_heads + head) * args.q_tiles + r0 / ROWS) * 2 + r / 64) * C::STAT_LD + r % 64;
+            nlse = live ? st[0] : -INFINITY;
+            ndot = live ? st[64] : 0.0f;
+            ds_scale = pair_ds_scale<HD>(live ? st[128] : 0.0f, v_max);
+        } else if (MODE == GRAD_Q) {
             const long long sqh = (long long)seq * a.q_heads + head;
             float norm2 = 0.0f;
             nlse = -INFINITY;
@@ -462,14 +502,17 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
             }
         }
         if (MODE == GRAD_KV && F16) {
+            // the largest |dout row| of the head group: a pair has one for each head, otherwise one for each tile
             float m = 0.0f;
-            const float* n = args.norms + ((long long)seq * a.q_heads + head * group) * args.q_tiles;
-            for (int i = lane; i < group * args.q_tiles; i += 32) m = fmaxf(m, n[i]);
+            const int per = PAIR ? 1 : args.q_tiles;
+            const float* n = args.norms + ((long long)seq * a.q_heads + head * group) * per;
+            for (int i = lane; i < group * per; i += 32) m = fmaxf(m, n[i]);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            ds_scale = 8.0f * inverse_power(m);
+            ds_scale = PAIR ? pair_ds_scale<HD>(m, v_max) : 8.0f * inverse_power(m);
         }
-        constexpr float P_LOG2 = !F16 ? 0.0f : MODE == FORWARD ? 7.0f : MODE == GRAD_KV ? 10.0f : 0.0f;
+        constexpr float P_LOG2 = !F16 ? 0.0f : MODE == FORWARD ? 7.0f : MODE == GRAD_KV ? (PAIR ? 15.0f : 10.0f) : 0.0f;
+        constexpr float P_SCALE = PAIR ? 32768.0f : 1024.0f;  // 2^P_LOG2 of dkv
 
         float m = -INFINITY, l = 0.0f;  // forward: running maximum (raw scores) and sum (times 2^P_LOG2)
         for (int g = wg; g < nblk; g += NWG) {
@@ -504,7 +547,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                 const float off = m == -INFINITY ? 0.0f : P_LOG2 - m * k2;
                 const uint64_t k22 = pack2(k2, k2), off2 = pack2(off, off);
                 uint64_t sum2[4] = {0, 0, 0, 0};
-                uint32_t w[32];
+                uint32_t w[32 * PARTS];  // pairs: per 16 columns 8 words of h, then 8 of l
 #pragma unroll
                 for (int c = 0; c < 64; c += 2) {
                     float x, y;
@@ -512,7 +555,10 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                     x = ex2_approx(x);
                     y = ex2_approx(y);
                     sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], pack2(x, y));
-                    w[c / 2] = pack_pair<T>(x, y);
+                    if constexpr (PAIR)
+                        split2x2(x, y, 1.0f, w[c / 16 * 16 + c % 16 / 2], w[c / 16 * 16 + 8 + c % 16 / 2]);
+                    else
+                        w[c / 2] = pack_pair<T>(x, y);
                 }
                 float sa, sb;
                 unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sa, sb);
@@ -538,11 +584,11 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                         tmem_st16(acc + cb, u);
                     }
                 }
-                tmem_st16(t, w);
-                tmem_st16(t + 16, w + 16);
+#pragma unroll
+                for (int i = 0; i < 2 * PARTS; i++) tmem_st16(t + 16 * i, w + 16 * i);
             } else {
                 const float4* st = reinterpret_cast<const float4*>(ring + (g % NST) * C::STAGE + 2 * C::CTILE);
-                const uint64_t k22 = pack2(k2, k2), scale2 = pack2(ds_scale, ds_scale);
+                const uint64_t k22 = pack2(k2, k2), scale2 = pack2(ds_scale, ds_scale), unit2 = pack2(dp_unit, dp_unit);
                 if (MODE == GRAD_KV)  // the statistics came by bulk copy: this thread's own wait makes them visible
                     ok = __all_sync(0xffffffffu,
                                     ok && mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
@@ -555,7 +601,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                     for (int h = 0; h < N; h += CH) {  // the weights go over scores that are read already
                         float s[CH], u[CH];
                         tmem_ld_pair<CH>(t1 + h, t2 + h, s, u);
-                        uint32_t pw[CH / 2], dw[CH / 2];
+                        uint32_t pw[CH / 2 * PARTS], dw[CH / 2 * PARTS];  // pairs: h, then l
 #pragma unroll
                         for (int c = 0; c < CH; c += 4) {
                             float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
@@ -574,18 +620,25 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                                 y = ex2_approx(y);
                                 if (masked && (cc < lo || cc >= hi)) x = 0.0f;
                                 if (masked && (cc + 1 < lo || cc + 1 >= hi)) y = 0.0f;
-                                uint64_t g2 = mul2(pack2(x, y), add2(pack2(u[c + e], u[c + e + 1]), d2));
+                                const uint64_t u2 = pack2(u[c + e], u[c + e + 1]);
+                                uint64_t g2 = mul2(pack2(x, y), PAIR ? fma2(u2, unit2, d2) : add2(u2, d2));
                                 if (F16) g2 = mul2(g2, scale2);
                                 unpack2(g2, gx, gy);
                                 if (masked && x == 0.0f) gx = 0.0f;
                                 if (masked && y == 0.0f) gy = 0.0f;
-                                if (MODE == GRAD_KV)
-                                    pw[(c + e) / 2] = F16 ? pack_pair<T>(x * 1024.0f, y * 1024.0f) : pack_pair<T>(x, y);
-                                dw[(c + e) / 2] = pack_pair<T>(gx, gy);
+                                const int i = (c + e) / 2;
+                                if constexpr (PAIR) {
+                                    if (MODE == GRAD_KV) split2x2(x, y, P_SCALE, pw[i], pw[CH / 2 + i]);
+                                    split2x2(gx, gy, 1.0f, dw[i], dw[CH / 2 + i]);
+                                } else {
+                                    if (MODE == GRAD_KV)
+                                        pw[i] = F16 ? pack_pair<T>(x * P_SCALE, y * P_SCALE) : pack_pair<T>(x, y);
+                                    dw[i] = pack_pair<T>(gx, gy);
+                                }
                             }
                         }
-                        if (MODE == GRAD_KV) tmem_st<CH / 2>(t1 + h / 2, pw);
-                        tmem_st<CH / 2>(t2 + h / 2, dw);
+                        if (MODE == GRAD_KV) tmem_st<CH / 2 * PARTS>(t1 + h / 2 * PARTS, pw);
+                        tmem_st<CH / 2 * PARTS>(t2 + h / 2 * PARTS, dw);
                     }
                 };
                 if (full)
@@ -625,18 +678,22 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
             }
             if (a.lse && wg == 0 && row < a.q_rows)
                 a.lse[((long long)seq * a.q_heads + head) * a.q_rows + row] = live ? lse : -INFINITY;
+            f0 /= s_v;
+            f1 /= s_v;
         } else {
-            f0 = args.factor;
-            if (F16) f0 /= ds_scale;
+            f0 = args.factor / ds_scale / (MODE == GRAD_Q ? s_k : s_q);
         }
-        // 64 columns of one accumulator (plus those of a second one) to a row's 128 bytes of staging
+        const float fv = F16 ? 1.0f / P_SCALE / s_do : 1.0f;  // of dv
+        // 64 columns of one accumulator (plus those of a second one) to this row's staging: a row of 64
+        // elements, its 16-byte words swizzled by the row
+        constexpr int EL = PAIR ? 4 : 2, WORDS = 64 * EL / 16, ROW = 64 * EL;
         auto stage_box = [&](uint32_t acc, float f, uint32_t acc2, float g2, uint8_t* box) {
 #pragma unroll 1
             for (int cb = 0; cb < 64; cb += 16) {
                 float o[16], o2[16];
                 if (nblk > 0) tmem_ld16(acc + cb, o);
                 if (acc2 && nblk > 1) tmem_ld16(acc2 + cb, o2);
-                uint32_t w[8];
+                uint32_t w[4 * EL];
 #pragma unroll
                 for (int d = 0; d < 16; d += 2) {
                     float x = 0.0f, y = 0.0f;
@@ -644,41 +701,58 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
                         x = o[d] * f, y = o[d + 1] * f;
                         if (acc2 && nblk > 1) x += o2[d] * g2, y += o2[d + 1] * g2;
                     }
-                    w[d / 2] = pack_pair<T>(x, y);
+                    if constexpr (PAIR)
+                        w[d] = __float_as_uint(x), w[d + 1] = __float_as_uint(y);
+                    else
+                        w[d / 2] = pack_pair<T>(x, y);
                 }
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-                    *reinterpret_cast<uint4*>(box + r * 128 + (((cb / 8 + i) ^ (r & 7)) << 4)) =
+                for (int i = 0; i < EL; i++)
+                    *reinterpret_cast<uint4*>(box + r * ROW + (((cb * EL / 16 + i) ^ (r & (WORDS - 1))) << 4)) =
                         make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
             }
         };
-        auto send_box = [&](const CUtensorMap* map, uint8_t* box, int d) {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0 && r0 + qd * 32 < row_cap) {
-                tma_store_4d(map, box + qd * 32 * 128, d, r0 + qd * 32, head, seq);
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        // a warp's 32 rows of the staging: one TMA store of 16-bit rows; fp32 rows, whose tensors may have
+        // any strides, two rows at a time
+        auto send_box = [&](const CUtensorMap* map, const HeadsView& t, uint8_t* box, int d) {
+            const int first = r0 + qd * 32;
+            if constexpr (PAIR) {
+                __syncwarp();
+                const int word = lane % 16;
+                float* p = static_cast<float*>(t.p) + (long long)seq * t.seq + (long long)head * t.head + d + 4 * word;
+                const bool wide = ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(t.row * 4)) & 15) == 0;
+                for (int i = lane / 16; i < 32 && first + i < row_cap; i += 2) {
+                    const int rr = qd * 32 + i;
+                    const float4 v = *reinterpret_cast<const float4*>(box + rr * ROW + ((word ^ (rr & 15)) << 4));
+                    float* to = p + (long long)(first + i) * t.row;
+                    if (wide)
+                        *reinterpret_cast<float4*>(to) = v;
+                    else
+                        to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+                }
+            } else {
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0 && first < row_cap) {
+                    tma_store_4d(map, box + qd * 32 * ROW, d, first, head, seq);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
             }
         };
-        // the row tiles are no longer read: they hold the staging, a box of 128 rows each
+        // the row tiles are no longer read: they hold the staging, a box of 128 rows for every 64 columns
         const uint32_t acc = lb + C::ACC;
-        if constexpr (MODE == FORWARD) {
-            if (NWG == 1) {
-                stage_box(acc, f0, 0, 0.0f, rows1);
-                send_box(&maps.out, rows1, 0);
-            } else {
-                stage_box(acc + 64 * wg, f0, acc + HD + 64 * wg, f1, rows1 + wg * ROWS * 128);
-                send_box(&maps.out, rows1 + wg * ROWS * 128, 64 * wg);
-            }
-        } else {
-            constexpr int PER = HD / 64, BOXES = MODE == GRAD_Q ? PER : 2 * PER;  // dq, or dk then dv
-            const float fv = F16 ? 1.0f / 1024.0f : 1.0f;
+        constexpr int PER = HD / 64, BOXES = MODE == GRAD_KV ? 2 * PER : PER;  // out, dq, or dk then dv
+        static_assert(BOXES * ROWS * ROW <= C::ROW_BYTES, "the staging fits the row tiles");
 #pragma unroll 1
-            for (int i = grp; i < BOXES; i += C::GROUPS) {
-                uint8_t* box = rows1 + i * ROWS * 128;
-                stage_box(acc + 64 * i, i < PER ? f0 : fv, 0, 0.0f, box);
-                send_box(MODE == GRAD_Q ? &maps.dq : i < PER ? &maps.dk : &maps.dv, box, 64 * (i % PER));
-            }
+        for (int i = grp; i < BOXES; i += C::GROUPS) {
+            uint8_t* box = rows1 + i * ROWS * ROW;
+            const int d = 64 * (i % PER);
+            if (MODE == FORWARD)
+                stage_box(acc + d, f0, NWG > 1 ? acc + HD + d : 0, f1, box);
+            else
+                stage_box(acc + 64 * i, MODE == GRAD_KV && i >= PER ? fv : f0, 0, 0.0f, box);
+            send_box(MODE == FORWARD ? &maps.out : MODE == GRAD_Q ? &maps.dq : i < PER ? &maps.dk : &maps.dv,
+                     MODE == FORWARD ? a.o : MODE == GRAD_Q ? a.dq : i < PER ? a.dk : a.dv, box, d);
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // staging read
     }
@@ -687,12 +761,12 @@ __global__ void __launch_bounds__(Cfg<HD, MODE>::THREADS, Cfg<HD, MODE>::PER_SM)
     if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
-template <class T, int HD, int MODE>
-void launch(cudaStream_t s, const AttnArgs& a) {
-    using C = Cfg<HD, MODE>;
+template <class T, int HD, int MODE, int PARTS>
+void launch(cudaStream_t s, const AttnArgs& a, const AttnSplitSpace* sp) {
+    using C = Cfg<HD, MODE, PARTS>;
     static std::atomic<unsigned long long> attr{0};
     once_per_device(attr, [] {
-        N3D_CUDA(cudaFuncSetAttribute(attention_train_tc_kernel<T, HD, MODE>,
+        N3D_CUDA(cudaFuncSetAttribute(attention_train_tc_kernel<T, HD, MODE, PARTS>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     });
     const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -706,17 +780,23 @@ void launch(cudaStream_t s, const AttnArgs& a) {
     auto map = [&](const HeadsView& v, int n, int h, int box) {
         return make_heads_map(v.p, bf16, a.seqs, n, h, HD, v.seq, v.row, v.head, box);
     };
+    // an operand: the tensor itself, or its pair [part][seqs][heads][rows][HD]
+    auto operand = [&](const HeadsView& v, void* pair, int n, int h) {
+        if (PARTS == 1) return map(v, n, h, 64);
+        return make_heads_map(pair, false, 2LL * a.seqs, n, h, HD, (long long)h * n * HD, HD, (long long)n * HD, 64);
+    };
+    const AttnSplitSpace none{};
+    const AttnSplitSpace& p = sp ? *sp : none;
     TcMaps m{};
     // a tensor without rows is never loaded: any valid map stands in for its own
-    const HeadsView& any = MODE == GRAD_KV ? a.k : a.q;
-    const CUtensorMap stand_in = map(any, rows, heads, 64);
-    m.q = a.q_rows ? map(a.q, a.q_rows, a.q_heads, 64) : stand_in;
-    m.k = a.k_rows ? map(a.k, a.k_rows, a.k_heads, 64) : stand_in;
-    m.v = a.k_rows ? map(a.v, a.k_rows, a.k_heads, 64) : stand_in;
-    if (MODE != FORWARD) m.dout = a.q_rows ? map(a.dout, a.q_rows, a.q_heads, 64) : stand_in;
-    if (MODE == FORWARD) m.out = map(a.o, a.q_rows, a.q_heads, 32);
-    if (MODE == GRAD_Q) m.dq = map(a.dq, a.q_rows, a.q_heads, 32);
-    if (MODE == GRAD_KV) {
+    const CUtensorMap stand_in = MODE == GRAD_KV ? operand(a.k, p.k, rows, heads) : operand(a.q, p.q, rows, heads);
+    m.q = a.q_rows ? operand(a.q, p.q, a.q_rows, a.q_heads) : stand_in;
+    m.k = a.k_rows ? operand(a.k, p.k, a.k_rows, a.k_heads) : stand_in;
+    m.v = a.k_rows ? operand(a.v, p.v, a.k_rows, a.k_heads) : stand_in;
+    if (MODE != FORWARD) m.dout = a.q_rows ? operand(a.dout, p.dout, a.q_rows, a.q_heads) : stand_in;
+    if (PARTS == 1 && MODE == FORWARD) m.out = map(a.o, a.q_rows, a.q_heads, 32);
+    if (PARTS == 1 && MODE == GRAD_Q) m.dq = map(a.dq, a.q_rows, a.q_heads, 32);
+    if (PARTS == 1 && MODE == GRAD_KV) {
         m.dk = map(a.dk, a.k_rows, a.k_heads, 32);
         m.dv = map(a.dv, a.k_rows, a.k_heads, 32);
     }
@@ -727,20 +807,26 @@ void launch(cudaStream_t s, const AttnArgs& a) {
     t.factor = a.scale;
     t.negate = a.scale < 0.0f;
     t.q_tiles = (a.q_rows + ROWS - 1) / ROWS;
-    t.stats = a.row_dot;
-    t.norms = a.row_dot + (size_t)a.seqs * a.q_heads * t.q_tiles * 256;
-    launch_pdl(attention_train_tc_kernel<T, HD, MODE>, dim3((unsigned)blocks), dim3(C::THREADS), C::SMEM, s, m, t);
+    if (PARTS == 1) {
+        t.stats = a.row_dot;
+        t.norms = a.row_dot + (size_t)a.seqs * a.q_heads * t.q_tiles * 256;
+    } else {
+        t.stats = p.stats;
+        t.norms = p.head_norm;
+        t.maxima = p.maxima;
+    }
+    launch_pdl(attention_train_tc_kernel<T, HD, MODE, PARTS>, dim3((unsigned)blocks), dim3(C::THREADS), C::SMEM, s, m, t);
 }
 
-template <class T, int HD>
-void launch_modes(cudaStream_t s, const AttnArgs& a, bool backward) {
-    if (!backward) return launch<T, HD, FORWARD>(s, a);
-    launch<T, HD, GRAD_Q>(s, a);
-    launch<T, HD, GRAD_KV>(s, a);
+template <class T, int HD, int PARTS>
+void launch_modes(cudaStream_t s, const AttnArgs& a, bool backward, const AttnSplitSpace* sp) {
+    if (!backward) return launch<T, HD, FORWARD, PARTS>(s, a, sp);
+    launch<T, HD, GRAD_Q, PARTS>(s, a, sp);
+    launch<T, HD, GRAD_KV, PARTS>(s, a, sp);
 }
-template <class T>
-void launch_dim(cudaStream_t s, const AttnArgs& a, bool backward) {
-    a.head_dim == 64 ? launch_modes<T, 64>(s, a, backward) : launch_modes<T, 128>(s, a, backward);
+template <class T, int PARTS>
+void launch_dim(cudaStream_t s, const AttnArgs& a, bool backward, const AttnSplitSpace* sp) {
+    a.head_dim == 64 ? launch_modes<T, 64, PARTS>(s, a, backward, sp) : launch_modes<T, 128, PARTS>(s, a, backward, sp);
 }
 
 // Whole 16-byte words, and strides that a tensor map can hold (above 0, below 2^40 bytes).
@@ -753,15 +839,28 @@ bool tma_view(const HeadsView& v, long long seqs, long long rows, long long head
 }  // namespace
 
 bool attention_tc_fits(const AttnArgs& a, int dtype, bool backward) {
-    if (dtype == N3D_F32) return false;
+    if (dtype == N3D_F32) return attention_split_pays(a.seqs, a.q_heads, a.q_rows, a.k_rows);
     auto q_side = [&](const HeadsView& v) { return tma_view(v, a.seqs, a.q_rows, a.q_heads); };
     auto k_side = [&](const HeadsView& v) { return tma_view(v, a.seqs, a.k_rows, a.k_heads); };
     const bool f = q_side(a.q) && q_side(a.o) && k_side(a.k) && k_side(a.v);
     return f && (!backward || (q_side(a.dout) && q_side(a.dq) && k_side(a.dk) && k_side(a.dv)));
 }
 
+bool attention_split_pays(size_t seqs, size_t q_heads, size_t q_rows, size_t k_rows) {
+    return seqs * q_heads * q_rows * k_rows > 0;
+}
+
 void launch_attention_train_tc(cudaStream_t s, const AttnArgs& a, int dtype, bool backward) {
-    dtype == N3D_BF16 ? launch_dim<__nv_bfloat16>(s, a, backward) : launch_dim<__half>(s, a, backward);
+    if (dtype == N3D_F32) {
+        AttnSplitSpace sp;
+        attn_split_space(a.row_dot, a.seqs, a.q_heads, a.k_heads, a.q_rows, a.k_rows, a.head_dim, backward, &sp);
+        launch_attention_split(s, a, sp, backward);
+        launch_dim<__half, 2>(s, a, backward, &sp);
+    } else if (dtype == N3D_BF16) {
+        launch_dim<__nv_bfloat16, 1>(s, a, backward, nullptr);
+    } else {
+        launch_dim<__half, 1>(s, a, backward, nullptr);
+    }
 }
 
 }  // namespace n3d

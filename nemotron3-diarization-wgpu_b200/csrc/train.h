@@ -65,7 +65,7 @@ void launch_residual_norm_grad(cudaStream_t s, const ResidualArgs& a, int residu
 struct AttnArgs {
     HeadsView q, k, v, o, dout, dq, dk, dv;
     float* lse;         // [seqs, q_heads, q_rows], null: not wanted (forward)
-    float* row_dot;     // workspace of attn_workspace_floats(): row statistics of the gradient
+    float* row_dot;     // the workspace
     int* err;           // where an expired wait records its site
     int seqs, q_rows, k_rows, q_heads, k_heads, head_dim;
     float scale;
@@ -100,16 +100,33 @@ struct AttnMask {
     }
 #endif
 };
-// Workspace of the gradient: on the fp32 units dout . out of each row; on the tensor cores
-// two blocks of 128 floats for every 128 query rows of a head (row statistics of 64 rows
-// each) and one float (the largest |dout row| of the 128).
+// Workspace of the gradient of 16-bit tensors, in floats: on the fp32 units dout . out of each
+// row; on the tensor cores two blocks of 128 for every 128 query rows of a head (row
+// statistics of 64 rows each) and one (the largest |dout row| of the 128).
 inline size_t attn_workspace_floats(size_t seqs, size_t q_heads, size_t q_rows) {
     return seqs * q_heads * ((q_rows + 127) / 128) * (2 * 128 + 1);
 }
+// Workspace of fp32 tensors on the tensor cores (attention_train_split.cu): the largest
+// magnitudes, the statistics, and each operand as two fp16 arrays [part][seqs][heads][rows][hd].
+constexpr int kSplitBlocks = 296;  // blocks that look for a tensor's largest magnitude
+constexpr int kSplitStat = 192;    // floats per 64 query rows: -lse log2 e | -D | |dout row|
+struct AttnSplitSpace {
+    float* maxima;     // [4]: q, k, v, dout
+    float* partial;    // [4][kSplitBlocks]
+    float* head_norm;  // [seqs * q_heads]: the largest |dout row|
+    float* stats;      // [seqs * q_heads][q tiles of 128][2][kSplitStat]
+    void *q, *k, *v, *dout;
+};
+// Lays the workspace out at `base` (may be null) and returns its size in bytes.
+size_t attn_split_space(void* base, size_t seqs, size_t q_heads, size_t k_heads, size_t q_rows, size_t k_rows,
+                        size_t head_dim, bool backward, AttnSplitSpace* out);
+void launch_attention_split(cudaStream_t s, const AttnArgs& a, const AttnSplitSpace& sp, bool backward);
 // attention_train_tc.cu: whether the call's tensors fit TMA (16-bit types, whole 16-byte
-// words, no broadcast dimension), and the launches.
+// words, no broadcast dimension), and the launches; fp32 tensors go through the split.
 bool attention_tc_fits(const AttnArgs& a, int dtype, bool backward);
 void launch_attention_train_tc(cudaStream_t s, const AttnArgs& a, int dtype, bool backward);
+// Whether fp32 tensors of these sizes are split for the tensor cores.
+bool attention_split_pays(size_t seqs, size_t q_heads, size_t q_rows, size_t k_rows);
 void launch_attention_forward(cudaStream_t s, const AttnArgs& a, int dtype);
 void launch_attention_backward(cudaStream_t s, const AttnArgs& a, int dtype);
 

@@ -391,9 +391,13 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config* cfg, co
 }
 
 size_t n3d_attention_workspace(const n3d_attn_config* cfg, size_t q_heads, size_t k_heads, int backward) {
-    if (!cfg || q_heads > 65535 || k_heads > 65535 || cfg->seqs > (size_t)INT_MAX || cfg->q_rows > (size_t)1 << 30)
+    if (!cfg || q_heads > 65535 || k_heads > 65535 || cfg->seqs > (size_t)INT_MAX || cfg->q_rows > (size_t)1 << 30 ||
+        cfg->k_rows > (size_t)1 << 30 || (cfg->head_dim != 64 && cfg->head_dim != 128))
         return 0;
-    return backward ? n3d::attn_workspace_floats(cfg->seqs, q_heads, cfg->q_rows) * sizeof(float) : 0;
+    const size_t rows = backward ? n3d::attn_workspace_floats(cfg->seqs, q_heads, cfg->q_rows) * sizeof(float) : 0;
+    if (cfg->dtype != N3D_F32 || !n3d::attention_split_pays(cfg->seqs, q_heads, cfg->q_rows, cfg->k_rows)) return rows;
+    return std::max(rows, n3d::attn_split_space(nullptr, cfg->seqs, q_heads, k_heads, cfg->q_rows, cfg->k_rows,
+                                                cfg->head_dim, backward != 0, nullptr));
 }
 
 n3d_status n3d_attention_forward(int device, const n3d_attn_config* cfg, const n3d_heads* q, const n3d_heads* k,
@@ -405,6 +409,7 @@ n3d_status n3d_attention_forward(int device, const n3d_attn_config* cfg, const n
         n3d::AttnArgs a = attn_args(*cfg, q, k, v, out, true, d_q_len, d_k_len);
         check_workspace(n3d_attention_workspace(cfg, q->heads, k->heads, 0), d_workspace, workspace_bytes);
         a.lse = d_lse;
+        a.row_dot = static_cast<float*>(d_workspace);
         if (cfg->seqs == 0 || cfg->q_rows == 0) return;
         DeviceGuard g(device);
         a.err = train_error(device);
