@@ -33,6 +33,13 @@
 // two, so that small weights and gradients keep fp16's precision; |dS| <= 2 P |dout row|
 // |v row| then stays inside fp16 while |v row| < 4096.
 //
+// fp32: every operand is a pair h + l of fp16 arrays (attention_train_split.cu), P and dS are split
+// in the softmax, and each product is l h + h l + h h.  The tensor cores' fp32 accumulators
+// truncate: about 2^-26 of the accumulator per MMA, always towards zero, which 12 MMAs a block
+// carry to 1.5e-5 at 4096 rows.  So an accumulator takes two blocks, the small products
+// of each first, and is then added to a sum that is rounded to nearest (more TMEM, or the
+// output tensor).
+//
 // Rows past a sequence's length: TMA fills what lies past the tensor with zeros, and the
 // T warp overwrites what lies past the length with zeros before a tile is used, so
 // nothing that stands there enters a product.  Pairs that the mask hides are cleared by a
@@ -54,7 +61,7 @@ namespace {
 enum Mode { FORWARD, GRAD_Q, GRAD_KV };
 constexpr int ROWS = 128, COLS = 64;
 constexpr int BOX = 64 * 128;  // a TMA box: 64 rows of 64 elements
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_LOG2 = 8.0f;  // forward: raise the running maximum when exponents would exceed 2^8
 constexpr int DEV_TIMEOUT_ATTN_TRAIN = 7;
 
@@ -63,7 +70,9 @@ template <int HD, int MODE, int PARTS>
 struct Cfg {
     static constexpr bool GRAD = MODE != FORWARD;
     static constexpr bool SMALL = HD == 64 && PARTS == 1;   // two blocks fit an SM
-    static constexpr int NWG = SMALL ? 1 : 2;               // column blocks in softmax at a time
+    static constexpr bool PAIR = PARTS == 2;
+    // column blocks in softmax at a time (an fp32 forward pass of head_dim 128 has TMEM for one)
+    static constexpr int NWG = SMALL || (PAIR && HD == 128 && MODE == FORWARD) ? 1 : 2;
     static constexpr int SPLIT = GRAD && SMALL ? 2 : 1;     // groups of 4 warps that share a block's columns
     static constexpr int CHUNK = 16;                        // columns a thread has in registers at a time (gradients)
     static constexpr int GROUPS = NWG * SPLIT;
@@ -76,17 +85,20 @@ struct Cfg {
     static constexpr int STAGE = 2 * CTILE + 1024 * (STATS > 0);
     static constexpr int ROW_BYTES = (GRAD ? 2 : 1) * RTILE;
     // barriers and the TMEM slot, the groups' row statistics, and slack to align the tiles to 1024 bytes
-    static constexpr int REST = 256 + (MODE == FORWARD && NWG > 1 ? 4 * 128 * 4 : 64) + 1024;
+    static constexpr int REST = 256 + (MODE == FORWARD && NWG > 1 ? (4 + 2 * PAIR) * 128 * 4 : 64) + 1024;
     static constexpr int ROOM = 226 * 1024 / PER_SM - ROW_BYTES - REST;
     static constexpr int NST = ROOM / STAGE > 4 ? 4 : ROOM / STAGE;
     static constexpr int SMEM = ROW_BYTES + NST * STAGE + REST;
     static constexpr uint32_t TBUF = GRAD ? 128 : 64;                     // TMEM columns of a score buffer
     static constexpr uint32_t ACC = NBUF * TBUF;                          // first accumulator
     static constexpr int NACC = MODE == FORWARD ? NWG : MODE == GRAD_Q ? 1 : 2;
+    // pairs: the accumulators are added up after them (see the head of the file); dk and dv
+    // of head_dim 128 are added up in the output tensors, for which there is no TMEM
+    static constexpr bool SUM = PAIR, SUM_OUT = PAIR && HD == 128 && MODE == GRAD_KV;
     static constexpr uint32_t TMEM_COLS = SMALL ? 256 : 512;
     static_assert(COLS / SPLIT % CHUNK == 0, "whole chunks");
     static_assert(NBUF % NWG == 0, "a score buffer belongs to one softmax group");
-    static_assert(ACC + NACC * HD <= TMEM_COLS && PER_SM * TMEM_COLS <= 512, "TMEM");
+    static_assert(ACC + (SUM && !SUM_OUT ? 2 : 1) * NACC * HD <= TMEM_COLS && PER_SM * TMEM_COLS <= 512, "TMEM");
     static_assert(NST >= 1 && (SMEM + 1024) * PER_SM <= 228 * 1024, "shared memory");
 };
 
@@ -202,6 +214,16 @@ __device__ __forceinline__ float inverse_power(float x) {
     return x > 0.0f && e > 0 && e < 254 ? __int_as_float((254 - e) << 23) : 1.0f;
 }
 
+// ln(l 2^(m k2 - shift)) for a row sum l >= 0: -inf for an empty row.  The exponent and the logarithm
+// of the mantissa are added in fp64, so that the result carries little more than its own rounding.
+__device__ __forceinline__ float row_lse(float l, float m, float k2, float shift) {
+    if (l == 0.0f) return -INFINITY;
+    if (!(l < INFINITY)) return l;
+    const int bits = __float_as_int(l);
+    const float mantissa = __int_as_float((bits & 0x7fffff) | 0x3f800000);
+    const double t = (double)m * (double)k2 + ((double)((bits >> 23) - 127) - (double)shift) + (double)log2f(mantissa);
+    return (float)(t * 0.6931471805599453);
+}
 // Pairs: the power of two that keeps |dS| times it within 2^15, from |dS| <= 2 |dout row| |v row| and
 // |v row| <= sqrt(head_dim) max|v|.
 template <int HD>
@@ -246,10 +268,11 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
     uint64_t* t_full = c_empty + NST;      // NBUF: T of block g completed (buffer g % NBUF)
     uint64_t* p_full = t_full + NBUF;      // NBUF: weights of block g written (4 warps)
     uint64_t* acc_done = p_full + NBUF;    // NBUF: second product of block g completed
-    uint64_t* all_done = acc_done + NBUF;  // 1: the last one completed
+    uint64_t* acc_free = acc_done + NBUF;  // NWG (pairs): the accumulator is added to its sum (4 warps)
+    uint64_t* all_done = acc_free + NWG;   // 1: the last one completed
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
     float* join = reinterpret_cast<float*>(bars + 32);  // forward with two groups: [2][128] maxima; then sums
-    static_assert(1 + 2 * NST + 3 * NBUF + 2 <= 32, "barriers and the TMEM slot fill at most 256 bytes");
+    static_assert(1 + 2 * NST + 3 * NBUF + NWG + 2 <= 32, "barriers and the TMEM slot fill at most 256 bytes");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0 && lane == 0) {
@@ -257,6 +280,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         for (int i = 0; i < NST; i++) mbar_init(&c_full[i], 1), mbar_init(&c_empty[i], 1);
         for (int i = 0; i < NBUF; i++)
             mbar_init(&t_full[i], 1), mbar_init(&p_full[i], 4 * C::SPLIT), mbar_init(&acc_done[i], 1);
+        for (int i = 0; i < NWG; i++) mbar_init(&acc_free[i], 4);
         mbar_init(all_done, 1);
         mbar_fence_init();
     }
@@ -377,13 +401,14 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             if (elect_one()) {
                 const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
                 const uint32_t t = tmem + (g % NBUF) * C::TBUF;
-                // pairs: l h + h l + h h, the dropped l l is 2^-22 of the product
+                // pairs: l h + h l + h h, the small products first (the accumulator truncates); the dropped
+                // l l is 2^-22 of the product
 #pragma unroll
                 for (int i = 0; i < (C::GRAD ? 2 : 1); i++)
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; kk++)
+                    for (int c = 0; c < (PAIR ? 3 : 1); c++)
 #pragma unroll
-                        for (int c = 0; c < (PAIR ? 3 : 1); c++) {
+                        for (int kk = 0; kk < HD / 16; kk++) {
                             const uint32_t ro = (i ? r2 : r1) + (PAIR && c == 0 ? RPART : 0) + (kk / 4) * 2 * BOX +
                                                 (kk % 4) * 32;
                             const uint32_t co = b + i * C::CTILE + (PAIR && c == 1 ? CPART : 0) + (kk / 4) * BOX +
@@ -407,18 +432,24 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             // block g + NBUF, hence this product)
             ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN) &&
                                              mbar_wait(&p_full[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            // block number of its accumulator: a pair's starts afresh every second one, once the softmax group
+            // has added it up (phase n / 2 - 1; the next needs this product)
+            const int n = MODE == FORWARD ? g / NWG : g;
+            if (C::SUM && ok && n >= 2 && n % 2 == 0)
+                ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[MODE == FORWARD ? g % NWG : 0], (n / 2 - 1) & 1, err,
+                                                       DEV_TIMEOUT_ATTN_TRAIN));
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t b = smem_u32(ring + (g % NST) * C::STAGE);
                 const uint32_t t = tmem + (g % NBUF) * C::TBUF;
                 const uint32_t acc = tmem + C::ACC + (MODE == FORWARD ? (g % NWG) * HD : 0);
-                const uint32_t first = MODE == FORWARD ? g < NWG : g == 0;
+                const uint32_t first = C::SUM ? n % 2 == 0 : n == 0;
                 auto second = [&](uint32_t d, uint32_t weights, uint32_t tile) {
 #pragma unroll
-                    for (int kk = 0; kk < COLS / 16; kk++)
+                    for (int c = 0; c < (PAIR ? 3 : 1); c++)
 #pragma unroll
-                        for (int c = 0; c < (PAIR ? 3 : 1); c++)
+                        for (int kk = 0; kk < COLS / 16; kk++)
                             umma_f16_ts(d, weights + weight_col(kk) + (PAIR && c == 0 ? 8 : 0),
                                         desc_mn_sw128(tile + (PAIR && c == 1 ? CPART : 0) + kk * 2048), acc_desc,
                                         kk + c != 0 || !first);
@@ -451,6 +482,10 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         const float k2 = PAIR ? args.k2 / s_q / s_k : args.k2;
         const float dp_unit = PAIR ? 1.0f / s_do / s_v : 1.0f;  // T2 times this is dP
         bool ok = true;
+        // this row in a fp32 output
+        auto out_row = [&](const HeadsView& t) {
+            return static_cast<float*>(t.p) + (long long)seq * t.seq + (long long)head * t.head + (long long)row * t.row;
+        };
 
         // dq: this row's -lse log2 e, -D and fp16 scale; dkv: the fp16 scale of the head group
         float nlse = 0.0f, ndot = 0.0f, ds_scale = 1.0f;
@@ -515,6 +550,8 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         constexpr float P_SCALE = PAIR ? 32768.0f : 1024.0f;  // 2^P_LOG2 of dkv
 
         float m = -INFINITY, l = 0.0f;  // forward: running maximum (raw scores) and sum (times 2^P_LOG2)
+        float m_sum = -INFINITY;        // pairs, forward: the maximum that the summed accumulators refer to
+        auto sum_factor = [&](float to) { return m_sum == to ? 1.0f : ex2_approx((m_sum - to) * k2); };
         for (int g = wg; g < nblk; g += NWG) {
             const int buf = g % NBUF, c0 = col0(g);
             const uint32_t t = lb + buf * C::TBUF;
@@ -563,7 +600,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 float sa, sb;
                 unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sa, sb);
                 l = l * corr + (sa + sb);
-                if (g >= NWG && __any_sync(0xffffffffu, raise)) {
+                if (g >= NWG && !(C::SUM && g / NWG % 2 == 0) && __any_sync(0xffffffffu, raise)) {
                     // this group's previous product (its phase: the buffer's next product needs P of
                     // this or a later block of the group)
                     ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_done[(g - NWG) % NBUF], ((g - NWG) / NBUF) & 1, err,
@@ -650,20 +687,58 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[buf]);
+
+            // pairs: after every second product into an accumulator, if another follows, add it to the sum
+            const int n = MODE == FORWARD ? g / NWG : g;
+            if (C::SUM && n % 2 == 1 && g + (MODE == FORWARD ? NWG : 1) < nblk) {
+                // (its phase: the buffer's next product needs weights of this group)
+                ok = __all_sync(0xffffffffu,
+                                ok && mbar_wait(&acc_done[buf], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                tc_fence_after();
+                const float f = MODE == FORWARD ? sum_factor(m) : 1.0f;
+                const uint32_t from = lb + C::ACC + (MODE == FORWARD ? wg * HD : 0);
+                constexpr int WIDTH = MODE == GRAD_KV ? 2 * HD : HD;
+#pragma unroll 1
+                for (int cb = 0; cb < WIDTH; cb += 16) {
+                    float o[16], u[16];
+                    tmem_ld16(from + cb, o);
+                    if constexpr (C::SUM_OUT) {
+                        if (live) {
+                            float* to = out_row(cb < HD ? a.dk : a.dv) + cb % HD;
+#pragma unroll
+                            for (int d = 0; d < 16; d++) to[d] = n == 1 ? o[d] : to[d] + o[d];
+                        }
+                    } else {
+                        if (n > 1) tmem_ld16(from + C::NACC * HD + cb, u);
+                        uint32_t w[16];
+#pragma unroll
+                        for (int d = 0; d < 16; d++) w[d] = __float_as_uint(n > 1 ? u[d] * f + o[d] : o[d]);
+                        tmem_st16(from + C::NACC * HD + cb, w);
+                    }
+                }
+                m_sum = m;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_free[MODE == FORWARD ? wg : 0]);
+            }
         }
 
         // ---- the accumulators, once every product has completed
         if (nblk > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(all_done, 0, err, DEV_TIMEOUT_ATTN_TRAIN));
         tc_fence_after();
+        if (C::SUM_OUT) asm volatile("bar.sync 1, 256;" ::: "memory");  // the sums in the outputs are written
         float f0 = 0.0f, f1 = 0.0f;  // what the accumulator(s) are multiplied by
+        float g0 = 0.0f, g1 = 0.0f;  // and their sums
         if (MODE == FORWARD) {
             float lse;
             if (NWG == 1) {
                 f0 = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN;
-                lse = l == 0.0f ? -INFINITY : (m * k2 + log2f(l) - P_LOG2) * LN2;
+                lse = row_lse(l, m, k2, P_LOG2);
             } else {
                 join[wg * 128 + r] = m;
                 join[256 + wg * 128 + r] = l;
+                if (C::SUM) join[512 + wg * 128 + r] = sum_factor(m);
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 const float m0 = join[r], m1 = join[128 + r], l0 = join[256 + r], l1 = join[256 + 128 + r];
                 const float mm = fmaxf(m0, m1);
@@ -674,32 +749,50 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : NAN;
                 f0 = e0 * inv;
                 f1 = nblk > 1 ? e1 * inv : 0.0f;
-                lse = sum == 0.0f ? -INFINITY : (mm * k2 + log2f(sum) - P_LOG2) * LN2;
+                lse = row_lse(sum, mm, k2, P_LOG2);
             }
             if (a.lse && wg == 0 && row < a.q_rows)
                 a.lse[((long long)seq * a.q_heads + head) * a.q_rows + row] = live ? lse : -INFINITY;
             f0 /= s_v;
             f1 /= s_v;
+            if (C::SUM) {
+                g0 = f0 * (NWG == 1 ? sum_factor(m) : join[512 + r]);
+                g1 = f1 * join[512 + 128 + r];
+            }
         } else {
             f0 = args.factor / ds_scale / (MODE == GRAD_Q ? s_k : s_q);
+            g0 = f0;
         }
         const float fv = F16 ? 1.0f / P_SCALE / s_do : 1.0f;  // of dv
-        // 64 columns of one accumulator (plus those of a second one) to this row's staging: a row of 64
+        // 64 columns of an accumulator (plus what belongs to it) to this row's staging: a row of 64
         // elements, its 16-byte words swizzled by the row
         constexpr int EL = PAIR ? 4 : 2, WORDS = 64 * EL / 16, ROW = 64 * EL;
-        auto stage_box = [&](uint32_t acc, float f, uint32_t acc2, float g2, uint8_t* box) {
+        // (second: the other group's accumulator; summed: what was added up before)
+        const bool second = MODE == FORWARD && NWG > 1 && nblk > 1;
+        const bool summed = C::SUM && nblk > 2 * (MODE == FORWARD ? NWG : 1), summed2 = C::SUM && second && nblk > 2 * NWG + 1;
+        auto stage_box = [&](uint32_t acc, float f, float gs, const float* sum_row, uint8_t* box) {
+            const uint32_t acc2 = acc + HD, sum = acc + C::NACC * HD;
 #pragma unroll 1
             for (int cb = 0; cb < 64; cb += 16) {
-                float o[16], o2[16];
+                float o[16], o2[16], u[16], u2[16];
                 if (nblk > 0) tmem_ld16(acc + cb, o);
-                if (acc2 && nblk > 1) tmem_ld16(acc2 + cb, o2);
+                if (second) tmem_ld16(acc2 + cb, o2);
+                if (C::SUM_OUT) {
+#pragma unroll
+                    for (int d = 0; d < 16; d++) u[d] = summed && live ? sum_row[cb + d] : 0.0f;
+                } else if (summed) {
+                    tmem_ld16(sum + cb, u);
+                }
+                if (summed2) tmem_ld16(sum + HD + cb, u2);
                 uint32_t w[4 * EL];
 #pragma unroll
                 for (int d = 0; d < 16; d += 2) {
                     float x = 0.0f, y = 0.0f;
                     if (live && nblk > 0) {
                         x = o[d] * f, y = o[d + 1] * f;
-                        if (acc2 && nblk > 1) x += o2[d] * g2, y += o2[d + 1] * g2;
+                        if (summed) x += u[d] * gs, y += u[d + 1] * gs;
+                        if (second) x += o2[d] * f1, y += o2[d + 1] * f1;
+                        if (summed2) x += u2[d] * g1, y += u2[d + 1] * g1;
                     }
                     if constexpr (PAIR)
                         w[d] = __float_as_uint(x), w[d + 1] = __float_as_uint(y);
@@ -747,10 +840,9 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         for (int i = grp; i < BOXES; i += C::GROUPS) {
             uint8_t* box = rows1 + i * ROWS * ROW;
             const int d = 64 * (i % PER);
-            if (MODE == FORWARD)
-                stage_box(acc + d, f0, NWG > 1 ? acc + HD + d : 0, f1, box);
-            else
-                stage_box(acc + 64 * i, MODE == GRAD_KV && i >= PER ? fv : f0, 0, 0.0f, box);
+            const bool is_dv = MODE == GRAD_KV && i >= PER;
+            stage_box(acc + 64 * i, is_dv ? fv : f0, is_dv ? fv : g0,
+                      C::SUM_OUT ? out_row(is_dv ? a.dv : a.dk) + d : nullptr, box);
             send_box(MODE == FORWARD ? &maps.out : MODE == GRAD_Q ? &maps.dq : i < PER ? &maps.dk : &maps.dv,
                      MODE == FORWARD ? a.o : MODE == GRAD_Q ? a.dq : i < PER ? a.dk : a.dv, box, d);
         }
@@ -839,15 +931,19 @@ bool tma_view(const HeadsView& v, long long seqs, long long rows, long long head
 }  // namespace
 
 bool attention_tc_fits(const AttnArgs& a, int dtype, bool backward) {
-    if (dtype == N3D_F32) return attention_split_pays(a.seqs, a.q_heads, a.q_rows, a.k_rows);
+    if (dtype == N3D_F32) return attention_split_pays(a.q_rows, a.k_rows, backward);
     auto q_side = [&](const HeadsView& v) { return tma_view(v, a.seqs, a.q_rows, a.q_heads); };
     auto k_side = [&](const HeadsView& v) { return tma_view(v, a.seqs, a.k_rows, a.k_heads); };
     const bool f = q_side(a.q) && q_side(a.o) && k_side(a.k) && k_side(a.v);
     return f && (!backward || (q_side(a.dout) && q_side(a.dq) && k_side(a.dk) && k_side(a.dv)));
 }
 
-bool attention_split_pays(size_t seqs, size_t q_heads, size_t q_rows, size_t k_rows) {
-    return seqs * q_heads * q_rows * k_rows > 0;
+// The split's two launches and its blocks of one per SM cost more than they save where all of a head is
+// one tile of the fp32 units: forward, 32 sequences x 8 heads of 64 rows take 35 us against 18 there, 128 of
+// 32 rows 91 against 52; 8 of 128 rows 21 against 20, 8 of 256 rows 31 against 49.  The gradient is at
+// least even everywhere (1 x 64 rows 21 us against 41, 128 x 32 rows 188 against 174).
+bool attention_split_pays(size_t q_rows, size_t k_rows, bool backward) {
+    return q_rows > 0 && k_rows > 0 && (backward || q_rows > 64 || k_rows > 64);
 }
 
 void launch_attention_train_tc(cudaStream_t s, const AttnArgs& a, int dtype, bool backward) {

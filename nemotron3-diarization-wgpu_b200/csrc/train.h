@@ -126,7 +126,7 @@ void launch_attention_split(cudaStream_t s, const AttnArgs& a, const AttnSplitSp
 bool attention_tc_fits(const AttnArgs& a, int dtype, bool backward);
 void launch_attention_train_tc(cudaStream_t s, const AttnArgs& a, int dtype, bool backward);
 // Whether fp32 tensors of these sizes are split for the tensor cores.
-bool attention_split_pays(size_t seqs, size_t q_heads, size_t q_rows, size_t k_rows);
+bool attention_split_pays(size_t q_rows, size_t k_rows, bool backward);
 void launch_attention_forward(cudaStream_t s, const AttnArgs& a, int dtype);
 void launch_attention_backward(cudaStream_t s, const AttnArgs& a, int dtype);
 

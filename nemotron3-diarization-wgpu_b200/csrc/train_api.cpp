@@ -395,7 +395,7 @@ size_t n3d_attention_workspace(const n3d_attn_config* cfg, size_t q_heads, size_
         cfg->k_rows > (size_t)1 << 30 || (cfg->head_dim != 64 && cfg->head_dim != 128))
         return 0;
     const size_t rows = backward ? n3d::attn_workspace_floats(cfg->seqs, q_heads, cfg->q_rows) * sizeof(float) : 0;
-    if (cfg->dtype != N3D_F32 || !n3d::attention_split_pays(cfg->seqs, q_heads, cfg->q_rows, cfg->k_rows)) return rows;
+    if (cfg->dtype != N3D_F32 || !n3d::attention_split_pays(cfg->q_rows, cfg->k_rows, backward != 0)) return rows;
     return std::max(rows, n3d::attn_split_space(nullptr, cfg->seqs, q_heads, k_heads, cfg->q_rows, cfg->k_rows,
                                                 cfg->head_dim, backward != 0, nullptr));
 }
