@@ -127,17 +127,17 @@ void launch_type(cudaStream_t s, const ResidualArgs& a) {
     if (!a.wide)
         C <= 1024 ? launch<RT, BT, 1, 32, 32>(s, a) : launch<RT, BT, 1, 256, 32>(s, a);
     else if (C <= 256)
-        launch<RT, BT, 8, 32, 8>(s, a);
+        launch<RT, BT, 4, 32, 8>(s, a);
     else if (C <= 512)
-        launch<RT, BT, 8, 32, 16>(s, a);
+        launch<RT, BT, 4, 32, 16>(s, a);
     else if (C <= 1024)
-        launch<RT, BT, 8, 32, 32>(s, a);
+        launch<RT, BT, 4, 32, 32>(s, a);
     else if (C <= 2048)
-        launch<RT, BT, 8, 128, 16>(s, a);
+        launch<RT, BT, 4, 128, 16>(s, a);
     else if (C <= 4096)
-        launch<RT, BT, 8, 256, 16>(s, a);
+        launch<RT, BT, 4, 256, 16>(s, a);
     else
-        launch<RT, BT, 8, 512, 16>(s, a);
+        launch<RT, BT, 4, 512, 16>(s, a);
 }
 
 }  // namespace

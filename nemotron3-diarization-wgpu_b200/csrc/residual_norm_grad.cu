@@ -11,14 +11,14 @@
 // Row statistics are taken again from r and block, which are read anyway: nothing of the
 // forward call is kept, and the statistics are those of the r at hand.
 //
-// Bound: memory (r, dr, block, dy read once, dx, dblock written once).  The column sums
-// (weights, biases, gate) stay in registers: a row's columns belong to the same threads
-// for all rows of a slot, 8 columns a thread, so each of the five sums costs 8 registers.
-// A slot is a contiguous range of rows; the next row's loads are issued before the
-// current row's three sums over the row.  Slots of a block are added through shared
-// memory, blocks by a second kernel, in a fixed order.  A gate row's gradient is complete
-// when its rows lie in one slot; at the borders of slots partial sums go to the workspace
-// and the second kernel adds them.
+// Bound: memory (r, dr, block, dy read once, dx, dblock written once); what costs time is
+// the latency of three sums over each row, so that many rows must be in work.  A row has
+// one thread for every 16 columns, and a slot of threads takes a contiguous range of rows.
+// The column sums (weights, biases, gate) of a slot are in shared memory, where each
+// thread alone adds to its 16 columns: in registers they would take up to 80 a thread.  Slots of a
+// block are added at the end, blocks by a second kernel, in a fixed order.  A gate row's
+// gradient is complete when its rows lie in one slot; at the borders of slots partial
+// sums go to the workspace and the second kernel adds them.
 
 #include <algorithm>
 #include <climits>
@@ -29,45 +29,53 @@ namespace n3d {
 
 namespace {
 
-constexpr int EPT = 8;  // columns of a thread
-
 __host__ __device__ inline long long slot_begin(long long rows, int slots, int i) { return rows * i / slots; }
 
-template <class RT, class BT, int VEC, int TPR>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : 2)
+// TPR threads a row, EPT columns a thread, R rows at a time.
+template <int TPR, int EPT>
+struct GradCfg {
+    static constexpr int THREADS = TPR > 256 ? TPR : 256, SLOTS = THREADS / TPR, PER_SM = 512 / THREADS;
+    static constexpr int SUM = THREADS * EPT;  // floats of one column sum of the block
+    static constexpr int BYTES = 5 * SUM * 4;
+};
+enum { POST_W, POST_B, PRE_W, PRE_B, GATE };  // the column sums
+
+template <class RT, class BT, int VEC, int TPR, int EPT, int R>
+__global__ void __launch_bounds__(GradCfg<TPR, EPT>::THREADS, GradCfg<TPR, EPT>::PER_SM)
     residual_norm_grad_kernel(const __grid_constant__ ResidualArgs a) {
-    constexpr int CH = EPT / VEC;
-    constexpr int THREADS = TPR > 256 ? TPR : 256, SLOTS = THREADS / TPR;
-    __shared__ float sums[SLOTS][9][TPR / 32];
-    __shared__ float part[SLOTS > 1 ? THREADS * EPT : 1];
+    using Cfg = GradCfg<TPR, EPT>;
+    constexpr int CH = EPT / VEC, SLOTS = Cfg::SLOTS;
+    extern __shared__ float4 smem4[];
+    __shared__ float sums[SLOTS][8 * R][TPR / 32];
     griddep_wait();
     griddep_launch_dependents();
     const int local = threadIdx.x / TPR, t = threadIdx.x % TPR;
     const int slot = blockIdx.x * SLOTS + local;
     const int C = a.cols;
     const float inv_c = 1.0f / (float)C;
-    float dgate[EPT] = {}, dpw[EPT] = {}, dpb[EPT] = {}, dqw[EPT] = {}, dqb[EPT] = {};  // p: post, q: pre
     const bool pre = a.pre != N3D_NORM_NONE, post = a.post != N3D_NORM_NONE;
+    // this thread's values of a column sum: 16-byte words, those of neighbours side by side
+    float* const mine = reinterpret_cast<float*>(smem4) + 4 * threadIdx.x;
+    auto at = [&](int which, int i) -> float4& {  // its columns 4 i ..
+        return *reinterpret_cast<float4*>(mine + which * Cfg::SUM + i * (Cfg::THREADS * 4));
+    };
+    auto add = [&](int which, int k, const float (&v)[VEC]) {  // the columns of chunk k
+        if constexpr (VEC == 4) {
+            float4 f = at(which, k);
+            f.x += v[0], f.y += v[1], f.z += v[2], f.w += v[3];
+            at(which, k) = f;
+        } else {
+            (&at(which, k / 4).x)[k % 4] += v[0];
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < 5; k++)
+#pragma unroll
+        for (int i = 0; i < EPT / 4; i++) at(k, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
     if (slot < a.slots) {
         const long long begin = slot_begin(a.rows, a.slots, slot), end = slot_begin(a.rows, a.slots, slot + 1);
-        Vec<RT, VEC> rv[CH], drv[CH];
-        Vec<BT, VEC> bv[CH], dyv[CH];
-        auto fetch = [&](long long row) {
-#pragma unroll
-            for (int k = 0; k < CH; k++) {
-                const int c = chunk_col<VEC, TPR>(k, t);
-                if (c < C) {
-                    if (pre) {
-                        rv[k].load_rw(static_cast<const RT*>(a.r) + row * a.ld_r + c);
-                        dyv[k].load_rw(static_cast<const BT*>(a.dy) + row * a.ld_dy + c);
-                    }
-                    if (a.dr) drv[k].load_rw(static_cast<const RT*>(a.dr) + row * a.ld_dr + c);
-                    bv[k].load_rw(static_cast<const BT*>(a.block) + row * a.ld_block + c);
-                }
-            }
-        };
-        // the gate row of the rows summed in dgate; flushed when it ends
+        // the gate row of the rows summed so far; flushed when it ends
         long long gate_row = a.rows_per_gate ? begin / a.rows_per_gate : 0;
         long long gate_end = a.rows_per_gate ? (gate_row + 1) * a.rows_per_gate : LLONG_MAX;
         auto flush_gate = [&](long long upto) {  // rows below `upto` are summed
@@ -78,159 +86,238 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : 2)
             else if (g1 > upto)
                 out = a.gate_parts + ((long long)slot * 2 + 1) * C;  // ends in a later one
 #pragma unroll
-            for (int k = 0; k < CH; k++) {
-                const int c = chunk_col<VEC, TPR>(k, t);
-                if (c < C) {
-                    if constexpr (VEC == 1) {
-                        out[c] = dgate[k];
-                    } else {
+            for (int i = 0; i < EPT / 4; i++) {
+                const float4 f = at(GATE, i);
+                at(GATE, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if constexpr (VEC == 1) {
+                    const float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-                        for (int i = 0; i < VEC; i += 4)
-                            *reinterpret_cast<float4*>(out + c + i) =
-                                make_float4(dgate[k * VEC + i], dgate[k * VEC + i + 1], dgate[k * VEC + i + 2],
-                                            dgate[k * VEC + i + 3]);
-                    }
+                    for (int j = 0; j < 4; j++)
+                        if (chunk_col<1, TPR>(4 * i + j, t) < C) out[chunk_col<1, TPR>(4 * i + j, t)] = v[j];
+                } else if (chunk_col<VEC, TPR>(i, t) < C) {
+                    *reinterpret_cast<float4*>(out + chunk_col<VEC, TPR>(i, t)) = f;
                 }
             }
-#pragma unroll
-            for (int i = 0; i < EPT; i++) dgate[i] = 0.0f;
         };
 
-        fetch(begin);
-        for (long long row = begin; row < end; row++) {
-            float h[EPT], g[EPT], b[EPT], d[EPT];  // r (then h), dy (then g), block (then k), dr (then dx)
-#pragma unroll
-            for (int i = 0; i < EPT; i++) h[i] = g[i] = b[i] = d[i] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < CH; k++)
-                if (chunk_col<VEC, TPR>(k, t) < C) {
-                    if (pre) {
-                        rv[k].get(h + k * VEC);
-                        dyv[k].get(g + k * VEC);
-                    }
-                    if (a.dr) drv[k].get(d + k * VEC);
-                    bv[k].get(b + k * VEC);
-                }
-            if (row + 1 < end) fetch(row + 1);
-            if (a.rows_per_gate && row == gate_end) {
+        long long row = begin;
+        while (row < end) {
+            if (row == gate_end) {
                 if (a.dgate) flush_gate(row);
                 gate_row++;
                 gate_end += a.rows_per_gate;
             }
-            float dy[EPT];
+            // R rows of one gate row, or what is left of it; the others are zeros, which add nothing
+            const int n = (int)min((long long)R, min(end, gate_end) - row);
+            Vec<RT, VEC> drv[R][CH];
+            Vec<BT, VEC> dyv[R][CH];
+            float h[R][EPT], g[R][EPT], b[R][EPT];  // r (then h), dy w (then e), block (then k)
+            {
+                Vec<RT, VEC> rv[R][CH];
+                Vec<BT, VEC> bv[R][CH];
 #pragma unroll
-            for (int k = 0; k < CH; k++) {
-                const int c = chunk_col<VEC, TPR>(k, t);
-                float w[VEC];
-                if (pre && c < C) load_weights<VEC>(a.pre_w, c, 1.0f, w);
+                for (int q = 0; q < R; q++)
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    dy[k * VEC + i] = g[k * VEC + i];
-                    if (pre && c < C) g[k * VEC + i] *= w[i];
+                    for (int k = 0; k < CH; k++) {
+                        const int c = chunk_col<VEC, TPR>(k, t);
+                        rv[q][k] = {}, dyv[q][k] = {}, bv[q][k] = {}, drv[q][k] = {};
+                        if (c < C && q < n) {
+                            if (pre) {
+                                rv[q][k].load_rw(static_cast<const RT*>(a.r) + (row + q) * a.ld_r + c);
+                                dyv[q][k].load_rw(static_cast<const BT*>(a.dy) + (row + q) * a.ld_dy + c);
+                            }
+                            bv[q][k].load_rw(static_cast<const BT*>(a.block) + (row + q) * a.ld_block + c);
+                            if (a.dr) drv[q][k].load_rw(static_cast<const RT*>(a.dr) + (row + q) * a.ld_dr + c);
+                        }
+                    }
+#pragma unroll
+                for (int k = 0; k < CH; k++) {
+                    const int c = chunk_col<VEC, TPR>(k, t);
+                    float w[VEC];
+                    load_weights<VEC>(c < C ? a.pre_w : nullptr, c, 1.0f, w);
+#pragma unroll
+                    for (int q = 0; q < R; q++) {
+                        rv[q][k].get(h[q] + k * VEC);
+                        dyv[q][k].get(g[q] + k * VEC);
+                        bv[q][k].get(b[q] + k * VEC);
+#pragma unroll
+                        for (int i = 0; i < VEC; i++) g[q][k * VEC + i] *= w[i];
+                    }
                 }
             }
-            // ---- sums of r, block and g
-            float s1[3] = {0.0f, 0.0f, 0.0f};
+            // ---- means of r, block and g, where a norm subtracts them
+            float mean_g[R] = {};
+            if (a.pre == N3D_NORM_LAYER || a.post == N3D_NORM_LAYER) {
+                float s1[3 * R] = {};
 #pragma unroll
-            for (int i = 0; i < EPT; i++) s1[0] += h[i], s1[1] += b[i], s1[2] += g[i];
-            row_sums<TPR>(s1, sums[local][0], local);
-            const float mean_r = a.pre == N3D_NORM_LAYER ? s1[0] * inv_c : 0.0f;
-            const float mean_b = a.post == N3D_NORM_LAYER ? s1[1] * inv_c : 0.0f;
-            const float mean_g = a.pre == N3D_NORM_LAYER ? s1[2] * inv_c : 0.0f;
+                for (int q = 0; q < R; q++)
+#pragma unroll
+                    for (int i = 0; i < EPT; i++)
+                        s1[3 * q] += h[q][i], s1[3 * q + 1] += b[q][i], s1[3 * q + 2] += g[q][i];
+                row_sums<TPR>(s1, sums[local][0], local);
+#pragma unroll
+                for (int q = 0; q < R; q++) {
+                    const float mean_r = a.pre == N3D_NORM_LAYER ? s1[3 * q] * inv_c : 0.0f;
+                    const float mean_b = a.post == N3D_NORM_LAYER ? s1[3 * q + 1] * inv_c : 0.0f;
+                    mean_g[q] = a.pre == N3D_NORM_LAYER ? s1[3 * q + 2] * inv_c : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < EPT; i++) h[q][i] -= mean_r, b[q][i] -= mean_b;
+                }
+            }
             // ---- squares of the centred values, and g against r
-            float s2[3] = {0.0f, 0.0f, 0.0f};
+            float s2[3 * R] = {};
 #pragma unroll
             for (int k = 0; k < CH; k++)
                 if (chunk_col<VEC, TPR>(k, t) < C)
 #pragma unroll
-                    for (int i = k * VEC; i < (k + 1) * VEC; i++) {
-                        h[i] -= mean_r;
-                        b[i] -= mean_b;
-                        s2[0] += h[i] * h[i];
-                        s2[1] += b[i] * b[i];
-                        s2[2] += g[i] * h[i];
-                    }
-            row_sums<TPR>(s2, sums[local][3], local);
-            const float rstd_r = pre ? rsqrtf(s2[0] * inv_c + a.pre_eps) : 0.0f;
-            const float rstd_b = post ? rsqrtf(s2[1] * inv_c + a.post_eps) : 1.0f;
-            const float mean_gh = s2[2] * inv_c * rstd_r;
+                    for (int q = 0; q < R; q++)
+#pragma unroll
+                        for (int i = k * VEC; i < (k + 1) * VEC; i++) {
+                            s2[3 * q] += h[q][i] * h[q][i];
+                            s2[3 * q + 1] += b[q][i] * b[q][i];
+                            s2[3 * q + 2] += g[q][i] * h[q][i];
+                        }
+            row_sums<TPR>(s2, sums[local][3 * R], local);
+            float rstd_b[R], s3[2 * R] = {};
             const float* gate = a.rows_per_gate ? a.gate + gate_row * C : nullptr;
-            float s3[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < CH; k++) {
-                const int c = chunk_col<VEC, TPR>(k, t);
-                if (c >= C) continue;
-                float gt[VEC], w[VEC], bias[VEC];
-                load_weights<VEC>(gate, c, 1.0f, gt);
-                load_weights<VEC>(post ? a.post_w : nullptr, c, 1.0f, w);
-                load_weights<VEC>(post ? a.post_b : nullptr, c, 0.0f, bias);
+            for (int q = 0; q < R; q++) {
+                const float rstd_r = pre ? rsqrtf(s2[3 * q] * inv_c + a.pre_eps) : 0.0f;
+                const float mean_gh = s2[3 * q + 2] * inv_c * rstd_r;
+                rstd_b[q] = post ? rsqrtf(s2[3 * q + 1] * inv_c + a.post_eps) : 1.0f;
 #pragma unroll
-                for (int j = 0; j < VEC; j++) {
-                    const int i = k * VEC + j;
-                    h[i] *= rstd_r;
-                    d[i] += rstd_r * (g[i] - mean_g - h[i] * mean_gh);
-                    dqw[i] += dy[i] * h[i];
-                    dqb[i] += dy[i];
-                    b[i] *= rstd_b;
-                    const float sd = a.scale * d[i];
-                    dgate[i] += sd * (b[i] * w[j] + bias[j]);
-                    const float du = sd * gt[j];
-                    dpw[i] += du * b[i];
-                    dpb[i] += du;
-                    g[i] = du * w[j];  // e
-                    s3[0] += g[i];
-                    s3[1] += g[i] * b[i];
+                for (int i = 0; i < EPT; i++) {
+                    h[q][i] *= rstd_r;
+                    g[q][i] = rstd_r * (g[q][i] - mean_g[q] - h[q][i] * mean_gh);
+                    b[q][i] *= rstd_b[q];
                 }
-                Vec<RT, VEC> o;
-                o.set(d + k * VEC);
-                o.store(static_cast<RT*>(a.dx) + row * a.ld_dx + c);
-            }
-            // ---- e, and e against k
-            float mean_e = 0.0f, mean_ek = 0.0f;
-            if (post) {
-                row_sums<TPR>(s3, sums[local][6], local);
-                mean_e = a.post == N3D_NORM_LAYER ? s3[0] * inv_c : 0.0f;
-                mean_ek = s3[1] * inv_c;
             }
 #pragma unroll
             for (int k = 0; k < CH; k++) {
                 const int c = chunk_col<VEC, TPR>(k, t);
                 if (c >= C) continue;
+                float v[VEC], d[VEC];
+                // dy h and dy
+                if (a.dpre_w || a.dpre_b) {
+                    float u[VEC];
 #pragma unroll
-                for (int i = k * VEC; i < (k + 1) * VEC; i++) g[i] = rstd_b * (g[i] - mean_e - b[i] * mean_ek);
-                Vec<BT, VEC> o;
-                o.set(g + k * VEC);
-                o.store(static_cast<BT*>(a.dblock) + row * a.ld_dblock + c);
+                    for (int i = 0; i < VEC; i++) u[i] = v[i] = 0.0f;
+#pragma unroll
+                    for (int q = 0; q < R; q++) {
+                        dyv[q][k].get(d);
+#pragma unroll
+                        for (int i = 0; i < VEC; i++) u[i] += d[i], v[i] += d[i] * h[q][k * VEC + i];
+                    }
+                    if (a.dpre_w) add(PRE_W, k, v);
+                    if (a.dpre_b) add(PRE_B, k, u);
+                }
+                // dx; from here g is scale dx
+#pragma unroll
+                for (int q = 0; q < R; q++) {
+                    float* gq = g[q] + k * VEC;
+                    if (a.dr) {
+                        drv[q][k].get(d);
+#pragma unroll
+                        for (int i = 0; i < VEC; i++) gq[i] += d[i];
+                    }
+                    if (q < n) {
+                        Vec<RT, VEC> o;
+                        o.set(gq);
+                        o.store(static_cast<RT*>(a.dx) + (row + q) * a.ld_dx + c);
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) gq[i] *= a.scale;
+                }
+                float w[VEC];
+                load_weights<VEC>(post ? a.post_w : nullptr, c, 1.0f, w);
+                if (a.dgate) {
+                    load_weights<VEC>(post ? a.post_b : nullptr, c, 0.0f, d);
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        v[i] = 0.0f;
+#pragma unroll
+                        for (int q = 0; q < R; q++) v[i] += g[q][k * VEC + i] * (b[q][k * VEC + i] * w[i] + d[i]);
+                    }
+                    add(GATE, k, v);
+                }
+                load_weights<VEC>(gate, c, 1.0f, d);
+#pragma unroll
+                for (int q = 0; q < R; q++)
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) g[q][k * VEC + i] *= d[i];
+                if (a.dpost_b) {
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        v[i] = 0.0f;
+#pragma unroll
+                        for (int q = 0; q < R; q++) v[i] += g[q][k * VEC + i];
+                    }
+                    add(POST_B, k, v);
+                }
+                if (a.dpost_w) {
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        v[i] = 0.0f;
+#pragma unroll
+                        for (int q = 0; q < R; q++) v[i] += g[q][k * VEC + i] * b[q][k * VEC + i];
+                    }
+                    add(POST_W, k, v);
+                }
+                // e, and e against k
+#pragma unroll
+                for (int q = 0; q < R; q++)
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        float& e = g[q][k * VEC + i];
+                        e *= w[i];
+                        s3[2 * q] += e;
+                        s3[2 * q + 1] += e * b[q][k * VEC + i];
+                    }
             }
+            if (post) row_sums<TPR>(s3, sums[local][6 * R], local);
+#pragma unroll
+            for (int q = 0; q < R; q++) {
+                if (q >= n) continue;
+                const float mean_e = a.post == N3D_NORM_LAYER ? s3[2 * q] * inv_c : 0.0f;
+                const float mean_ek = post ? s3[2 * q + 1] * inv_c : 0.0f;
+#pragma unroll
+                for (int k = 0; k < CH; k++) {
+                    const int c = chunk_col<VEC, TPR>(k, t);
+                    if (c >= C) continue;
+                    float v[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; i++)
+                        v[i] = rstd_b[q] * (g[q][k * VEC + i] - mean_e - b[q][k * VEC + i] * mean_ek);
+                    Vec<BT, VEC> o;
+                    o.set(v);
+                    o.store(static_cast<BT*>(a.dblock) + (row + q) * a.ld_dblock + c);
+                }
+            }
+            row += n;
         }
         if (a.dgate) flush_gate(end);
     }
-    // ---- the block's slots, then its sums to the workspace
-    float* mine = a.sums + (long long)blockIdx.x * 4 * C;
-    auto emit = [&](float (&v)[EPT], int which) {
-        if constexpr (SLOTS > 1) {
-            __syncthreads();
+    // ---- the slots of the block in order, to the workspace
+    __syncthreads();
+    float* out = a.sums + (long long)blockIdx.x * 4 * C;
+    for (int which = 0; which < 4; which++) {
+        const float* wanted = which == POST_W ? a.dpost_w : which == POST_B ? a.dpost_b : which == PRE_W ? a.dpre_w : a.dpre_b;
+        if (!wanted || local != 0) continue;
 #pragma unroll
-            for (int i = 0; i < EPT; i++) part[(local * EPT + i) * TPR + t] = v[i];
-            __syncthreads();
-            if (local == 0)
-#pragma unroll
-                for (int i = 0; i < EPT; i++)
-                    for (int o = 1; o < SLOTS; o++) v[i] += part[(o * EPT + i) * TPR + t];
-        }
-        if (local == 0)
-#pragma unroll
-            for (int k = 0; k < CH; k++) {
-                const int c = chunk_col<VEC, TPR>(k, t);
-                if (c < C)
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) mine[(long long)which * C + c + i] = v[k * VEC + i];
+        for (int i = 0; i < EPT / 4; i++) {
+            float4 f = at(which, i);
+            for (int o = 1; o < SLOTS; o++) {
+                const float4 e = *(&at(which, i) + o * TPR);
+                f.x += e.x, f.y += e.y, f.z += e.z, f.w += e.w;
             }
-    };
-    if (a.dpost_w) emit(dpw, 0);
-    if (a.dpost_b) emit(dpb, 1);
-    if (a.dpre_w) emit(dqw, 2);
-    if (a.dpre_b) emit(dqb, 3);
+            const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int c = VEC == 1 ? chunk_col<VEC, TPR>(4 * i + j, t) : chunk_col<VEC, TPR>(i, t) + j;
+                if (c < C) out[(long long)which * C + c] = v[j];
+            }
+        }
+    }
 }
 
 // Adds the partial sums: blockIdx.y < 4 the blocks' weight and bias sums, the others the
@@ -277,43 +364,48 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-template <class RT, class BT, int VEC, int TPR>
+template <class RT, class BT, int VEC, int TPR, int EPT, int R>
 void launch(cudaStream_t s, const ResidualArgs& a, const ResidualSplit& sp) {
-    constexpr int THREADS = TPR > 256 ? TPR : 256;
-    launch_pdl(residual_norm_grad_kernel<RT, BT, VEC, TPR>, dim3(sp.blocks), dim3(THREADS), 0, s, a);
+    using Cfg = GradCfg<TPR, EPT>;
+    static std::atomic<unsigned long long> attr{0};
+    once_per_device(attr, [] {
+        N3D_CUDA(cudaFuncSetAttribute(residual_norm_grad_kernel<RT, BT, VEC, TPR, EPT, R>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::BYTES));
+    });
+    launch_pdl(residual_norm_grad_kernel<RT, BT, VEC, TPR, EPT, R>, dim3(sp.blocks), dim3(Cfg::THREADS), Cfg::BYTES, s, a);
 }
 
 template <class RT, class BT>
 void launch_type(cudaStream_t s, const ResidualArgs& a, const ResidualSplit& sp) {
     if (!a.wide) {
-        sp.threads == 128 ? launch<RT, BT, 1, 128>(s, a, sp) : launch<RT, BT, 1, 1024>(s, a, sp);
+        sp.threads == 128 ? launch<RT, BT, 1, 128, 8, 2>(s, a, sp) : launch<RT, BT, 1, 512, 16, 1>(s, a, sp);
         return;
     }
-    switch (sp.threads) {
-        case 32: return launch<RT, BT, 8, 32>(s, a, sp);
-        case 64: return launch<RT, BT, 8, 64>(s, a, sp);
-        case 128: return launch<RT, BT, 8, 128>(s, a, sp);
-        case 256: return launch<RT, BT, 8, 256>(s, a, sp);
-        case 512: return launch<RT, BT, 8, 512>(s, a, sp);
-        default: return launch<RT, BT, 8, 1024>(s, a, sp);
+    switch (sp.threads * (a.cols > 4096 ? 2 : 1)) {
+        case 32: return launch<RT, BT, 4, 32, 8, 2>(s, a, sp);
+        case 64: return launch<RT, BT, 4, 64, 8, 2>(s, a, sp);
+        case 128: return launch<RT, BT, 4, 128, 8, 2>(s, a, sp);
+        case 256: return launch<RT, BT, 4, 256, 8, 2>(s, a, sp);
+        case 512: return launch<RT, BT, 4, 512, 8, 2>(s, a, sp);
+        default: return launch<RT, BT, 4, 512, 16, 1>(s, a, sp);
     }
 }
 
 }  // namespace
 
-// Two blocks of 256 threads fit an SM, one of 512 or 1024: 148 SMs' worth of blocks, and
-// no more slots than rows.  (The count is fixed, so that results do not depend on the GPU.)
+// 512 threads fit an SM (128 registers each): 148 SMs' worth of blocks, and no more slots
+// than rows.  (The count is fixed, so that results do not depend on the GPU.)
 ResidualSplit residual_split(long long rows, int cols, bool wide) {
     ResidualSplit sp;
-    if (wide) {
+    if (wide) {  // 8 columns a thread, 16 beyond 512 threads
         sp.threads = 32;
-        while (sp.threads * EPT < cols) sp.threads *= 2;
+        while (sp.threads < 512 && sp.threads * 8 < cols) sp.threads *= 2;
     } else {
-        sp.threads = cols <= 128 * EPT ? 128 : 1024;
+        sp.threads = cols <= 1024 ? 128 : 512;
     }
     const int block = std::max(sp.threads, 256);
     sp.per_block = block / sp.threads;
-    const long long most = (block == 256 ? 296LL : 148LL) * sp.per_block;
+    const long long most = 148LL * (512 / block) * sp.per_block;
     sp.slots = (int)std::max<long long>(1, std::min(most, rows));
     sp.blocks = (sp.slots + sp.per_block - 1) / sp.per_block;
     return sp;

@@ -50,7 +50,7 @@ struct ResidualArgs {
     float* sums;        // [blocks][4][cols]: post weight and bias, pre weight and bias
     float* gate_parts;  // [slots][2][cols]
     int slots;          // row ranges of the gradient kernel
-    int wide;           // every row, weight and row stride is a whole number of 16-byte words
+    int wide;           // every row and weight starts on four whole elements, as do the row strides and cols
 };
 void launch_residual_norm(cudaStream_t s, const ResidualArgs& a, int residual_dtype, int block_dtype);
 // How the gradient kernel splits the rows: `slots` ranges (range i is rows

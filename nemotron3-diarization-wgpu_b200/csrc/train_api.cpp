@@ -100,8 +100,7 @@ void check_rows(const n3d_rows& t, size_t rows, size_t cols, int dtype, bool dis
     }
 }
 bool wide_rows(const n3d_rows* t, int dtype) {
-    const int per = 16 / n3d::dtype_size(dtype);
-    return !t || (reinterpret_cast<uintptr_t>(t->d_data) % 16 == 0 && t->row_stride % per == 0);
+    return !t || (reinterpret_cast<uintptr_t>(t->d_data) % (4 * n3d::dtype_size(dtype)) == 0 && t->row_stride % 4 == 0);
 }
 bool wide_weights(std::initializer_list<const float*> ws) {
     for (const float* w : ws)
@@ -318,7 +317,7 @@ n3d_status n3d_residual_norm(int device, const n3d_residual_config* cfg, const n
         a.block = block->d_data, a.ld_block = block->row_stride;
         a.r_out = r->d_data, a.ld_r_out = r->row_stride;
         if (pre) a.y = y->d_data, a.ld_y = y->row_stride;
-        a.wide = cfg->cols % 8 == 0 && wide_rows(x, cfg->residual_dtype) && wide_rows(r, cfg->residual_dtype) &&
+        a.wide = cfg->cols % 4 == 0 && wide_rows(x, cfg->residual_dtype) && wide_rows(r, cfg->residual_dtype) &&
                  wide_rows(block, cfg->block_dtype) && wide_rows(pre ? y : nullptr, cfg->block_dtype) &&
                  wide_weights({d_post_w, d_post_b, d_gate, d_pre_w, d_pre_b});
         if (cfg->rows == 0) return;
@@ -382,7 +381,7 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config* cfg, co
         a.dgate = d_dgate, a.dpost_w = d_dpost_w, a.dpost_b = d_dpost_b, a.dpre_w = d_dpre_w, a.dpre_b = d_dpre_b;
         a.sums = static_cast<float*>(d_workspace);
         a.gate_parts = a.sums + w.sums;
-        a.wide = cols % 8 == 0 && wide_rows(block, bt) && wide_rows(dx, rt) && wide_rows(dblock, bt) &&
+        a.wide = cols % 4 == 0 && wide_rows(block, bt) && wide_rows(dx, rt) && wide_rows(dblock, bt) &&
                  wide_rows(pre ? r : nullptr, rt) && wide_rows(pre ? dy : nullptr, bt) && wide_rows(dr, rt) &&
                  wide_weights({d_post_w, d_post_b, d_gate, d_pre_w, d_dgate});
         a.slots = n3d::residual_split(a.rows, a.cols, a.wide).slots;

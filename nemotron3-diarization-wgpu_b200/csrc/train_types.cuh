@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace n3d {
 
@@ -64,24 +65,26 @@ __device__ __forceinline__ float2 unpack_pair<__half>(uint32_t w) {
     return __half22float2(*reinterpret_cast<__half2*>(&w));
 }
 
-// N consecutive elements as raw words, loaded and stored 16 bytes at a time (N elements
-// must fill whole 16-byte words and p must be 16-byte aligned), or one element (N = 1).
+// N consecutive elements as raw words, loaded and stored in words of 8 bytes (four 16-bit
+// elements) or 16 (N elements must fill whole words and p must be aligned to them), or one
+// element (N = 1).
 template <class T, int N>
 struct Vec {
-    static constexpr int WORDS = N * (int)sizeof(T) / 16;
-    uint4 w[WORDS];
+    using W = typename std::conditional<N * sizeof(T) == 8, uint2, uint4>::type;
+    static constexpr int WORDS = N * (int)sizeof(T) / (int)sizeof(W);
+    W w[WORDS];
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int i = 0; i < WORDS; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        for (int i = 0; i < WORDS; i++) w[i] = __ldg(reinterpret_cast<const W*>(p) + i);
     }
     // for data that the same kernel writes (in-place calls): no read-only path
     __device__ __forceinline__ void load_rw(const T* p) {
 #pragma unroll
-        for (int i = 0; i < WORDS; i++) w[i] = *(reinterpret_cast<const uint4*>(p) + i);
+        for (int i = 0; i < WORDS; i++) w[i] = *(reinterpret_cast<const W*>(p) + i);
     }
     __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
-        for (int i = 0; i < WORDS; i++) reinterpret_cast<uint4*>(p)[i] = w[i];
+        for (int i = 0; i < WORDS; i++) reinterpret_cast<W*>(p)[i] = w[i];
     }
     __device__ __forceinline__ void get(float* f) const {
         const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
