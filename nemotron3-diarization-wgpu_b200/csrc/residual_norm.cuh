@@ -37,30 +37,49 @@ __device__ __forceinline__ void load_weights(const float* p, int col, float othe
 }
 
 // Sums of NV values over the TPR threads of a row, the same in every thread and taken in
-// a fixed order: a butterfly in each warp, then the warps' sums by another.  `buf` (one
-// per call site of a row, TPR / 32 * NV floats) may be written again once a later sum of
-// the row has been taken.  Threads of a row wait only for one another (named barrier
-// 1 + slot of the block).
+// a fixed order.  In a warp the values are first dealt out: each exchange halves the
+// values a lane holds (8 values take 4 + 2 + 1 shuffles and two more, instead of 40), until
+// GS lanes share one value; the warps' sums meet in `buf` (one per call site of a row,
+// TPR / 32 * NV floats, which may be written again once a later sum of the row has been
+// taken).  Threads of a row wait only for one another (named barrier 1 + slot of the block).
 template <int TPR, int NV>
 __device__ __forceinline__ void row_sums(float (&v)[NV], float* buf, int slot) {
+    constexpr int P = NV == 1 ? 1 : NV == 2 ? 2 : NV <= 4 ? 4 : 8, GS = 32 / P;
+    static_assert(NV <= 8, "at most 8 values");
+    const int lane = threadIdx.x & 31, q = lane / GS;  // the value of this lane
+    float x[P];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int i = 0; i < P; i++) x[i] = i < NV ? v[i] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    for (int n = P / 2, o = 16; n > 0; n /= 2, o /= 2)
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const bool up = lane & o;
+            const float keep = up ? x[n + i] : x[i], send = up ? x[i] : x[n + i];
+            x[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    float z = x[0];
+#pragma unroll
+    for (int o = GS / 2; o > 0; o /= 2) z += __shfl_xor_sync(0xffffffffu, z, o);
     if constexpr (TPR > 32) {
         constexpr int W = TPR / 32;
-        const int lane = threadIdx.x & 31, warp = (threadIdx.x % TPR) >> 5;
-        if (lane == 0)
-#pragma unroll
-            for (int i = 0; i < NV; i++) buf[i * W + warp] = v[i];
+        const int warp = (threadIdx.x % TPR) >> 5, i = lane % GS;
+        if (i == 0 && q < NV) buf[q * W + warp] = z;
         asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "n"(TPR) : "memory");
+        z = 0.0f;
+        if (q < NV) {
+            if constexpr (W > GS) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) v[i] = buf[i * W + lane % W];
+                for (int j = 0; j < W / GS; j++) z += buf[q * W + i * (W / GS) + j];
+            } else if (i < W) {
+                z = buf[q * W + i];
+            }
+        }
 #pragma unroll
-        for (int o = W / 2; o > 0; o >>= 1)
-#pragma unroll
-            for (int i = 0; i < NV; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        for (int o = GS / 2; o > 0; o /= 2) z += __shfl_xor_sync(0xffffffffu, z, o);
     }
+#pragma unroll
+    for (int i = 0; i < NV; i++) v[i] = NV == 1 ? z : __shfl_sync(0xffffffffu, z, i * GS);
 }
 
 }  // namespace n3d
