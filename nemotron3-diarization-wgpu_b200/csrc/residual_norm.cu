@@ -137,7 +137,7 @@ void launch_type(cudaStream_t s, const ResidualArgs& a) {
     else if (C <= 4096)
         launch<RT, BT, 4, 256, 16>(s, a);
     else
-        launch<RT, BT, 4, 512, 16>(s, a);
+        launch<RT, BT, 4, 256, 32>(s, a);
 }
 
 }  // namespace
