@@ -17,8 +17,7 @@
 //   warp 2      issues the second products (with both kinds on one thread, which issues an MMA of 64
 //               columns every ~55 clocks, that thread was the bottleneck; a thread for each of the
 //               four products of dkv gains nothing more: the MMAs then wait for one another)
-//   warps 3..   softmax groups of 4 warps, one thread per row; NWG blocks are in work at a time, the
-//               SPLIT groups of a block take 64 / SPLIT of its columns each
+//   warps 3..   softmax groups of 4 warps, one thread per row; NWG column blocks are in work at a time
 // head_dim 64: one group and two blocks per SM, which interleave (256 TMEM columns each);
 // head_dim 128: one block per SM with two groups on alternating column blocks (forward:
 // each with its own running maximum, sum and accumulator, joined at the end).
@@ -73,22 +72,26 @@ struct Cfg {
     static constexpr bool PAIR = PARTS == 2;
     // column blocks in softmax at a time (an fp32 forward pass of head_dim 128 has TMEM for one)
     static constexpr int NWG = SMALL || (PAIR && HD == 128 && MODE == FORWARD) ? 1 : 2;
-    static constexpr int SPLIT = GRAD && SMALL ? 2 : 1;     // groups of 4 warps that share a block's columns
     static constexpr int CHUNK = 16;                        // columns a thread has in registers at a time (gradients)
-    static constexpr int GROUPS = NWG * SPLIT;
     static constexpr int NBUF = MODE == FORWARD ? 2 : NWG;  // score buffers
     static constexpr int SOFTMAX = 3;                       // first softmax warp
-    static constexpr int THREADS = 32 * SOFTMAX + 128 * GROUPS, PER_SM = SMALL ? 2 : 1;
+    static constexpr int THREADS = 32 * SOFTMAX + 128 * NWG, PER_SM = SMALL ? 2 : 1;
     static constexpr int RTILE = ROWS * HD * 2 * PARTS, CTILE = COLS * HD * 2 * PARTS;  // bytes
     static constexpr int STATS = MODE == GRAD_KV ? 512 : 0;               // 64 x (-lse log2 e), 64 x (-D)
     static constexpr int STAT_LD = PARTS == 1 ? 128 : kSplitStat;         // floats of a block of 64 rows
     static constexpr int STAGE = 2 * CTILE + 1024 * (STATS > 0);
     static constexpr int ROW_BYTES = (GRAD ? 2 : 1) * RTILE;
-    // barriers and the TMEM slot, the groups' row statistics, and slack to align the tiles to 1024 bytes
-    static constexpr int REST = 256 + (MODE == FORWARD && NWG > 1 ? (4 + 2 * PAIR) * 128 * 4 : 64) + 1024;
-    static constexpr int ROOM = 226 * 1024 / PER_SM - ROW_BYTES - REST;
-    static constexpr int NST = ROOM / STAGE > 4 ? 4 : ROOM / STAGE;
-    static constexpr int SMEM = ROW_BYTES + NST * STAGE + REST;
+    // floats of the groups' row statistics (double-buffered by item)
+    static constexpr int JOIN = MODE == FORWARD && NWG > 1 ? (4 + 2 * PAIR) * 128 : 4;
+    // barriers, items, the TMEM slot, the statistics, and slack to align the tiles to 1024 bytes
+    static constexpr int REST = 704 + 2 * JOIN * 4 + 1024;
+    static constexpr int ROOM = 226 * 1024 / PER_SM - REST;
+    // Row tiles of two items, so that the next one's load during this one's work, where that leaves enough
+    // stages.  Gradient of 64 windows of 384 rows of 64: 155 us with two and two, 174 with one and four;
+    // of 2 x 4096 rows of 128, with one block per SM: 1091 against 958.
+    static constexpr int RB = (ROOM - 2 * ROW_BYTES) / STAGE >= (SMALL ? 2 : 3) ? 2 : 1;
+    static constexpr int NST = (ROOM - RB * ROW_BYTES) / STAGE > 4 ? 4 : (ROOM - RB * ROW_BYTES) / STAGE;
+    static constexpr int SMEM = RB * ROW_BYTES + NST * STAGE + REST;
     static constexpr uint32_t TBUF = GRAD ? 128 : 64;                     // TMEM columns of a score buffer
     static constexpr uint32_t ACC = NBUF * TBUF;                          // first accumulator
     static constexpr int NACC = MODE == FORWARD ? NWG : MODE == GRAD_Q ? 1 : 2;
@@ -96,7 +99,7 @@ struct Cfg {
     // of head_dim 128 are added up in the output tensors, for which there is no TMEM
     static constexpr bool SUM = PAIR, SUM_OUT = PAIR && HD == 128 && MODE == GRAD_KV;
     static constexpr uint32_t TMEM_COLS = SMALL ? 256 : 512;
-    static_assert(COLS / SPLIT % CHUNK == 0, "whole chunks");
+    static_assert(COLS % CHUNK == 0, "whole chunks");
     static_assert(NBUF % NWG == 0, "a score buffer belongs to one softmax group");
     static_assert(ACC + (SUM && !SUM_OUT ? 2 : 1) * NACC * HD <= TMEM_COLS && PER_SM * TMEM_COLS <= 512, "TMEM");
     static_assert(NST >= 1 && (SMEM + 1024) * PER_SM <= 228 * 1024, "shared memory");
@@ -142,6 +145,30 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, int bytes,
                      smem_u32(dst)),
                  "l"(src), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
+}
+// Cluster launch control: takes the next block of the grid that has not started, if any, over
+// from the scheduler; the answer (16 bytes) arrives on `bar`.
+__device__ __forceinline__ void try_cancel(void* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(answer)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// The block taken over, -1 if none was left.
+__device__ __forceinline__ int cancelled_block(const void* answer) {
+    uint32_t ok, x = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t.reg .b32 y, z, w;\n\t"
+        "ld.shared.b128 a, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, a;\n\t}"
+        : "=r"(ok), "=r"(x)
+        : "r"(smem_u32(answer))
+        : "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    return ok ? (int)x : -1;
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -249,6 +276,15 @@ struct TcArgs {
 };
 
 // T: the type of the MMA operands; tensors are of type T (PARTS 1) or fp32 (PARTS 2, T = fp16).
+// What a block works on: 128 rows of a head and the column blocks they see.
+struct Item {
+    int seq, head, r0, row_len, col_len;
+    int c_begin, per_head, nblk;  // first column block, blocks of one column head, blocks
+    int full_lo, full_hi;         // columns that every live row sees
+    int valid, pad;
+};
+static_assert(sizeof(Item) == 48, "two items in 96 bytes");
+
 template <class T, int HD, int MODE, int PARTS>
 __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, PARTS>::PER_SM)
     attention_train_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs args) {
@@ -258,30 +294,39 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
     constexpr int NWG = C::NWG, NBUF = C::NBUF, NST = C::NST;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* rows1 = smem;              // q, q, k: HD / 64 boxes of [128 rows x 128 B]
-    uint8_t* rows2 = smem + C::RTILE;   // -, dout, v
-    uint8_t* ring = smem + C::ROW_BYTES;
+    uint8_t* rows = smem;                        // RB x (rows 1 | rows 2)
+    uint8_t* ring = smem + C::RB * C::ROW_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NST * C::STAGE);
-    uint64_t* r_full = bars;               // 1: the row tiles landed
-    uint64_t* c_full = bars + 1;           // NST: the column tiles of block g landed (stage g % NST)
-    uint64_t* c_empty = c_full + NST;      // NST: block g's second product completed
-    uint64_t* t_full = c_empty + NST;      // NBUF: T of block g completed (buffer g % NBUF)
-    uint64_t* p_full = t_full + NBUF;      // NBUF: weights of block g written (4 warps)
-    uint64_t* acc_done = p_full + NBUF;    // NBUF: second product of block g completed
-    uint64_t* acc_free = acc_done + NBUF;  // NWG (pairs): the accumulator is added to its sum (4 warps)
-    uint64_t* all_done = acc_free + NWG;   // 1: the last one completed
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
-    float* join = reinterpret_cast<float*>(bars + 32);  // forward with two groups: [2][128] maxima; then sums
-    static_assert(1 + 2 * NST + 3 * NBUF + NWG + 2 <= 32, "barriers and the TMEM slot fill at most 256 bytes");
+    uint64_t* r_full = bars;               // RB: row tiles of loaded item n landed (buffer n % RB)
+    uint64_t* r_free = r_full + 2;         // RB: their item's outputs have left the buffer (every softmax warp)
+    uint64_t* c_full = r_free + 2;         // NST: the column tiles of block g landed (stage g % NST)
+    uint64_t* c_empty = c_full + 4;        // NST: block g's second products completed
+    uint64_t* t_full = c_empty + 4;        // NBUF: T of block g completed (buffer g % NBUF)
+    uint64_t* p_full = t_full + 2;         // NBUF: weights of block g written
+    uint64_t* acc_done = p_full + 2;       // NBUF: second products of block g completed
+    uint64_t* acc_free = acc_done + 2;     // NWG (pairs): the accumulator is added to its sum (4 warps)
+    uint64_t* all_done = acc_free + 2;     // 1: phase n = the last product of loaded item n completed
+    uint64_t* acc_read = all_done + 1;     // 1: phase n = its accumulators are read (every softmax warp)
+    uint64_t* item_full = acc_read + 1;    // 2: item k is known (slot k % 2)
+    uint64_t* item_empty = item_full + 2;  // 2: item k was read by every other warp
+    uint64_t* answered = item_empty + 2;   // 1: the scheduler's answer arrived
+    static_assert(NST <= 4 && NBUF <= 2 && NWG <= 2 && C::RB <= 2, "barriers");
+    Item* items = reinterpret_cast<Item*>(bars + 32);  // 2
+    uint8_t* answer = reinterpret_cast<uint8_t*>(bars + 44);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46);
+    float* joins = reinterpret_cast<float*>(bars + 48);  // 2 x JOIN
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0 && lane == 0) {
-        mbar_init(r_full, 1);
+        for (int i = 0; i < C::RB; i++) mbar_init(&r_full[i], 1), mbar_init(&r_free[i], 4 * NWG);
         for (int i = 0; i < NST; i++) mbar_init(&c_full[i], 1), mbar_init(&c_empty[i], 1);
         for (int i = 0; i < NBUF; i++)
-            mbar_init(&t_full[i], 1), mbar_init(&p_full[i], 4 * C::SPLIT), mbar_init(&acc_done[i], 1);
+            mbar_init(&t_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&acc_done[i], 1);
         for (int i = 0; i < NWG; i++) mbar_init(&acc_free[i], 4);
         mbar_init(all_done, 1);
+        mbar_init(acc_read, 4 * NWG);
+        for (int i = 0; i < 2; i++) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 2 + 4 * NWG);
+        mbar_init(answered, 1);
         mbar_fence_init();
     }
     if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -292,72 +337,127 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
     griddep_wait();
     griddep_launch_dependents();
 
-    // ---- this block's rows and the column blocks they see
     const AttnArgs& a = args.a;
     int* const err = a.err;
     const int heads = MODE == GRAD_KV ? a.k_heads : a.q_heads, group = a.q_heads / a.k_heads;
-    // Heads in runs of args.run: within a run the same tile of every head, then the next tile.
-    // Under a one-sided window the tiles with the most columns go first (the last query tiles see
-    // the most keys, the first key tiles the most queries), so that the blocks that finish
-    // last are short.  Without one the run is 1: the tiles of a head, which read the same columns,
-    // are neighbours.
-    const int run0 = blockIdx.x / (args.run * args.tiles) * args.run, in_run = blockIdx.x - run0 * args.tiles;
-    const int width = min(args.run, heads * a.seqs - run0), order = in_run / width;
-    const int sh = run0 + in_run - order * width, head = sh % heads, seq = sh / heads;
-    const int r0 = ((MODE == GRAD_KV) == args.ascending ? order : args.tiles - 1 - order) * ROWS;
-    const AttnMask mask(a, seq);
-    const int row_len = MODE == GRAD_KV ? mask.k_len : mask.q_len, col_len = MODE == GRAD_KV ? mask.q_len : mask.k_len;
     const int row_cap = MODE == GRAD_KV ? a.k_rows : a.q_rows, col_cap = MODE == GRAD_KV ? a.q_rows : a.k_rows;
-    auto first_col = [&](int r) { return MODE == GRAD_KV ? mask.first_query(r) : mask.first_key(r); };
-    auto last_col = [&](int r) { return MODE == GRAD_KV ? mask.last_query(r) : mask.last_key(r); };
-    const int r_last = min(r0 + ROWS, row_len) - 1;
-    int c_begin = 0, per_head = 0;  // first column block, blocks of one column head
-    if (r_last >= r0) {
-        const int lo = first_col(r0), hi = last_col(r_last);
-        if (hi > lo) c_begin = lo / COLS, per_head = (hi + COLS - 1) / COLS - c_begin;
-    }
-    const int nblk = per_head * (MODE == GRAD_KV ? group : 1);
-    auto col0 = [&](int g) { return (c_begin + (MODE == GRAD_KV ? g % per_head : g)) * COLS; };
-    auto col_head = [&](int g) { return MODE == GRAD_KV ? head * group + g / per_head : head / group; };
+    auto first_col = [&](const AttnMask& mask, int r) { return MODE == GRAD_KV ? mask.first_query(r) : mask.first_key(r); };
+    auto last_col = [&](const AttnMask& mask, int r) { return MODE == GRAD_KV ? mask.last_query(r) : mask.last_key(r); };
+    auto col0 = [&](const Item& it, int g) { return (it.c_begin + (MODE == GRAD_KV ? g % it.per_head : g)) * COLS; };
+    auto col_head = [&](const Item& it, int g) {
+        return MODE == GRAD_KV ? it.head * group + g / it.per_head : it.head / group;
+    };
+    // item k for every warp but the first: false after the last one, or when a wait expired
+    auto next_item = [&](int k, Item& it) {
+        // (phase k / 2 of its slot: the next needs this warp's arrival below)
+        if (!__all_sync(0xffffffffu, mbar_wait(&item_full[k & 1], (k >> 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN))) return false;
+        it = items[k & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[k & 1]);
+        return it.valid != 0;
+    };
 
+    // Every role walks the same items; g counts the column blocks and n the items with any, over all of them:
+    // buffers, stages and phases go by these numbers.
     if (warp == 0) {
-        if (lane == 0 && nblk > 0) {
+        if (lane == 0) {
             const CUtensorMap* rm1 = MODE == GRAD_KV ? &maps.k : &maps.q;
             const CUtensorMap* rm2 = MODE == GRAD_KV ? &maps.v : &maps.dout;
             const CUtensorMap* cm1 = MODE == GRAD_KV ? &maps.q : &maps.k;
             const CUtensorMap* cm2 = MODE == GRAD_KV ? &maps.dout : &maps.v;
-            mbar_arrive_expect_tx(r_full, C::ROW_BYTES);
-            // part p of a pair is the maps' sequence p * seqs + seq
-#pragma unroll
-            for (int i = 0; i < PARTS * HD / 64; i++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {  // 64 rows each
-                    const int o = (2 * i + h) * BOX, d = i % (HD / 64) * 64, sq = i / (HD / 64) * a.seqs + seq;
-                    tma_load_4d(rows1 + o, rm1, r_full, d, r0 + 64 * h, head, sq);
-                    if (C::GRAD) tma_load_4d(rows2 + o, rm2, r_full, d, r0 + 64 * h, head, sq);
+            bool ok = true;
+            int gt = 0, n = 0, block = blockIdx.x;
+            for (int k = 0; ok; k++) {
+                // ---- item k: heads in runs of args.run; within a run the same tile of every head, then the next
+                // tile.  Under a one-sided window the tiles with the most columns go first (the last query
+                // tiles see the most keys, the first key tiles the most queries), so that the blocks that finish
+                // last are short.  Without one the run is 1: the tiles of a head, which read the same
+                // columns, are neighbours.
+                Item it{};
+                it.valid = block >= 0;
+                if (it.valid) {
+                    const int run0 = block / (args.run * args.tiles) * args.run, in_run = block - run0 * args.tiles;
+                    const int width = min(args.run, heads * a.seqs - run0), order = in_run / width;
+                    const int sh = run0 + in_run - order * width;
+                    it.seq = sh / heads;
+                    it.head = sh - it.seq * heads;
+                    it.r0 = ((MODE == GRAD_KV) == args.ascending ? order : args.tiles - 1 - order) * ROWS;
+                    const AttnMask mask(a, it.seq);
+                    it.row_len = MODE == GRAD_KV ? mask.k_len : mask.q_len;
+                    it.col_len = MODE == GRAD_KV ? mask.q_len : mask.k_len;
+                    const int r_last = min(it.r0 + ROWS, it.row_len) - 1;
+                    if (r_last >= it.r0) {
+                        const int lo = first_col(mask, it.r0), hi = last_col(mask, r_last);
+                        if (hi > lo) it.c_begin = lo / COLS, it.per_head = (hi + COLS - 1) / COLS - it.c_begin;
+                        it.full_lo = first_col(mask, r_last);
+                        it.full_hi = last_col(mask, it.r0);
+                    }
+                    it.nblk = it.per_head * (MODE == GRAD_KV ? group : 1);
                 }
-            int g = 0;
-            for (; g < nblk; g++) {
-                // the stage's previous block (phase g / NST - 1; the one after it needs this load)
-                if (g >= NST && !mbar_wait(&c_empty[g % NST], (g / NST - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN)) break;
-                uint8_t* st = ring + (g % NST) * C::STAGE;
-                uint64_t* bar = &c_full[g % NST];
-                const int c0 = col0(g), ch = col_head(g);
-                mbar_arrive_expect_tx(bar, 2 * C::CTILE + C::STATS);
+                // (phase k / 2 - 1 of its slot: the next needs this item)
+                if (k >= 2) ok = mbar_wait(&item_empty[k & 1], (k / 2 - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN);
+                if (!ok) break;
+                items[k & 1] = it;
+                mbar_arrive(&item_full[k & 1]);
+                if (!it.valid) break;
+                // ---- its loads
+                if (it.nblk > 0) {
+                    uint64_t* bar = &r_full[n % C::RB];
+                    uint8_t* rb = rows + n % C::RB * C::ROW_BYTES;
+                    // the buffer's previous item (phase n / RB - 1; the next needs these loads)
+                    if (n >= C::RB) ok = mbar_wait(&r_free[n % C::RB], (n / C::RB - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN);
+                    if (ok) {
+                        mbar_arrive_expect_tx(bar, C::ROW_BYTES);
+                        // part p of a pair is the maps' sequence p * seqs + seq
 #pragma unroll
-                for (int i = 0; i < PARTS * HD / 64; i++) {
-                    const int d = i % (HD / 64) * 64, sq = i / (HD / 64) * a.seqs + seq;
-                    tma_load_4d(st + i * BOX, cm1, bar, d, c0, ch, sq);
-                    tma_load_4d(st + C::CTILE + i * BOX, cm2, bar, d, c0, ch, sq);
+                        for (int i = 0; i < PARTS * HD / 64; i++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {  // 64 rows each
+                                const int o = (2 * i + h) * BOX, d = i % (HD / 64) * 64, sq = i / (HD / 64) * a.seqs + it.seq;
+                                tma_load_4d(rb + o, rm1, bar, d, it.r0 + 64 * h, it.head, sq);
+                                if (C::GRAD) tma_load_4d(rb + C::RTILE + o, rm2, bar, d, it.r0 + 64 * h, it.head, sq);
+                            }
+                        n++;
+                    }
+                    for (int gi = 0; ok && gi < it.nblk; gi++) {
+                        const int g = gt + gi;
+                        // the stage's previous block (phase g / NST - 1; the one after it needs this load)
+                        if (g >= NST) ok = mbar_wait(&c_empty[g % NST], (g / NST - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN);
+                        if (!ok) {
+                            gt = g;
+                            break;
+                        }
+                        uint8_t* st = ring + (g % NST) * C::STAGE;
+                        uint64_t* cb = &c_full[g % NST];
+                        const int c0 = col0(it, gi), ch = col_head(it, gi);
+                        mbar_arrive_expect_tx(cb, 2 * C::CTILE + C::STATS);
+#pragma unroll
+                        for (int i = 0; i < PARTS * HD / 64; i++) {
+                            const int d = i % (HD / 64) * 64, sq = i / (HD / 64) * a.seqs + it.seq;
+                            tma_load_4d(st + i * BOX, cm1, cb, d, c0, ch, sq);
+                            tma_load_4d(st + C::CTILE + i * BOX, cm2, cb, d, c0, ch, sq);
+                        }
+                        if (MODE == GRAD_KV)
+                            bulk_load(st + 2 * C::CTILE,
+                                      args.stats + (((long long)it.seq * a.q_heads + ch) * args.q_tiles * 2 + c0 / COLS) *
+                                                       C::STAT_LD,
+                                      C::STATS, cb);
+                    }
+                    if (ok) gt += it.nblk;
                 }
-                if (MODE == GRAD_KV)
-                    bulk_load(st + 2 * C::CTILE,
-                              args.stats + (((long long)seq * a.q_heads + ch) * args.q_tiles * 2 + c0 / COLS) * C::STAT_LD,
-                              C::STATS, bar);
+                // The next item is claimed once this one's loads are under way, a ring of stages before its end:
+                // claimed at its start, the longest items would take the next longest with them.
+                // (phase k; the next needs another request)
+                mbar_arrive_expect_tx(answered, 16);
+                try_cancel(answer, answered);
+                const bool came = mbar_wait(answered, k & 1, err, DEV_TIMEOUT_ATTN_TRAIN);
+                ok = ok && came;
+                block = came ? cancelled_block(answer) : -1;
             }
             // every load has landed before the block may exit (already true unless a wait expired)
-            mbar_wait(r_full, 0, err, DEV_TIMEOUT_ATTN_TRAIN);
-            for (int x = max(0, g - NST); x < g; x++)
+            for (int x = max(0, n - C::RB); x < n; x++)
+                mbar_wait(&r_full[x % C::RB], (x / C::RB) & 1, err, DEV_TIMEOUT_ATTN_TRAIN);
+            for (int x = max(0, gt - NST); x < gt; x++)
                 mbar_wait(&c_full[x % NST], (x / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN);
         }
     } else if (warp == 1) {
@@ -369,107 +469,123 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     *reinterpret_cast<uint4*>(tile + i * n * 128 + x * 16) = make_uint4(0, 0, 0, 0);
         };
         const uint32_t t_desc = idesc<T>(COLS, false, false), t_neg = idesc<T>(COLS, false, true);
-        bool ok = nblk > 0;
-        if (ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait(r_full, 0, err, DEV_TIMEOUT_ATTN_TRAIN));
-            if (!PAIR && ok && r0 + ROWS > row_len && row_len < row_cap) {
-                clear(rows1, max(row_len - r0, 0), ROWS);
-                if (C::GRAD) clear(rows2, max(row_len - r0, 0), ROWS);
+        bool ok = true;
+        Item it;
+        for (int k = 0, gt = 0, n = 0; ok && next_item(k, it); k++) {
+            if (it.nblk == 0) continue;
+            uint8_t* rows1 = rows + n % C::RB * C::ROW_BYTES;
+            uint8_t* rows2 = rows1 + C::RTILE;
+            // (phase n / RB; the next needs this item's outputs)
+            ok = __all_sync(0xffffffffu, mbar_wait(&r_full[n % C::RB], (n / C::RB) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            if (!PAIR && ok && it.r0 + ROWS > it.row_len && it.row_len < row_cap) {
+                clear(rows1, it.row_len - it.r0, ROWS);
+                if (C::GRAD) clear(rows2, it.row_len - it.r0, ROWS);
                 fence_async_smem();
                 __syncwarp();
             }
-        }
-        for (int g = 0; ok && g < nblk; g++) {
-            // the column tiles of block g (phase g / NST; the next needs this block's second product)
-            ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-            if (!ok) break;
-            uint8_t* st = ring + (g % NST) * C::STAGE;
-            const int c0 = col0(g);
-            if (!PAIR && c0 + COLS > col_len && col_len < col_cap) {
-                clear(st, col_len - c0, COLS);
-                clear(st + C::CTILE, col_len - c0, COLS);
-                fence_async_smem();
+            for (int gi = 0; ok && gi < it.nblk; gi++) {
+                const int g = gt + gi;
+                // the column tiles of block g (phase g / NST; the next needs this block's second product)
+                ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                if (!ok) break;
+                uint8_t* st = ring + (g % NST) * C::STAGE;
+                const int c0 = col0(it, gi);
+                if (!PAIR && c0 + COLS > it.col_len && it.col_len < col_cap) {
+                    clear(st, it.col_len - c0, COLS);
+                    clear(st + C::CTILE, it.col_len - c0, COLS);
+                    fence_async_smem();
+                    __syncwarp();
+                }
+                // T of block g overwrites the weights of block g - NBUF, which its second products have read
+                // (phase g / NBUF - 1; the next needs this T)
+                if (g >= NBUF)
+                    ok = __all_sync(0xffffffffu,
+                                    mbar_wait(&acc_done[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
+                    const uint32_t t = tmem + (g % NBUF) * C::TBUF;
+                    // pairs: l h + h l + h h, the small products first (the accumulator truncates); the
+                    // dropped l l is 2^-22 of the product
+#pragma unroll
+                    for (int i = 0; i < (C::GRAD ? 2 : 1); i++)
+#pragma unroll
+                        for (int c = 0; c < (PAIR ? 3 : 1); c++)
+#pragma unroll
+                            for (int kk = 0; kk < HD / 16; kk++) {
+                                const uint32_t ro = (i ? r2 : r1) + (PAIR && c == 0 ? RPART : 0) + (kk / 4) * 2 * BOX +
+                                                    (kk % 4) * 32;
+                                const uint32_t co = b + i * C::CTILE + (PAIR && c == 1 ? CPART : 0) + (kk / 4) * BOX +
+                                                    (kk % 4) * 32;
+                                umma_f16(t + 64 * i, desc_k_sw128(ro), desc_k_sw128(co),
+                                         i == 0 && args.negate ? t_neg : t_desc, kk + c != 0);
+                            }
+                    umma_commit(&t_full[g % NBUF]);
+                }
                 __syncwarp();
             }
-            // T of block g overwrites the weights of block g - NBUF, which its second products have read
-            // (phase g / NBUF - 1; the next needs this T)
-            if (g >= NBUF)
-                ok = __all_sync(0xffffffffu,
-                                mbar_wait(&acc_done[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
-                const uint32_t t = tmem + (g % NBUF) * C::TBUF;
-                // pairs: l h + h l + h h, the small products first (the accumulator truncates); the dropped
-                // l l is 2^-22 of the product
-#pragma unroll
-                for (int i = 0; i < (C::GRAD ? 2 : 1); i++)
-#pragma unroll
-                    for (int c = 0; c < (PAIR ? 3 : 1); c++)
-#pragma unroll
-                        for (int kk = 0; kk < HD / 16; kk++) {
-                            const uint32_t ro = (i ? r2 : r1) + (PAIR && c == 0 ? RPART : 0) + (kk / 4) * 2 * BOX +
-                                                (kk % 4) * 32;
-                            const uint32_t co = b + i * C::CTILE + (PAIR && c == 1 ? CPART : 0) + (kk / 4) * BOX +
-                                                (kk % 4) * 32;
-                            umma_f16(t + 64 * i, desc_k_sw128(ro), desc_k_sw128(co),
-                                     i == 0 && args.negate ? t_neg : t_desc, kk + c != 0);
-                        }
-                umma_commit(&t_full[g % NBUF]);
-            }
-            __syncwarp();
+            gt += it.nblk;
+            n++;
         }
     } else if (warp == 2) {
         // ---- second products: P v (forward); dS k, or dS^T q and P^T dout
         constexpr uint32_t acc_desc = idesc<T>(HD, true);
-        // where the weights of columns 16 kk.. are: each group's over its own scores, a pair's h and l
-        // side by side
-        auto weight_col = [](int kk) { return PAIR ? 16 * kk : C::SPLIT == 1 ? 8 * kk : 32 * (kk / 2) + 8 * (kk % 2); };
+        // where the weights of columns 16 kk.. are; a pair's h and l are side by side
+        auto weight_col = [](int kk) { return PAIR ? 16 * kk : 8 * kk; };
         bool ok = true;
-        for (int g = 0; ok && g < nblk; g++) {
-            // the column tiles (as above) and the weights of block g (phase g / NBUF; the next needs T of
-            // block g + NBUF, hence this product)
-            ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN) &&
-                                             mbar_wait(&p_full[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-            // block number of its accumulator: a pair's starts afresh every second one, once the softmax group
-            // has added it up (phase n / 2 - 1; the next needs this product)
-            const int n = MODE == FORWARD ? g / NWG : g;
-            if (C::SUM && ok && n >= 2 && n % 2 == 0)
-                ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[MODE == FORWARD ? g % NWG : 0], (n / 2 - 1) & 1, err,
-                                                       DEV_TIMEOUT_ATTN_TRAIN));
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t b = smem_u32(ring + (g % NST) * C::STAGE);
-                const uint32_t t = tmem + (g % NBUF) * C::TBUF;
-                const uint32_t acc = tmem + C::ACC + (MODE == FORWARD ? (g % NWG) * HD : 0);
-                const uint32_t first = C::SUM ? n % 2 == 0 : n == 0;
-                auto second = [&](uint32_t d, uint32_t weights, uint32_t tile) {
+        Item it;
+        int added[2] = {0, 0};  // pairs: sums of each accumulator taken so far
+        for (int k = 0, gt = 0, n = 0; ok && next_item(k, it); k++) {
+            if (it.nblk == 0) continue;
+            // the accumulators of the item before (phase n - 1; the next needs this item's products)
+            if (n > 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_read, (n - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            for (int gi = 0; ok && gi < it.nblk; gi++) {
+                const int g = gt + gi;
+                // the column tiles (as above) and the weights of block g (phase g / NBUF; the next needs T of
+                // block g + NBUF, hence this product)
+                ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN) &&
+                                                 mbar_wait(&p_full[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                // which accumulator, and the block's number there: a pair's starts afresh every second one,
+                // once the softmax group has added it up (the next addition needs this product)
+                const int which = MODE == FORWARD ? g % NWG : 0, m = MODE == FORWARD ? gi / NWG : gi;
+                if (C::SUM && ok && m >= 2 && m % 2 == 0) {
+                    ok = __all_sync(0xffffffffu,
+                                    mbar_wait(&acc_free[which], added[which] & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                    added[which]++;
+                }
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t b = smem_u32(ring + (g % NST) * C::STAGE);
+                    const uint32_t t = tmem + (g % NBUF) * C::TBUF;
+                    const uint32_t acc = tmem + C::ACC + which * HD;
+                    const uint32_t first = C::SUM ? m % 2 == 0 : m == 0;
+                    auto second = [&](uint32_t d, uint32_t weights, uint32_t tile) {
 #pragma unroll
-                    for (int c = 0; c < (PAIR ? 3 : 1); c++)
+                        for (int c = 0; c < (PAIR ? 3 : 1); c++)
 #pragma unroll
-                        for (int kk = 0; kk < COLS / 16; kk++)
-                            umma_f16_ts(d, weights + weight_col(kk) + (PAIR && c == 0 ? 8 : 0),
-                                        desc_mn_sw128(tile + (PAIR && c == 1 ? CPART : 0) + kk * 2048), acc_desc,
-                                        kk + c != 0 || !first);
-                };
-                second(acc, t + (C::GRAD ? 64 : 0), b + (MODE == FORWARD ? C::CTILE : 0));
-                if (MODE == GRAD_KV) second(acc + HD, t, b + C::CTILE);
-                umma_commit(&acc_done[g % NBUF]);
-                umma_commit(&c_empty[g % NST]);
-                if (g == nblk - 1) umma_commit(all_done);
+                            for (int kk = 0; kk < COLS / 16; kk++)
+                                umma_f16_ts(d, weights + weight_col(kk) + (PAIR && c == 0 ? 8 : 0),
+                                            desc_mn_sw128(tile + (PAIR && c == 1 ? CPART : 0) + kk * 2048), acc_desc,
+                                            kk + c != 0 || !first);
+                    };
+                    second(acc, t + (C::GRAD ? 64 : 0), b + (MODE == FORWARD ? C::CTILE : 0));
+                    if (MODE == GRAD_KV) second(acc + HD, t, b + C::CTILE);
+                    umma_commit(&acc_done[g % NBUF]);
+                    umma_commit(&c_empty[g % NST]);
+                    if (gi == it.nblk - 1) umma_commit(all_done);
+                }
+                __syncwarp();
             }
-            __syncwarp();
+            gt += it.nblk;
+            n++;
         }
     } else {
-        // ---- softmax: group wg, TMEM lane quadrant warp % 4, one row per thread
-        const int grp = (warp - C::SOFTMAX) / 4, wg = grp / C::SPLIT, part = grp % C::SPLIT;
-        const int qd = warp & 3, r = qd * 32 + lane, row = r0 + r;
+        // ---- softmax: TMEM lane quadrant warp % 4, one row per thread
+        const int wg = (warp - C::SOFTMAX) / 4;
+        const int qd = warp & 3, r = qd * 32 + lane;
         const uint32_t lb = tmem + (static_cast<uint32_t>(qd * 32) << 16);
-        const bool live = row < row_len;
-        const int lo = first_col(row), hi = last_col(row);
-        const int full_lo = r_last >= r0 ? first_col(r_last) : 0, full_hi = r_last >= r0 ? last_col(r0) : 0;
         // pairs: the powers of two that q, k, v and dout were multiplied by
         float s_q = 1.0f, s_k = 1.0f, s_v = 1.0f, s_do = 1.0f, v_max = 0.0f;
         if (PAIR) {
@@ -481,372 +597,419 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         }
         const float k2 = PAIR ? args.k2 / s_q / s_k : args.k2;
         const float dp_unit = PAIR ? 1.0f / s_do / s_v : 1.0f;  // T2 times this is dP
-        bool ok = true;
-        // this row in a fp32 output
-        auto out_row = [&](const HeadsView& t) {
-            return static_cast<float*>(t.p) + (long long)seq * t.seq + (long long)head * t.head + (long long)row * t.row;
-        };
-
-        // dq: this row's -lse log2 e, -D and fp16 scale; dkv: the fp16 scale of the head group
-        float nlse = 0.0f, ndot = 0.0f, ds_scale = 1.0f;
-        if (MODE == GRAD_Q && PAIR) {
-            const float* st =
-                args.stats + ((((long long)seq * a.q_heads + head) * args.q_tiles + r0 / ROWS) * 2 + r / 64) * C::STAT_LD + r % 64;
-            nlse = live ? st[0] : -INFINITY;
-            ndot = live ? st[64] : 0.0f;
-            ds_scale = pair_ds_scale<HD>(live ? st[128] : 0.0f, v_max);
-        } else if (MODE == GRAD_Q) {
-            const long long sqh = (long long)seq * a.q_heads + head;
-            float norm2 = 0.0f;
-            nlse = -INFINITY;
-            if (live) {
-                const T* o = static_cast<const T*>(a.o.p) + seq * a.o.seq + head * a.o.head + (long long)row * a.o.row;
-                const T* d =
-                    static_cast<const T*>(a.dout.p) + seq * a.dout.seq + head * a.dout.head + (long long)row * a.dout.row;
-                float dot = 0.0f;
-#pragma unroll 4
-                for (int c = 0; c < HD; c += 8) {
-                    Vec<T, 8> vo, vd;
-                    vo.load(o + c);
-                    vd.load(d + c);
-                    float x[8], y[8];
-                    vo.get(x);
-                    vd.get(y);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) dot += x[i] * y[i], norm2 += y[i] * y[i];
-                }
-                ndot = -dot;
-                const float l = a.lse[sqh * a.q_rows + row];
-                if (l != -INFINITY) nlse = -l * LOG2E;
-            }
-            const float norm = sqrtf(norm2);
-            if (F16) ds_scale = 8.0f * inverse_power(norm);
-            if (grp == 0) {
-                float* st = args.stats + ((sqh * args.q_tiles + r0 / ROWS) * 2 + r / 64) * 128 + r % 64;
-                st[0] = nlse;
-                st[64] = ndot;
-                if (F16) {
-                    float m = norm;
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    if (lane == 0) join[qd] = m;
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                    if (r == 0)
-                        args.norms[sqh * args.q_tiles + r0 / ROWS] = fmaxf(fmaxf(join[0], join[1]), fmaxf(join[2], join[3]));
-                }
-            }
-        }
-        if (MODE == GRAD_KV && F16) {
-            // the largest |dout row| of the head group: a pair has one for each head, otherwise one for each tile
-            float m = 0.0f;
-            const int per = PAIR ? 1 : args.q_tiles;
-            const float* n = args.norms + ((long long)seq * a.q_heads + head * group) * per;
-            for (int i = lane; i < group * per; i += 32) m = fmaxf(m, n[i]);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            ds_scale = PAIR ? pair_ds_scale<HD>(m, v_max) : 8.0f * inverse_power(m);
-        }
         constexpr float P_LOG2 = !F16 ? 0.0f : MODE == FORWARD ? 7.0f : MODE == GRAD_KV ? (PAIR ? 15.0f : 10.0f) : 0.0f;
         constexpr float P_SCALE = PAIR ? 32768.0f : 1024.0f;  // 2^P_LOG2 of dkv
+        bool ok = true;
+        Item it;
+        for (int k = 0, gt = 0, n = 0; next_item(k, it); k++) {
+            const int seq = it.seq, head = it.head, r0 = it.r0, row = r0 + r, nblk = it.nblk;
+            const bool live = row < it.row_len;
+            const AttnMask mask(a, it.seq, it.row_len, it.col_len, MODE == GRAD_KV);
+            const int lo = first_col(mask, row), hi = last_col(mask, row);
+            float* join = joins + (k & 1) * C::JOIN;
+            uint8_t* rows1 = rows + n % C::RB * C::ROW_BYTES;  // the staging of the outputs, at the end
+            // this row in a fp32 output
+            auto out_row = [&](const HeadsView& t) {
+                return static_cast<float*>(t.p) + (long long)seq * t.seq + (long long)head * t.head + (long long)row * t.row;
+            };
 
-        float m = -INFINITY, l = 0.0f;  // forward: running maximum (raw scores) and sum (times 2^P_LOG2)
-        float m_sum = -INFINITY;        // pairs, forward: the maximum that the summed accumulators refer to
-        auto sum_factor = [&](float to) { return m_sum == to ? 1.0f : ex2_approx((m_sum - to) * k2); };
-        for (int g = wg; g < nblk; g += NWG) {
-            const int buf = g % NBUF, c0 = col0(g);
-            const uint32_t t = lb + buf * C::TBUF;
-            const bool full = c0 >= full_lo && c0 + COLS <= full_hi;
-            // T of block g (phase g / NBUF of its buffer: the next needs this block's weights).  After an
-            // expired wait the loop keeps running (results unused).
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(&t_full[buf], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-            tc_fence_after();
-            if constexpr (MODE == FORWARD) {
-                float s[64];
-                tmem_ld32(t, s);
-                tmem_ld32(t + 32, s + 32);
-                if (!full) {
+            // dq: this row's -lse log2 e, -D and fp16 scale; dkv: the fp16 scale of the head group
+            float nlse = 0.0f, ndot = 0.0f, ds_scale = 1.0f;
+            if (MODE == GRAD_Q && PAIR) {
+                const float* st =
+                    args.stats + ((((long long)seq * a.q_heads + head) * args.q_tiles + r0 / ROWS) * 2 + r / 64) * C::STAT_LD + r % 64;
+                nlse = live ? st[0] : -INFINITY;
+                ndot = live ? st[64] : 0.0f;
+                ds_scale = pair_ds_scale<HD>(live ? st[128] : 0.0f, v_max);
+            } else if (MODE == GRAD_Q) {
+                const long long sqh = (long long)seq * a.q_heads + head;
+                float norm2 = 0.0f;
+                nlse = -INFINITY;
+                if (live) {
+                    const T* o = static_cast<const T*>(a.o.p) + seq * a.o.seq + head * a.o.head + (long long)row * a.o.row;
+                    const T* d =
+                        static_cast<const T*>(a.dout.p) + seq * a.dout.seq + head * a.dout.head + (long long)row * a.dout.row;
+                    float dot = 0.0f;
+#pragma unroll 4
+                    for (int c = 0; c < HD; c += 8) {
+                        Vec<T, 8> vo, vd;
+                        vo.load(o + c);
+                        vd.load(d + c);
+                        float x[8], y[8];
+                        vo.get(x);
+                        vd.get(y);
 #pragma unroll
-                    for (int c = 0; c < 64; c++)
-                        if (c0 + c < lo || c0 + c >= hi) s[c] = -INFINITY;
+                        for (int i = 0; i < 8; i++) dot += x[i] * y[i], norm2 += y[i] * y[i];
+                    }
+                    ndot = -dot;
+                    const float l = a.lse[sqh * a.q_rows + row];
+                    if (l != -INFINITY) nlse = -l * LOG2E;
                 }
-                float mx[8];
+                const float norm = sqrtf(norm2);
+                if (F16) ds_scale = 8.0f * inverse_power(norm);
+                if (wg == 0) {
+                    float* st = args.stats + ((sqh * args.q_tiles + r0 / ROWS) * 2 + r / 64) * 128 + r % 64;
+                    st[0] = nlse;
+                    st[64] = ndot;
+                    if (F16) {
+                        float m = norm;
 #pragma unroll
-                for (int c = 0; c < 8; c++) mx[c] = fmaxf(s[c], s[c + 8]);
-#pragma unroll
-                for (int c = 16; c < 64; c += 16)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) mx[i] = max3f(mx[i], s[c + i], s[c + 8 + i]);
-                const float mb = max3f(max3f(mx[0], mx[1], mx[2]), max3f(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
-                // (an unseen block leaves mb = -inf: no raise, and the exponents below stay -inf)
-                const bool raise = mb > m && (mb - m) * k2 > RESCALE_LOG2;
-                const float corr = raise ? ex2_approx((m - mb) * k2) : 1.0f;  // 0 from m = -inf
-                if (raise) m = mb;
-                const float off = m == -INFINITY ? 0.0f : P_LOG2 - m * k2;
-                const uint64_t k22 = pack2(k2, k2), off2 = pack2(off, off);
-                uint64_t sum2[4] = {0, 0, 0, 0};
-                uint32_t w[32 * PARTS];  // pairs: per 16 columns 8 words of h, then 8 of l
-#pragma unroll
-                for (int c = 0; c < 64; c += 2) {
-                    float x, y;
-                    unpack2(fma2(pack2(s[c], s[c + 1]), k22, off2), x, y);
-                    x = ex2_approx(x);
-                    y = ex2_approx(y);
-                    sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], pack2(x, y));
-                    if constexpr (PAIR)
-                        split2x2(x, y, 1.0f, w[c / 16 * 16 + c % 16 / 2], w[c / 16 * 16 + 8 + c % 16 / 2]);
-                    else
-                        w[c / 2] = pack_pair<T>(x, y);
-                }
-                float sa, sb;
-                unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sa, sb);
-                l = l * corr + (sa + sb);
-                if (g >= NWG && !(C::SUM && g / NWG % 2 == 0) && __any_sync(0xffffffffu, raise)) {
-                    // this group's previous product (its phase: the buffer's next product needs P of
-                    // this or a later block of the group)
-                    ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_done[(g - NWG) % NBUF], ((g - NWG) / NBUF) & 1, err,
-                                                                 DEV_TIMEOUT_ATTN_TRAIN));
-                    tc_fence_after();
-                    const uint32_t acc = lb + C::ACC + wg * HD;
-                    const uint64_t c2 = pack2(corr, corr);
-#pragma unroll 1
-                    for (int cb = 0; cb < HD; cb += 16) {
-                        float o[16];
-                        uint32_t u[16];
-                        tmem_ld16(acc + cb, o);
-#pragma unroll
-                        for (int d = 0; d < 16; d += 2) {
-                            unpack2(mul2(pack2(o[d], o[d + 1]), c2), o[d], o[d + 1]);
-                            u[d] = __float_as_uint(o[d]), u[d + 1] = __float_as_uint(o[d + 1]);
-                        }
-                        tmem_st16(acc + cb, u);
+                        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        if (lane == 0) join[qd] = m;
+                        asm volatile("bar.sync 1, 128;" ::: "memory");
+                        if (r == 0)
+                            args.norms[sqh * args.q_tiles + r0 / ROWS] = fmaxf(fmaxf(join[0], join[1]), fmaxf(join[2], join[3]));
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 2 * PARTS; i++) tmem_st16(t + 16 * i, w + 16 * i);
-            } else {
-                const float4* st = reinterpret_cast<const float4*>(ring + (g % NST) * C::STAGE + 2 * C::CTILE);
-                const uint64_t k22 = pack2(k2, k2), scale2 = pack2(ds_scale, ds_scale), unit2 = pack2(dp_unit, dp_unit);
-                if (MODE == GRAD_KV)  // the statistics came by bulk copy: this thread's own wait makes them visible
-                    ok = __all_sync(0xffffffffu,
-                                    ok && mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-                auto weights = [&](auto masked) {
-                    constexpr int N = COLS / C::SPLIT, CH = C::CHUNK;  // this group's columns, and how many at a time
-                    const uint32_t t1 = t + N * part, t2 = t1 + 64;
-                    const int cp = c0 + N * part;
-                    const float4* sp = st + N / 4 * part;
-#pragma unroll
-                    for (int h = 0; h < N; h += CH) {  // the weights go over scores that are read already
-                        float s[CH], u[CH];
-                        tmem_ld_pair<CH>(t1 + h, t2 + h, s, u);
-                        uint32_t pw[CH / 2 * PARTS], dw[CH / 2 * PARTS];  // pairs: h, then l
-#pragma unroll
-                        for (int c = 0; c < CH; c += 4) {
-                            float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
-                            if (MODE == GRAD_KV) {
-                                nl = sp[(h + c) / 4];
-                                nd = sp[16 + (h + c) / 4];
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; e += 2) {
-                                const uint64_t n2 = e == 0 ? pack2(nl.x, nl.y) : pack2(nl.z, nl.w);
-                                const uint64_t d2 = e == 0 ? pack2(nd.x, nd.y) : pack2(nd.z, nd.w);
-                                const int cc = cp + h + c + e;
-                                float x, y, gx, gy;
-                                unpack2(fma2(pack2(s[c + e], s[c + e + 1]), k22, n2), x, y);
-                                x = ex2_approx(x);
-                                y = ex2_approx(y);
-                                if (masked && (cc < lo || cc >= hi)) x = 0.0f;
-                                if (masked && (cc + 1 < lo || cc + 1 >= hi)) y = 0.0f;
-                                const uint64_t u2 = pack2(u[c + e], u[c + e + 1]);
-                                uint64_t g2 = mul2(pack2(x, y), PAIR ? fma2(u2, unit2, d2) : add2(u2, d2));
-                                if (F16) g2 = mul2(g2, scale2);
-                                unpack2(g2, gx, gy);
-                                if (masked && x == 0.0f) gx = 0.0f;
-                                if (masked && y == 0.0f) gy = 0.0f;
-                                const int i = (c + e) / 2;
-                                if constexpr (PAIR) {
-                                    if (MODE == GRAD_KV) split2x2(x, y, P_SCALE, pw[i], pw[CH / 2 + i]);
-                                    split2x2(gx, gy, 1.0f, dw[i], dw[CH / 2 + i]);
-                                } else {
-                                    if (MODE == GRAD_KV)
-                                        pw[i] = F16 ? pack_pair<T>(x * P_SCALE, y * P_SCALE) : pack_pair<T>(x, y);
-                                    dw[i] = pack_pair<T>(gx, gy);
-                                }
-                            }
-                        }
-                        if (MODE == GRAD_KV) tmem_st<CH / 2 * PARTS>(t1 + h / 2 * PARTS, pw);
-                        tmem_st<CH / 2 * PARTS>(t2 + h / 2 * PARTS, dw);
-                    }
-                };
-                if (full)
-                    weights(std::false_type());
-                else
-                    weights(std::true_type());
             }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[buf]);
-
-            // pairs: after every second product into an accumulator, if another follows, add it to the sum
-            const int n = MODE == FORWARD ? g / NWG : g;
-            if (C::SUM && n % 2 == 1 && g + (MODE == FORWARD ? NWG : 1) < nblk) {
-                // (its phase: the buffer's next product needs weights of this group)
-                ok = __all_sync(0xffffffffu,
-                                ok && mbar_wait(&acc_done[buf], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-                tc_fence_after();
-                const float f = MODE == FORWARD ? sum_factor(m) : 1.0f;
-                const uint32_t from = lb + C::ACC + (MODE == FORWARD ? wg * HD : 0);
-                constexpr int WIDTH = MODE == GRAD_KV ? 2 * HD : HD;
-#pragma unroll 1
-                for (int cb = 0; cb < WIDTH; cb += 16) {
-                    float o[16], u[16];
-                    tmem_ld16(from + cb, o);
-                    if constexpr (C::SUM_OUT) {
-                        if (live) {
-                            float* to = out_row(cb < HD ? a.dk : a.dv) + cb % HD;
+            if (MODE == GRAD_KV && F16) {
+                // the largest |dout row| of the head group: a pair has one for each head, otherwise one for each tile
+                float m = 0.0f;
+                const int per = PAIR ? 1 : args.q_tiles;
+                const float* n = args.norms + ((long long)seq * a.q_heads + head * group) * per;
+                for (int i = lane; i < group * per; i += 32) m = fmaxf(m, n[i]);
 #pragma unroll
-                            for (int d = 0; d < 16; d++) to[d] = n == 1 ? o[d] : to[d] + o[d];
-                        }
-                    } else {
-                        if (n > 1) tmem_ld16(from + C::NACC * HD + cb, u);
+                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                ds_scale = PAIR ? pair_ds_scale<HD>(m, v_max) : 8.0f * inverse_power(m);
+            }
+
+            float m = -INFINITY, l = 0.0f;  // forward: running maximum (raw scores) and sum (times 2^P_LOG2)
+            float m_sum = -INFINITY;        // pairs, forward: the maximum that the summed accumulators refer to
+            auto sum_factor = [&](float to) { return m_sum == to ? 1.0f : ex2_approx((m_sum - to) * k2); };
+            for (int gi = NWG == 1 ? 0 : (wg + gt) & 1; gi < nblk; gi += NWG) {
+                const int g = gt + gi, buf = g % NBUF, c0 = col0(it, gi);
+                const uint32_t t = lb + buf * C::TBUF;
+                const bool full = c0 >= it.full_lo && c0 + COLS <= it.full_hi;
+                // T of block g (phase g / NBUF of its buffer: the next needs this block's weights).  After an
+                // expired wait the loop keeps running (results unused).
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(&t_full[buf], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                tc_fence_after();
+                if constexpr (MODE == FORWARD) {
+                    float s[64];
+                    tmem_ld32(t, s);
+                    tmem_ld32(t + 32, s + 32);
+                    if (!full) {
+#pragma unroll
+                        for (int c = 0; c < 64; c++)
+                            if (c0 + c < lo || c0 + c >= hi) s[c] = -INFINITY;
+                    }
+                    float mx[8];
+#pragma unroll
+                    for (int c = 0; c < 8; c++) mx[c] = fmaxf(s[c], s[c + 8]);
+#pragma unroll
+                    for (int c = 16; c < 64; c += 16)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) mx[i] = max3f(mx[i], s[c + i], s[c + 8 + i]);
+                    const float mb = max3f(max3f(mx[0], mx[1], mx[2]), max3f(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+                    // (an unseen block leaves mb = -inf: no raise, and the exponents below stay -inf)
+                    const bool raise = mb > m && (mb - m) * k2 > RESCALE_LOG2;
+                    const float corr = raise ? ex2_approx((m - mb) * k2) : 1.0f;  // 0 from m = -inf
+                    if (raise) m = mb;
+                    const float off = m == -INFINITY ? 0.0f : P_LOG2 - m * k2;
+                    const uint64_t k22 = pack2(k2, k2), off2 = pack2(off, off);
+                    uint64_t sum2[4] = {0, 0, 0, 0};
+                    // 16 words of weights at a time, over scores that are in registers (pairs: 16 columns, 8 words of
+                    // h and 8 of l)
+                    constexpr int CW = 32 / PARTS;
+#pragma unroll
+                    for (int i = 0; i < 64; i += CW) {
                         uint32_t w[16];
 #pragma unroll
-                        for (int d = 0; d < 16; d++) w[d] = __float_as_uint(n > 1 ? u[d] * f + o[d] : o[d]);
-                        tmem_st16(from + C::NACC * HD + cb, w);
+                        for (int c = i; c < i + CW; c += 2) {
+                            float x, y;
+                            unpack2(fma2(pack2(s[c], s[c + 1]), k22, off2), x, y);
+                            x = ex2_approx(x);
+                            y = ex2_approx(y);
+                            sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], pack2(x, y));
+                            const int j = (c - i) / 2;
+                            if constexpr (PAIR)
+                                split2x2(x, y, 1.0f, w[j], w[8 + j]);
+                            else
+                                w[j] = pack_pair<T>(x, y);
+                        }
+                        tmem_st16(t + i / CW * 16, w);
                     }
+                    float sa, sb;
+                    unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sa, sb);
+                    l = l * corr + (sa + sb);
+                    if (gi >= NWG && !(C::SUM && gi / NWG % 2 == 0) && __any_sync(0xffffffffu, raise)) {
+                        // this group's previous product (its phase: the buffer's next product needs P of
+                        // this or a later block of the group)
+                        ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_done[(g - NWG) % NBUF], ((g - NWG) / NBUF) & 1, err,
+                                                                     DEV_TIMEOUT_ATTN_TRAIN));
+                        tc_fence_after();
+                        const uint32_t acc = lb + C::ACC + wg * HD;
+                        const uint64_t c2 = pack2(corr, corr);
+#pragma unroll 1
+                        for (int cb = 0; cb < HD; cb += 16) {
+                            float o[16];
+                            uint32_t u[16];
+                            tmem_ld16(acc + cb, o);
+#pragma unroll
+                            for (int d = 0; d < 16; d += 2) {
+                                unpack2(mul2(pack2(o[d], o[d + 1]), c2), o[d], o[d + 1]);
+                                u[d] = __float_as_uint(o[d]), u[d + 1] = __float_as_uint(o[d + 1]);
+                            }
+                            tmem_st16(acc + cb, u);
+                        }
+                    }
+                } else {
+                    const float4* st = reinterpret_cast<const float4*>(ring + (g % NST) * C::STAGE + 2 * C::CTILE);
+                    const uint64_t k22 = pack2(k2, k2), scale2 = pack2(ds_scale, ds_scale), unit2 = pack2(dp_unit, dp_unit);
+                    if (MODE == GRAD_KV)  // the statistics came by bulk copy: this thread's own wait makes them visible
+                        ok = __all_sync(0xffffffffu,
+                                        ok && mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                    auto weights = [&](auto masked) {
+                        constexpr int CH = C::CHUNK;
+#pragma unroll
+                        for (int h = 0; h < COLS; h += CH) {  // the weights go over scores that are read already
+                            float s[CH], u[CH];
+                            tmem_ld_pair<CH>(t + h, t + 64 + h, s, u);
+                            uint32_t pw[CH / 2 * PARTS], dw[CH / 2 * PARTS];  // pairs: h, then l
+#pragma unroll
+                            for (int c = 0; c < CH; c += 4) {
+                                float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
+                                if (MODE == GRAD_KV) {
+                                    nl = st[(h + c) / 4];
+                                    nd = st[16 + (h + c) / 4];
+                                }
+#pragma unroll
+                                for (int e = 0; e < 4; e += 2) {
+                                    const uint64_t n2 = e == 0 ? pack2(nl.x, nl.y) : pack2(nl.z, nl.w);
+                                    const uint64_t d2 = e == 0 ? pack2(nd.x, nd.y) : pack2(nd.z, nd.w);
+                                    const int cc = c0 + h + c + e;
+                                    float x, y, gx, gy;
+                                    unpack2(fma2(pack2(s[c + e], s[c + e + 1]), k22, n2), x, y);
+                                    x = ex2_approx(x);
+                                    y = ex2_approx(y);
+                                    if (masked && (cc < lo || cc >= hi)) x = 0.0f;
+                                    if (masked && (cc + 1 < lo || cc + 1 >= hi)) y = 0.0f;
+                                    const uint64_t u2 = pack2(u[c + e], u[c + e + 1]);
+                                    uint64_t g2 = mul2(pack2(x, y), PAIR ? fma2(u2, unit2, d2) : add2(u2, d2));
+                                    if (F16) g2 = mul2(g2, scale2);
+                                    unpack2(g2, gx, gy);
+                                    if (masked && x == 0.0f) gx = 0.0f;
+                                    if (masked && y == 0.0f) gy = 0.0f;
+                                    const int i = (c + e) / 2;
+                                    if constexpr (PAIR) {
+                                        if (MODE == GRAD_KV) split2x2(x, y, P_SCALE, pw[i], pw[CH / 2 + i]);
+                                        split2x2(gx, gy, 1.0f, dw[i], dw[CH / 2 + i]);
+                                    } else {
+                                        if (MODE == GRAD_KV)
+                                            pw[i] = F16 ? pack_pair<T>(x * P_SCALE, y * P_SCALE) : pack_pair<T>(x, y);
+                                        dw[i] = pack_pair<T>(gx, gy);
+                                    }
+                                }
+                            }
+                            if (MODE == GRAD_KV) tmem_st<CH / 2 * PARTS>(t + h / 2 * PARTS, pw);
+                            tmem_st<CH / 2 * PARTS>(t + 64 + h / 2 * PARTS, dw);
+                        }
+                    };
+                    if (full)
+                        weights(std::false_type());
+                    else
+                        weights(std::true_type());
                 }
-                m_sum = m;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_free[MODE == FORWARD ? wg : 0]);
-            }
-        }
+                if (lane == 0) mbar_arrive(&p_full[buf]);
 
-        // ---- the accumulators, once every product has completed
-        if (nblk > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(all_done, 0, err, DEV_TIMEOUT_ATTN_TRAIN));
-        tc_fence_after();
-        if (C::SUM_OUT) asm volatile("bar.sync 1, 256;" ::: "memory");  // the sums in the outputs are written
-        float f0 = 0.0f, f1 = 0.0f;  // what the accumulator(s) are multiplied by
-        float g0 = 0.0f, g1 = 0.0f;  // and their sums
-        if (MODE == FORWARD) {
-            float lse;
-            if (NWG == 1) {
-                f0 = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN;
-                lse = row_lse(l, m, k2, P_LOG2);
-            } else {
-                join[wg * 128 + r] = m;
-                join[256 + wg * 128 + r] = l;
-                if (C::SUM) join[512 + wg * 128 + r] = sum_factor(m);
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float m0 = join[r], m1 = join[128 + r], l0 = join[256 + r], l1 = join[256 + 128 + r];
-                const float mm = fmaxf(m0, m1);
-                // a group that saw nothing has m = -inf and l = 0
-                const float e0 = l0 == 0.0f ? 0.0f : ex2_approx((m0 - mm) * k2);
-                const float e1 = l1 == 0.0f ? 0.0f : ex2_approx((m1 - mm) * k2);
-                const float sum = l0 * e0 + l1 * e1;
-                const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : NAN;
-                f0 = e0 * inv;
-                f1 = nblk > 1 ? e1 * inv : 0.0f;
-                lse = row_lse(sum, mm, k2, P_LOG2);
-            }
-            if (a.lse && wg == 0 && row < a.q_rows)
-                a.lse[((long long)seq * a.q_heads + head) * a.q_rows + row] = live ? lse : -INFINITY;
-            f0 /= s_v;
-            f1 /= s_v;
-            if (C::SUM) {
-                g0 = f0 * (NWG == 1 ? sum_factor(m) : join[512 + r]);
-                g1 = f1 * join[512 + 128 + r];
-            }
-        } else {
-            f0 = args.factor / ds_scale / (MODE == GRAD_Q ? s_k : s_q);
-            g0 = f0;
-        }
-        const float fv = F16 ? 1.0f / P_SCALE / s_do : 1.0f;  // of dv
-        // 64 columns of an accumulator (plus what belongs to it) to this row's staging: a row of 64
-        // elements, its 16-byte words swizzled by the row
-        constexpr int EL = PAIR ? 4 : 2, WORDS = 64 * EL / 16, ROW = 64 * EL;
-        // (second: the other group's accumulator; summed: what was added up before)
-        const bool second = MODE == FORWARD && NWG > 1 && nblk > 1;
-        const bool summed = C::SUM && nblk > 2 * (MODE == FORWARD ? NWG : 1), summed2 = C::SUM && second && nblk > 2 * NWG + 1;
-        auto stage_box = [&](uint32_t acc, float f, float gs, const float* sum_row, uint8_t* box) {
-            const uint32_t acc2 = acc + HD, sum = acc + C::NACC * HD;
+                // pairs: after every second product into an accumulator, if another follows, add it to the sum
+                const int nth = MODE == FORWARD ? gi / NWG : gi;
+                if (C::SUM && nth % 2 == 1 && gi + (MODE == FORWARD ? NWG : 1) < nblk) {
+                    // (its phase: the buffer's next product needs weights of this group)
+                    ok = __all_sync(0xffffffffu,
+                                    ok && mbar_wait(&acc_done[buf], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                    tc_fence_after();
+                    const float f = MODE == FORWARD ? sum_factor(m) : 1.0f;
+                    const uint32_t from = lb + C::ACC + (MODE == FORWARD ? wg * HD : 0);
+                    constexpr int WIDTH = MODE == GRAD_KV ? 2 * HD : HD;
 #pragma unroll 1
-            for (int cb = 0; cb < 64; cb += 16) {
-                float o[16], o2[16], u[16], u2[16];
-                if (nblk > 0) tmem_ld16(acc + cb, o);
-                if (second) tmem_ld16(acc2 + cb, o2);
-                if (C::SUM_OUT) {
+                    for (int cb = 0; cb < WIDTH; cb += 16) {
+                        float o[16], u[16];
+                        tmem_ld16(from + cb, o);
+                        if constexpr (C::SUM_OUT) {
+                            if (live) {
+                                float* to = out_row(cb < HD ? a.dk : a.dv) + cb % HD;
 #pragma unroll
-                    for (int d = 0; d < 16; d++) u[d] = summed && live ? sum_row[cb + d] : 0.0f;
-                } else if (summed) {
-                    tmem_ld16(sum + cb, u);
-                }
-                if (summed2) tmem_ld16(sum + HD + cb, u2);
-                uint32_t w[4 * EL];
+                                for (int d = 0; d < 16; d++) to[d] = nth == 1 ? o[d] : to[d] + o[d];
+                            }
+                        } else {
+                            if (nth > 1) tmem_ld16(from + C::NACC * HD + cb, u);
+                            uint32_t w[16];
 #pragma unroll
-                for (int d = 0; d < 16; d += 2) {
-                    float x = 0.0f, y = 0.0f;
-                    if (live && nblk > 0) {
-                        x = o[d] * f, y = o[d + 1] * f;
-                        if (summed) x += u[d] * gs, y += u[d + 1] * gs;
-                        if (second) x += o2[d] * f1, y += o2[d + 1] * f1;
-                        if (summed2) x += u2[d] * g1, y += u2[d + 1] * g1;
+                            for (int d = 0; d < 16; d++) w[d] = __float_as_uint(nth > 1 ? u[d] * f + o[d] : o[d]);
+                            tmem_st16(from + C::NACC * HD + cb, w);
+                        }
                     }
-                    if constexpr (PAIR)
-                        w[d] = __float_as_uint(x), w[d + 1] = __float_as_uint(y);
-                    else
-                        w[d / 2] = pack_pair<T>(x, y);
+                    m_sum = m;
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_free[MODE == FORWARD ? wg : 0]);
                 }
-#pragma unroll
-                for (int i = 0; i < EL; i++)
-                    *reinterpret_cast<uint4*>(box + r * ROW + (((cb * EL / 16 + i) ^ (r & (WORDS - 1))) << 4)) =
-                        make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
             }
-        };
-        // a warp's 32 rows of the staging: one TMA store of 16-bit rows; fp32 rows, whose tensors may have
-        // any strides, two rows at a time
-        auto send_box = [&](const CUtensorMap* map, const HeadsView& t, uint8_t* box, int d) {
-            const int first = r0 + qd * 32;
-            if constexpr (PAIR) {
-                __syncwarp();
-                const int word = lane % 16;
-                float* p = static_cast<float*>(t.p) + (long long)seq * t.seq + (long long)head * t.head + d + 4 * word;
-                const bool wide = ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(t.row * 4)) & 15) == 0;
-                for (int i = lane / 16; i < 32 && first + i < row_cap; i += 2) {
-                    const int rr = qd * 32 + i;
-                    const float4 v = *reinterpret_cast<const float4*>(box + rr * ROW + ((word ^ (rr & 15)) << 4));
-                    float* to = p + (long long)(first + i) * t.row;
-                    if (wide)
-                        *reinterpret_cast<float4*>(to) = v;
-                    else
-                        to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+
+            if (nblk == 0) {
+                // nothing is seen: zeros, straight to the outputs
+                if (MODE == FORWARD && a.lse && wg == 0 && row < a.q_rows)
+                    a.lse[((long long)seq * a.q_heads + head) * a.q_rows + row] = -INFINITY;
+                for (int o = 0; o < (MODE == GRAD_KV ? 2 : 1); o++) {
+                    const HeadsView& t = MODE == FORWARD ? a.o : MODE == GRAD_Q ? a.dq : o ? a.dv : a.dk;
+                    using Out = typename std::conditional<PAIR, float, T>::type;
+                    Out* p = static_cast<Out*>(t.p) + (long long)seq * t.seq + (long long)head * t.head;
+                    // 16-bit rows are whole 16-byte words, fp32 rows may start anywhere
+                    constexpr int N = PAIR ? 1 : 8, PER_ROW = HD / N;
+                    for (int i = threadIdx.x - 32 * C::SOFTMAX; i < ROWS * PER_ROW; i += 128 * NWG) {
+                        const int rr = r0 + i / PER_ROW;
+                        if (rr >= row_cap) break;
+                        Out* to = p + (long long)rr * t.row + i % PER_ROW * N;
+                        if constexpr (PAIR)
+                            *to = 0.0f;
+                        else
+                            *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                continue;
+            }
+            // ---- the accumulators, once every product has completed (phase n; the next needs acc_read)
+            if (nblk > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(all_done, n & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            tc_fence_after();
+            if (C::SUM_OUT) asm volatile("bar.sync 1, 256;" ::: "memory");  // the sums in the outputs are written
+            float f0 = 0.0f, f1 = 0.0f;  // what the accumulator(s) are multiplied by
+            float g0 = 0.0f, g1 = 0.0f;  // and their sums
+            if (MODE == FORWARD) {
+                float lse;
+                if (NWG == 1) {
+                    f0 = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN;
+                    lse = row_lse(l, m, k2, P_LOG2);
+                } else {
+                    join[wg * 128 + r] = m;
+                    join[256 + wg * 128 + r] = l;
+                    if (C::SUM) join[512 + wg * 128 + r] = sum_factor(m);
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    const float m0 = join[r], m1 = join[128 + r], l0 = join[256 + r], l1 = join[256 + 128 + r];
+                    const float mm = fmaxf(m0, m1);
+                    // a group that saw nothing has m = -inf and l = 0
+                    const float e0 = l0 == 0.0f ? 0.0f : ex2_approx((m0 - mm) * k2);
+                    const float e1 = l1 == 0.0f ? 0.0f : ex2_approx((m1 - mm) * k2);
+                    const float sum = l0 * e0 + l1 * e1;
+                    const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : NAN;
+                    f0 = e0 * inv;
+                    f1 = e1 * inv;
+                    lse = row_lse(sum, mm, k2, P_LOG2);
+                }
+                if (a.lse && wg == 0 && row < a.q_rows)
+                    a.lse[((long long)seq * a.q_heads + head) * a.q_rows + row] = live ? lse : -INFINITY;
+                f0 /= s_v;
+                f1 /= s_v;
+                if (C::SUM) {
+                    g0 = f0 * (NWG == 1 ? sum_factor(m) : join[512 + r]);
+                    g1 = f1 * join[512 + 128 + r];
                 }
             } else {
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0 && first < row_cap) {
-                    tma_store_4d(map, box + qd * 32 * ROW, d, first, head, seq);
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                }
+                f0 = args.factor / ds_scale / (MODE == GRAD_Q ? s_k : s_q);
+                g0 = f0;
             }
-        };
-        // the row tiles are no longer read: they hold the staging, a box of 128 rows for every 64 columns
-        const uint32_t acc = lb + C::ACC;
-        constexpr int PER = HD / 64, BOXES = MODE == GRAD_KV ? 2 * PER : PER;  // out, dq, or dk then dv
-        static_assert(BOXES * ROWS * ROW <= C::ROW_BYTES, "the staging fits the row tiles");
+            const float fv = F16 ? 1.0f / P_SCALE / s_do : 1.0f;  // of dv
+            // 64 columns of an accumulator (plus what belongs to it) to this row's staging: a row of 64
+            // elements, its 16-byte words swizzled by the row
+            constexpr int EL = PAIR ? 4 : 2, WORDS = 64 * EL / 16, ROW = 64 * EL;
+            // (second: the other group's accumulator; summed: what was added up before)
+            // blocks of each accumulator: the groups of the forward pass take turns, from the group of block gt
+            const int mine0 = MODE == FORWARD && NWG > 1 ? (nblk + 1 - (gt & 1)) / 2 : nblk;
+            const bool have = mine0 > 0, second = MODE == FORWARD && NWG > 1 && nblk > mine0;
+            const bool summed = C::SUM && mine0 > 2, summed2 = C::SUM && second && nblk - mine0 > 2;
+            auto stage_box = [&](uint32_t acc, float f, float gs, const float* sum_row, uint8_t* box) {
+                const uint32_t acc2 = acc + HD, sum = acc + C::NACC * HD;
 #pragma unroll 1
-        for (int i = grp; i < BOXES; i += C::GROUPS) {
-            uint8_t* box = rows1 + i * ROWS * ROW;
-            const int d = 64 * (i % PER);
-            const bool is_dv = MODE == GRAD_KV && i >= PER;
-            stage_box(acc + 64 * i, is_dv ? fv : f0, is_dv ? fv : g0,
-                      C::SUM_OUT ? out_row(is_dv ? a.dv : a.dk) + d : nullptr, box);
-            send_box(MODE == FORWARD ? &maps.out : MODE == GRAD_Q ? &maps.dq : i < PER ? &maps.dk : &maps.dv,
-                     MODE == FORWARD ? a.o : MODE == GRAD_Q ? a.dq : i < PER ? a.dk : a.dv, box, d);
+                for (int cb = 0; cb < 64; cb += 16) {
+                    float o[16], o2[16], u[16], u2[16];
+                    if (have) tmem_ld16(acc + cb, o);
+                    if (second) tmem_ld16(acc2 + cb, o2);
+                    if (C::SUM_OUT) {
+#pragma unroll
+                        for (int d = 0; d < 16; d++) u[d] = summed && live ? sum_row[cb + d] : 0.0f;
+                    } else if (summed) {
+                        tmem_ld16(sum + cb, u);
+                    }
+                    if (summed2) tmem_ld16(sum + HD + cb, u2);
+                    uint32_t w[4 * EL];
+#pragma unroll
+                    for (int d = 0; d < 16; d += 2) {
+                        float x = 0.0f, y = 0.0f;
+                        if (live && nblk > 0) {
+                            if (have) x = o[d] * f, y = o[d + 1] * f;
+                            if (summed) x += u[d] * gs, y += u[d + 1] * gs;
+                            if (second) x += o2[d] * f1, y += o2[d + 1] * f1;
+                            if (summed2) x += u2[d] * g1, y += u2[d + 1] * g1;
+                        }
+                        if constexpr (PAIR)
+                            w[d] = __float_as_uint(x), w[d + 1] = __float_as_uint(y);
+                        else
+                            w[d / 2] = pack_pair<T>(x, y);
+                    }
+#pragma unroll
+                    for (int i = 0; i < EL; i++)
+                        *reinterpret_cast<uint4*>(box + r * ROW + (((cb * EL / 16 + i) ^ (r & (WORDS - 1))) << 4)) =
+                            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
+            };
+            // a warp's 32 rows of the staging: one TMA store of 16-bit rows; fp32 rows, whose tensors may have
+            // any strides, two rows at a time
+            auto send_box = [&](const CUtensorMap* map, const HeadsView& t, uint8_t* box, int d) {
+                const int first = r0 + qd * 32;
+                if constexpr (PAIR) {
+                    __syncwarp();
+                    const int word = lane % 16;
+                    float* p = static_cast<float*>(t.p) + (long long)seq * t.seq + (long long)head * t.head + d + 4 * word;
+                    const bool wide = ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(t.row * 4)) & 15) == 0;
+                    for (int i = lane / 16; i < 32 && first + i < row_cap; i += 2) {
+                        const int rr = qd * 32 + i;
+                        const float4 v = *reinterpret_cast<const float4*>(box + rr * ROW + ((word ^ (rr & 15)) << 4));
+                        float* to = p + (long long)(first + i) * t.row;
+                        if (wide)
+                            *reinterpret_cast<float4*>(to) = v;
+                        else
+                            to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+                    }
+                } else {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && first < row_cap) {
+                        tma_store_4d(map, box + qd * 32 * ROW, d, first, head, seq);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+            };
+            // the row tiles are no longer read: they hold the staging, a box of 128 rows for every 64 columns
+            const uint32_t acc = lb + C::ACC;
+            constexpr int PER = HD / 64, BOXES = MODE == GRAD_KV ? 2 * PER : PER;  // out, dq, or dk then dv
+            static_assert(BOXES * ROWS * ROW <= C::ROW_BYTES, "the staging fits the row tiles");
+#pragma unroll 1
+            for (int i = wg; i < BOXES; i += NWG) {
+                uint8_t* box = rows1 + i * ROWS * ROW;
+                const int d = 64 * (i % PER);
+                const bool is_dv = MODE == GRAD_KV && i >= PER;
+                stage_box(acc + 64 * i, is_dv ? fv : f0, is_dv ? fv : g0,
+                          C::SUM_OUT ? out_row(is_dv ? a.dv : a.dk) + d : nullptr, box);
+                send_box(MODE == FORWARD ? &maps.out : MODE == GRAD_Q ? &maps.dq : i < PER ? &maps.dk : &maps.dv,
+                         MODE == FORWARD ? a.o : MODE == GRAD_Q ? a.dq : i < PER ? a.dk : a.dv, box, d);
+            }
+            // ---- the accumulators are read, and (once the stores have read it) the staging, which the next loads
+            // overwrite
+            tc_fence_before();
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(acc_read);
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                mbar_arrive(&r_free[n % C::RB]);
+            }
+            gt += nblk;
+            n++;
         }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // staging read
     }
     tc_fence_before();
     __syncthreads();

@@ -84,6 +84,13 @@ struct AttnMask {
           left(a.left),
           right(a.right),
           offset(a.offset) {}
+    // the same of a sequence whose row and column lengths are known (`by_key`: rows are keys)
+    __device__ __forceinline__ AttnMask(const AttnArgs& a, int, int row_len, int col_len, bool by_key)
+        : q_len(by_key ? col_len : row_len),
+          k_len(by_key ? row_len : col_len),
+          left(a.left),
+          right(a.right),
+          offset(a.offset) {}
     // key rows [first, last) of query row i, empty when last <= first
     __device__ __forceinline__ int first_key(int i) const {
         return left >= kNoLimit ? 0 : (int)max(0LL, (long long)i + offset - left);
