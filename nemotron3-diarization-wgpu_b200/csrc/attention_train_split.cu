@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "n3d_device.cuh"
 #include "train.h"
@@ -21,64 +22,77 @@ namespace n3d {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int ILP = 4;  // lines of a thread in flight
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Operand {
     HeadsView t;
     const int32_t* len;
     int rows, heads;
-    long long lines;  // seqs * heads * rows
-    __half* out;      // part 0; part 1 lies lines * head_dim further
+    int lines;    // seqs * heads * rows
+    int wide;     // every line starts on 16 bytes
+    __half* out;  // part 0; part 1 lies lines * head_dim further
 };
 struct SplitArgs {
     Operand op[4];  // q, k, v, dout
     HeadsView o;
+    int o_wide;
     const float* lse;
     AttnSplitSpace sp;
-    long long heads_total;  // seqs * q_heads
+    int heads_total;  // seqs * q_heads
     int q_tiles, backward;
 };
 
-// Line i of an operand: sequence, head, row; whether the row is inside its length.
+// Line i of an operand: sequence * heads + head, sequence, row; whether the row is inside its length.
 struct Line {
-    long long seq;
-    int head, row;
+    int sh, seq, row;
     bool live;
 };
-__device__ __forceinline__ Line line_of(const Operand& p, long long i) {
+__device__ __forceinline__ Line line_of(const Operand& p, int i) {
     Line l;
-    const long long sh = i / p.rows;
-    l.row = (int)(i - sh * p.rows);
-    l.seq = sh / p.heads;
-    l.head = (int)(sh - l.seq * p.heads);
+    l.sh = i / p.rows;
+    l.row = i - l.sh * p.rows;
+    l.seq = l.sh / p.heads;
     l.live = !p.len || l.row < p.len[l.seq];
     return l;
 }
-__device__ __forceinline__ const float* line_ptr(const HeadsView& t, const Line& l) {
-    return static_cast<const float*>(t.p) + l.seq * t.seq + (long long)l.row * t.row + l.head * t.head;
+// Four consecutive elements of a line from c on.
+__device__ __forceinline__ float4 line_load(const HeadsView& t, const Line& l, int heads, int c, bool wide) {
+    const float* x = static_cast<const float*>(t.p) + l.seq * t.seq + l.row * t.row + (l.sh - l.seq * heads) * t.head + c;
+    return wide ? *reinterpret_cast<const float4*>(x) : make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// blockIdx.y: the operand.  A warp per line.  Infinities and NaN do not count: they make
-// their own products NaN whatever the scale.
-template <int PER>  // elements of a lane: head_dim / 32
+// blockIdx.y: the operand.  HD / 4 threads a line, ILP lines a thread.  Infinities and NaN
+// do not count: they make their own products NaN whatever the scale.
+template <int HD>
 __global__ void __launch_bounds__(THREADS) attention_absmax_kernel(const __grid_constant__ SplitArgs a) {
+    constexpr int TPL = HD / 4, LINES = THREADS / TPL;
     __shared__ float part[THREADS / 32];
     griddep_wait();
     griddep_launch_dependents();
     const Operand& p = a.op[blockIdx.y];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x % TPL * 4;
     if (a.backward && blockIdx.y == 3)
-        for (long long i = blockIdx.x * THREADS + threadIdx.x; i < a.heads_total; i += gridDim.x * THREADS)
+        for (int i = blockIdx.x * THREADS + threadIdx.x; i < a.heads_total; i += gridDim.x * THREADS)
             a.sp.head_norm[i] = 0.0f;
     float m = 0.0f;
-    for (long long i = blockIdx.x * (THREADS / 32) + warp; i < p.lines; i += gridDim.x * (THREADS / 32)) {
-        const Line l = line_of(p, i);
-        if (!l.live) continue;
-        const float* x = line_ptr(p.t, l);
+    for (long long first = (long long)blockIdx.x * LINES * ILP; first < p.lines; first += (long long)gridDim.x * LINES * ILP) {
+        float4 v[ILP];
 #pragma unroll
-        for (int c = 0; c < PER; c++) {
-            const float v = fabsf(x[lane + 32 * c]);
-            if (v < INFINITY) m = fmaxf(m, v);
+        for (int j = 0; j < ILP; j++) {
+            v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const long long i = first + j * LINES + threadIdx.x / TPL;
+            if (i < p.lines) {
+                const Line l = line_of(p, (int)i);
+                if (l.live) v[j] = line_load(p.t, l, p.heads, c, p.wide);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < ILP; j++) {
+            const float x[4] = {fabsf(v[j].x), fabsf(v[j].y), fabsf(v[j].z), fabsf(v[j].w)};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (x[e] < INFINITY) m = fmaxf(m, x[e]);
         }
     }
 #pragma unroll
@@ -91,15 +105,16 @@ __global__ void __launch_bounds__(THREADS) attention_absmax_kernel(const __grid_
     }
 }
 
-template <int PER>
+template <int HD>
 __global__ void __launch_bounds__(THREADS) attention_split_kernel(const __grid_constant__ SplitArgs a) {
+    constexpr int TPL = HD / 4, LINES = THREADS / TPL;
     __shared__ float part[THREADS / 32];
     griddep_wait();
     griddep_launch_dependents();
     const Operand& p = a.op[blockIdx.y];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x % TPL * 4;
     float m = 0.0f;
-    for (int i = threadIdx.x; i < kSplitBlocks; i += THREADS) m = fmaxf(m, a.sp.partial[blockIdx.y * kSplitBlocks + i]);
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += THREADS) m = fmaxf(m, a.sp.partial[blockIdx.y * kSplitBlocks + i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) part[warp] = m;
@@ -108,58 +123,72 @@ __global__ void __launch_bounds__(THREADS) attention_split_kernel(const __grid_c
     for (int i = 1; i < THREADS / 32; i++) m = fmaxf(m, part[i]);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.sp.maxima[blockIdx.y] = m;
     const float s = split_scale_of(m);
-    for (long long i = blockIdx.x * (THREADS / 32) + warp; i < p.lines; i += gridDim.x * (THREADS / 32)) {
-        const Line l = line_of(p, i);
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (l.live) {
-            const float* x = line_ptr(p.t, l) + lane * PER;
+    const bool stats = a.backward && blockIdx.y == 3;
+    // the largest |dout row| of the head that this thread is at: a maximum of non-negative floats, the same
+    // in any order
+    int norm_head = 0;
+    float norm = 0.0f;
+    auto keep_norm = [&](int next) {
+        if (norm > 0.0f) atomicMax(reinterpret_cast<int*>(a.sp.head_norm + norm_head), __float_as_int(norm));
+        norm_head = next;
+        norm = 0.0f;
+    };
+    for (long long first = (long long)blockIdx.x * LINES * ILP; first < p.lines; first += (long long)gridDim.x * LINES * ILP) {
+        float4 v[ILP], o[ILP];
+        Line l[ILP];
+        long long at[ILP];
 #pragma unroll
-            for (int c = 0; c < PER; c++) v[c] = x[c];
-        }
-        uint32_t h[2], lo[2];
-        split2x2(v[0], v[1], s, h[0], lo[0]);
-        split2x2(v[2], v[3], s, h[1], lo[1]);
-        __half* out = p.out + i * 32 * PER + lane * PER;
-        __half* low = out + p.lines * 32 * PER;
-        if (PER == 2) {
-            *reinterpret_cast<uint32_t*>(out) = h[0];
-            *reinterpret_cast<uint32_t*>(low) = lo[0];
-        } else {
-            *reinterpret_cast<uint2*>(out) = make_uint2(h[0], h[1]);
-            *reinterpret_cast<uint2*>(low) = make_uint2(lo[0], lo[1]);
-        }
-        if (a.backward && blockIdx.y == 3) {
-            float dot = 0.0f, norm2 = 0.0f;
-            if (l.live) {
-                const float* o = line_ptr(a.o, l) + lane * PER;
-#pragma unroll
-                for (int c = 0; c < PER; c++) dot += v[c] * o[c], norm2 += v[c] * v[c];
+        for (int j = 0; j < ILP; j++) {
+            v[j] = o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            at[j] = first + j * LINES + threadIdx.x / TPL;
+            l[j] = line_of(p, (int)min(at[j], (long long)p.lines - 1));
+            if (l[j].live) {
+                v[j] = line_load(p.t, l[j], p.heads, c, p.wide);
+                if (stats) o[j] = line_load(a.o, l[j], p.heads, c, a.o_wide);
             }
+        }
 #pragma unroll
-            for (int k = 16; k > 0; k >>= 1) {
-                dot += __shfl_xor_sync(0xffffffffu, dot, k);
-                norm2 += __shfl_xor_sync(0xffffffffu, norm2, k);
+        for (int j = 0; j < ILP; j++) {
+            const bool inside = at[j] < p.lines;
+            uint2 h, lo;
+            const float x[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+            split2x4(x, s, h, lo);
+            if (inside) {
+                __half* out = p.out + at[j] * HD + c;
+                *reinterpret_cast<uint2*>(out) = h;
+                *reinterpret_cast<uint2*>(out + (long long)p.lines * HD) = lo;
             }
-            if (lane == 0) {
-                const long long sqh = l.seq * p.heads + l.head;
-                float* st = a.sp.stats + (sqh * a.q_tiles * 2 + l.row / 64) * kSplitStat + l.row % 64;
-                const float lse = l.live ? a.lse[sqh * p.rows + l.row] : -INFINITY;
-                st[0] = lse == -INFINITY ? -INFINITY : -lse * LOG2E;
-                st[64] = -dot;
-                st[128] = sqrtf(norm2);
-                // a maximum of non-negative floats, the same in any order
-                if (norm2 > 0.0f) atomicMax(reinterpret_cast<int*>(a.sp.head_norm + sqh), __float_as_int(sqrtf(norm2)));
-                // the rows of the last block of 64 that do not exist belong to it too
-                if (l.row == p.rows - 1)
-                    for (int r = p.rows; r % 64 != 0; r++) {
-                        float* e = a.sp.stats + (sqh * a.q_tiles * 2 + r / 64) * kSplitStat + r % 64;
-                        e[0] = -INFINITY;
-                        e[64] = 0.0f;
-                        e[128] = 0.0f;
-                    }
+            if (stats) {
+                float dot = x[0] * o[j].x + x[1] * o[j].y + x[2] * o[j].z + x[3] * o[j].w;
+                float norm2 = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
+#pragma unroll
+                for (int k = TPL / 2; k > 0; k >>= 1) {
+                    dot += __shfl_xor_sync(0xffffffffu, dot, k);
+                    norm2 += __shfl_xor_sync(0xffffffffu, norm2, k);
+                }
+                if (inside && c == 0) {
+                    const int row = l[j].row;
+                    float* const tiles = a.sp.stats + (long long)l[j].sh * a.q_tiles * 2 * kSplitStat;
+                    float* st = tiles + row / 64 * kSplitStat + row % 64;
+                    const float lse = l[j].live ? a.lse[(long long)l[j].sh * p.rows + row] : -INFINITY;
+                    st[0] = lse == -INFINITY ? -INFINITY : -lse * LOG2E;
+                    st[64] = -dot;
+                    st[128] = sqrtf(norm2);
+                    if (l[j].sh != norm_head) keep_norm(l[j].sh);
+                    if (norm2 > 0.0f) norm = fmaxf(norm, sqrtf(norm2));
+                    // the rows of the last block of 64 that do not exist belong to it too
+                    if (row == p.rows - 1)
+                        for (int r = p.rows; r % 64 != 0; r++) {
+                            float* e = tiles + r / 64 * kSplitStat + r % 64;
+                            e[0] = -INFINITY;
+                            e[64] = 0.0f;
+                            e[128] = 0.0f;
+                        }
+                }
             }
         }
     }
+    if (stats) keep_norm(0);
 }
 
 }  // namespace
@@ -192,6 +221,10 @@ void launch_attention_split(cudaStream_t s, const AttnArgs& a, const AttnSplitSp
     SplitArgs t{};
     const HeadsView views[4] = {a.q, a.k, a.v, a.dout};
     void* const outs[4] = {sp.q, sp.k, sp.v, sp.dout};
+    auto wide = [](const HeadsView& v) {
+        return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && v.seq % 4 == 0 && v.row % 4 == 0 && v.head % 4 == 0;
+    };
+    long long most = 0;
     for (int i = 0; i < (backward ? 4 : 3); i++) {
         const bool keys = i == 1 || i == 2;
         Operand& p = t.op[i];
@@ -199,22 +232,28 @@ void launch_attention_split(cudaStream_t s, const AttnArgs& a, const AttnSplitSp
         p.len = keys ? a.k_len : a.q_len;
         p.rows = keys ? a.k_rows : a.q_rows;
         p.heads = keys ? a.k_heads : a.q_heads;
-        p.lines = (long long)a.seqs * p.heads * p.rows;
+        const long long lines = (long long)a.seqs * p.heads * p.rows;
+        if (lines > INT_MAX) throw Error(13, "attention: more than 2^31 rows of heads");
+        p.lines = (int)lines;
+        p.wide = wide(p.t);
         p.out = static_cast<__half*>(outs[i]);
+        most = std::max(most, lines);
     }
     t.o = a.o;
+    t.o_wide = wide(a.o);
     t.lse = a.lse;
     t.sp = sp;
-    t.heads_total = (long long)a.seqs * a.q_heads;
+    t.heads_total = a.seqs * a.q_heads;
     t.q_tiles = (a.q_rows + 127) / 128;
     t.backward = backward;
-    const dim3 grid(kSplitBlocks, backward ? 4 : 3);
+    const long long per = (long long)THREADS / (a.head_dim / 4) * ILP;
+    const dim3 grid((unsigned)std::clamp<long long>((most + per - 1) / per, 1, kSplitBlocks), backward ? 4 : 3);
     if (a.head_dim == 64) {
-        launch_pdl(attention_absmax_kernel<2>, grid, dim3(THREADS), 0, s, t);
-        launch_pdl(attention_split_kernel<2>, grid, dim3(THREADS), 0, s, t);
+        launch_pdl(attention_absmax_kernel<64>, grid, dim3(THREADS), 0, s, t);
+        launch_pdl(attention_split_kernel<64>, grid, dim3(THREADS), 0, s, t);
     } else {
-        launch_pdl(attention_absmax_kernel<4>, grid, dim3(THREADS), 0, s, t);
-        launch_pdl(attention_split_kernel<4>, grid, dim3(THREADS), 0, s, t);
+        launch_pdl(attention_absmax_kernel<128>, grid, dim3(THREADS), 0, s, t);
+        launch_pdl(attention_split_kernel<128>, grid, dim3(THREADS), 0, s, t);
     }
 }
 

@@ -12,8 +12,9 @@
 //
 // A unit is one 16-byte word of each half of the rotary part (half layout), one word of
 // it (interleaved), or one word that is copied; threads walk units with the word index
-// fixed, so neighbouring threads touch neighbouring words of a head.  Sizes, strides or
-// pointers that are not multiples of 16 bytes take the same walk with single pairs.
+// fixed, so neighbouring threads touch neighbouring words of a head.  A rotary part that is
+// not whole words takes the same walk with single pairs, and single elements up to the
+// next word; strides or pointers that are not, with single elements throughout.
 
 #include <algorithm>
 #include <climits>
@@ -35,7 +36,7 @@ struct Token {
 
 template <class T, int VEC, bool HALF>
 __global__ void __launch_bounds__(THREADS)
-    rope_kernel(const __grid_constant__ RopeArgs a, const __grid_constant__ n3d_rope_plan plan, int tile) {
+    rope_kernel(const __grid_constant__ RopeArgs a, const __grid_constant__ n3d_rope_plan plan, int tile, int wide) {
     extern __shared__ float2 trig[];  // [tile][rotary_dim / 2]: m cos, m sin
     __shared__ Token tok[MAX_TOKENS];
     griddep_wait();
@@ -64,8 +65,12 @@ __global__ void __launch_bounds__(THREADS)
     }
     __syncthreads();
 
-    const int turned = (HALF ? half : a.rotary_dim) / VEC;  // words (pairs of words) that turn
-    const int words = VEC == 1 ? half + (a.head_dim - a.rotary_dim) : turned + (a.head_dim - a.rotary_dim) / VEC;
+    // words (pairs of words) that turn, then those that are copied; single pairs are followed by single
+    // elements up to the first 16-byte boundary and by whole words where the tensors allow (`wide`)
+    constexpr int WORD = 16 / (int)sizeof(T);
+    const int turned = (HALF || VEC == 1 ? half : a.rotary_dim) / VEC, rest = a.head_dim - a.rotary_dim;
+    const int single = VEC > 1 ? 0 : wide ? min(rest, (WORD - a.rotary_dim % WORD) % WORD) : rest;
+    const int words = turned + single + (rest - single) / (VEC > 1 ? VEC : WORD);
     const int lanes = THREADS / words;  // (token, head) rows a block walks at a time
     const int w = threadIdx.x % words;
     int h = threadIdx.x / words, t = 0;
@@ -73,7 +78,7 @@ __global__ void __launch_bounds__(THREADS)
     t = h / a.heads;
     h -= t * a.heads;
     const int dt = lanes / a.heads, dh = lanes - dt * a.heads;
-    const bool turns = VEC == 1 ? w < half : w < turned;
+    const bool turns = w < turned;
     for (; t < nt; t += dt, h += dh) {
         if (h >= a.heads) {
             h -= a.heads;
@@ -85,10 +90,15 @@ __global__ void __launch_bounds__(THREADS)
         T* y = static_cast<T*>(a.y[which].p) + tok[t].y[which] + hh * a.y[which].head;
         if (!turns) {
             if (a.in_place[which]) continue;
-            const int c = a.rotary_dim + (VEC == 1 ? w - half : (w - turned) * VEC);
-            Vec<T, VEC> v;
-            v.load_rw(x + c);
-            v.store(y + c);
+            const int i = w - turned;
+            if (i < single) {
+                y[a.rotary_dim + i] = x[a.rotary_dim + i];
+            } else {
+                const int c = a.rotary_dim + single + (i - single) * WORD;
+                Vec<T, WORD> v;
+                v.load_rw(x + c);
+                v.store(y + c);
+            }
         } else if (HALF || VEC == 1) {
             const int ca = HALF ? w * VEC : 2 * w, cb = HALF ? half + w * VEC : 2 * w + 1;
             Vec<T, VEC> va, vb;
@@ -127,31 +137,32 @@ __global__ void __launch_bounds__(THREADS)
 }
 
 template <class T, int VEC, bool HALF>
-void launch(cudaStream_t s, const RopeArgs& a, const n3d_rope_plan& plan) {
-    const int half = a.rotary_dim / 2, rest = a.head_dim - a.rotary_dim;
-    const int words = VEC == 1 ? half + rest : (HALF ? half : a.rotary_dim) / VEC + rest / VEC;
+void launch(cudaStream_t s, const RopeArgs& a, const n3d_rope_plan& plan, bool wide) {
+    const int half = a.rotary_dim / 2, rest = a.head_dim - a.rotary_dim, word = 16 / (int)sizeof(T);
+    const int words = VEC == 1 ? half + (wide ? rest / word + 1 : rest) : (HALF ? half : a.rotary_dim) / VEC + rest / VEC;
     // about 8 units per thread, halved while that leaves SMs without four blocks
     int tile = (int)std::clamp<long long>(8LL * THREADS / ((long long)words * a.heads), 1, MAX_TOKENS);
     while (tile > 1 && (a.tokens + tile - 1) / tile < 4LL * sm_count()) tile /= 2;
     const long long blocks = (a.tokens + tile - 1) / tile;
     if (blocks > INT_MAX) throw Error(13, "n3d_rope: more than 2^31 blocks of tokens");
     launch_pdl(rope_kernel<T, VEC, HALF>, dim3((unsigned)blocks), dim3(THREADS), (size_t)tile * half * sizeof(float2), s,
-               a, plan, tile);
+               a, plan, tile, (int)wide);
 }
 
 template <class T>
 void launch_type(cudaStream_t s, const RopeArgs& a, const n3d_rope_plan& plan) {
     constexpr int VEC = 16 / (int)sizeof(T);
     const bool half = plan.layout == N3D_ROPE_HALF;
-    bool wide = a.head_dim % VEC == 0 && (half ? a.rotary_dim / 2 : a.rotary_dim) % VEC == 0;
+    bool wide = a.head_dim % VEC == 0;  // whole 16-byte words of the tensors, if not of the rotary part
     for (int i = 0; i < 2; i++)
         for (const HeadsView* v : {&a.x[i], &a.y[i]})
             wide = wide && reinterpret_cast<uintptr_t>(v->p) % 16 == 0 && v->seq % VEC == 0 && v->row % VEC == 0 &&
                    v->head % VEC == 0;
+    const bool words = wide && (half ? a.rotary_dim / 2 : a.rotary_dim) % VEC == 0;
     if (half)
-        wide ? launch<T, VEC, true>(s, a, plan) : launch<T, 1, true>(s, a, plan);
+        words ? launch<T, VEC, true>(s, a, plan, true) : launch<T, 1, true>(s, a, plan, wide);
     else
-        wide ? launch<T, VEC, false>(s, a, plan) : launch<T, 1, false>(s, a, plan);
+        words ? launch<T, VEC, false>(s, a, plan, true) : launch<T, 1, false>(s, a, plan, wide);
 }
 
 }  // namespace
