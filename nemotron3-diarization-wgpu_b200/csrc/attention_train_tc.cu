@@ -613,6 +613,8 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 return static_cast<float*>(t.p) + (long long)seq * t.seq + (long long)head * t.head + (long long)row * t.row;
             };
 
+            // dq, 16-bit: does the row see keys of one block only?  Then D is taken from that block (below)
+            const bool single = MODE == GRAD_Q && !PAIR && live && hi > lo && (hi - 1) / COLS == lo / COLS;
             // dq: this row's -lse log2 e, -D and fp16 scale; dkv: the fp16 scale of the head group
             float nlse = 0.0f, ndot = 0.0f, ds_scale = 1.0f;
             if (MODE == GRAD_Q && PAIR) {
@@ -650,7 +652,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 if (wg == 0) {
                     float* st = args.stats + ((sqh * args.q_tiles + r0 / ROWS) * 2 + r / 64) * 128 + r % 64;
                     st[0] = nlse;
-                    st[64] = ndot;
+                    if (!single) st[64] = ndot;
                     if (F16) {
                         float m = norm;
 #pragma unroll
@@ -759,6 +761,30 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     if (MODE == GRAD_KV)  // the statistics came by bulk copy: this thread's own wait makes them visible
                         ok = __all_sync(0xffffffffu,
                                         ok && mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                    // A row of few keys has large P, and dP - D cancels: with D from the rounded output, dS would
+                    // keep that rounding (a row with one key has dS = 0).  Where the row's keys are all here,
+                    // D = sum P dP, for dkv too.
+                    if constexpr (MODE == GRAD_Q && !PAIR) {
+                        const bool here = single && lo / COLS * COLS == c0;
+                        if (__any_sync(0xffffffffu, here)) {
+                            float d = 0.0f;
+#pragma unroll 1
+                            for (int h = 0; h < COLS; h += 16) {
+                                float s[16], u[16];
+                                tmem_ld_pair<16>(t + h, t + 64 + h, s, u);
+#pragma unroll
+                                for (int c = 0; c < 16; c++) {
+                                    const int cc = c0 + h + c;
+                                    if (cc >= lo && cc < hi) d += ex2_approx(fmaf(s[c], k2, nlse)) * u[c];
+                                }
+                            }
+                            if (here) {
+                                ndot = -d;
+                                args.stats[((((long long)seq * a.q_heads + head) * args.q_tiles + r0 / ROWS) * 2 + r / 64) * 128 +
+                                           64 + r % 64] = ndot;
+                            }
+                        }
+                    }
                     auto weights = [&](auto masked) {
                         constexpr int CH = C::CHUNK;
 #pragma unroll
