@@ -637,6 +637,7 @@ _pack_rows = struct.Struct("Pq").pack               # n3d_rows
 _pack_residual = struct.Struct("NNiiiifff4xN").pack  # n3d_residual_config
 _pack_attn = struct.Struct("NNNNif qqq").pack       # n3d_attn_config
 _dtype_codes: dict = {}                             # a library's dtype object -> n3d_dtype
+_dtype_names: dict = {}                             # -> its name
 
 
 def _bad(message: str) -> DiarizationError:
@@ -660,28 +661,33 @@ def _device(t) -> int:
     return d
 
 
-def _heads(t, seqs, rows, heads, hd, dtype, device):
-    """The fields of n3d_heads of a [seqs, rows, heads, hd] tensor (heads None: any)."""
-    if len(t.shape) != 4:
-        raise _bad("a [seqs, rows, heads, head_dim] tensor is wanted")
-    s, r, h, d = t.shape
-    a, b, c, e = t.stride()
-    if s != seqs or r != rows or d != hd or (h != heads and heads is not None):
-        raise _bad(f"a tensor of shape {tuple(t.shape)} where {(seqs, rows, heads, hd)} is wanted")
+def _refuse(t, shape, dtype, device):
+    """Says what is wrong with a tensor that is not of this shape and type, or on another device."""
+    if tuple(t.shape) != tuple(shape):
+        raise _bad(f"a tensor of shape {tuple(t.shape)} where {tuple(shape)} is wanted")
     if t.dtype != dtype:
         raise _bad(f"a tensor of type {t.dtype} where {dtype} is wanted")
-    if e != 1 and d > 1:
+    raise _bad(f"a tensor on device {t.get_device()} where {device} is wanted")
+
+
+def _heads(t, shape, dtype, device):
+    """The fields of n3d_heads of a [seqs, rows, heads, hd] tensor."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != device:
+        _refuse(t, shape, dtype, device)
+    a, b, c, e = t.stride()
+    if e != 1 and shape[3] > 1:
         raise _bad("the elements of a head must be consecutive")
-    if t.get_device() != device:
-        raise _bad("the tensors are not all on one device")
-    return t.data_ptr(), h, a, b, c
+    return t.data_ptr(), shape[2], a, b, c
 
 
 def _flat(t, count: int, dtype: str, device: int):
     """The pointer of a contiguous tensor of `count` elements (None: NULL)."""
     if t is None:
         return None
-    if t.numel() != count or not t.is_contiguous() or t.get_device() != device or str(t.dtype).rpartition(".")[2] != dtype:
+    name = _dtype_names.get(t.dtype)
+    if name is None:
+        name = _dtype_names[t.dtype] = str(t.dtype).rpartition(".")[2]
+    if name != dtype or t.numel() != count or t.get_device() != device or not t.is_contiguous():
         raise _bad(f"a contiguous {dtype} tensor of {count} elements on device {device} is wanted")
     return t.data_ptr()
 
@@ -734,46 +740,46 @@ def rope(plan: RopePlan, xs, ys, positions=None, first_position: int = 0, transp
     n = len(xs)
     if n not in (1, 2) or len(ys) != n or len(xs[0].shape) != 4:
         raise _bad("rope: one or two [seqs, rows, heads, head_dim] tensors, and as many outputs, are wanted")
-    seqs, rows, heads, hd = xs[0].shape
+    q = xs[0]
+    shape, dt, dev = q.shape, q.dtype, _device(q)
+    seqs, rows, _, hd = shape
     if hd != plan.head_dim:
         raise _bad(f"rope: head_dim {hd}, the plan has {plan.head_dim}")
-    dt, dev = xs[0].dtype, _device(xs[0])
-    x = _heads(xs[0], seqs, rows, heads, hd, dt, dev)
-    y = _heads(ys[0], seqs, rows, heads, hd, dt, dev)
     if n == 2:
-        x1 = _heads(xs[1], seqs, rows, None, hd, dt, dev)
-        x, y = _pack_heads2(*x, *x1), _pack_heads2(*y, *_heads(ys[1], seqs, rows, x1[1], hd, dt, dev))
+        k = xs[1]
+        other = k.shape
+        if len(other) != 4 or other[0] != seqs or other[1] != rows or other[3] != hd:
+            raise _bad("rope: the tensors differ in more than their heads")
+        x = _pack_heads2(*_heads(q, shape, dt, dev), *_heads(k, other, dt, dev))
+        y = _pack_heads2(*_heads(ys[0], shape, dt, dev), *_heads(ys[1], other, dt, dev))
     else:
-        x, y = _pack_heads(*x), _pack_heads(*y)
+        x, y = _pack_heads(*_heads(q, shape, dt, dev)), _pack_heads(*_heads(ys[0], shape, dt, dev))
     st = (_lib or lib()).n3d_rope(dev, plan._at, _dtype(dt), seqs, rows, n, x, y,
                                   _flat(positions, seqs * rows, "int32", dev), first_position, transpose, stream)
     if st:
         _check(st)
 
 
-def _matrix(t, rows, cols, dtype, device):
+def _matrix(t, shape, dtype, device):
     """A [rows, cols] tensor as n3d_rows (None: NULL)."""
     if t is None:
         return None
-    if tuple(t.shape) != (rows, cols):
-        raise _bad(f"a matrix of shape {tuple(t.shape)} where {(rows, cols)} is wanted")
-    if t.dtype != dtype:
-        raise _bad(f"a matrix of type {t.dtype} where {dtype} is wanted")
+    if t.shape != shape or t.dtype != dtype or t.get_device() != device:
+        _refuse(t, shape, dtype, device)
     a, b = t.stride()
-    if b != 1 and cols > 1:
+    if b != 1 and shape[1] > 1:
         raise _bad("the elements of a row must be consecutive")
-    if t.get_device() != device:
-        raise _bad("the tensors are not all on one device")
     return _pack_rows(t.data_ptr(), a)
 
 
 def _residual_config(residual, block, post, pre, eps, scale, gate, gate_rows):
-    """(n3d_residual_config, rows, cols, values of the gate)"""
+    """(n3d_residual_config, shape, cols, values of the gate)"""
     if post not in NORMS or pre not in NORMS:
         raise _bad(f"unknown norm {post} or {pre}")
-    if len(block.shape) != 2:
+    shape = block.shape
+    if len(shape) != 2:
         raise _bad("a [rows, cols] matrix is wanted")
-    rows, cols = block.shape
+    rows, cols = shape
     if gate is None:
         gate_rows = gates = 0
     elif gate_rows < 1:
@@ -781,7 +787,7 @@ def _residual_config(residual, block, post, pre, eps, scale, gate, gate_rows):
     else:
         gates = -(-rows // gate_rows) * cols
     return _pack_residual(rows, cols, _dtype(residual.dtype), _dtype(block.dtype), NORMS[post], NORMS[pre], eps, eps,
-                          scale, gate_rows), rows, cols, gates
+                          scale, gate_rows), shape, cols, gates
 
 
 def residual_norm(x, block, r, y, post: str = "none", pre: str = "layer", eps: float = 1e-5, scale: float = 1.0,
@@ -790,13 +796,13 @@ def residual_norm(x, block, r, y, post: str = "none", pre: str = "layer", eps: f
     """r = x + scale * gate * Norm_post(block), y = Norm_pre(r) (n3d_residual_norm); norms are "none",
     "layer" or "rms".  gate [ceil(rows / gate_rows), cols], weights and biases [cols]: fp32 or None.
     r may be x, y may be block; y is None when pre is "none"."""
-    cfg, rows, cols, gates = _residual_config(x, block, post, pre, eps, scale, gate, gate_rows)
+    cfg, sh, cols, gates = _residual_config(x, block, post, pre, eps, scale, gate, gate_rows)
     dev, rt, bt = _device(x), x.dtype, block.dtype
     st = (_lib or lib()).n3d_residual_norm(
-        dev, cfg, _matrix(x, rows, cols, rt, dev), _matrix(block, rows, cols, bt, dev),
+        dev, cfg, _matrix(x, sh, rt, dev), _matrix(block, sh, bt, dev),
         _flat(post_w, cols, "float32", dev), _flat(post_b, cols, "float32", dev), _flat(gate, gates, "float32", dev),
-        _flat(pre_w, cols, "float32", dev), _flat(pre_b, cols, "float32", dev), _matrix(r, rows, cols, rt, dev),
-        _matrix(y, rows, cols, bt, dev), stream)
+        _flat(pre_w, cols, "float32", dev), _flat(pre_b, cols, "float32", dev), _matrix(r, sh, rt, dev),
+        _matrix(y, sh, bt, dev), stream)
     if st:
         _check(st)
 
@@ -813,14 +819,14 @@ def residual_norm_grad(block, r, dy, dr, dx, dblock, post: str = "none", pre: st
     """The gradient of residual_norm (n3d_residual_norm_grad): dy and dr (or None) -> dx, dblock, and the
     fp32 gradients that are not None.  `workspace`: a tensor of at least residual_norm_workspace bytes.
     pre_b does not enter; it is accepted so that both calls take the same arguments."""
-    cfg, rows, cols, gates = _residual_config(dx, block, post, pre, eps, scale, gate, gate_rows)
+    cfg, sh, cols, gates = _residual_config(dx, block, post, pre, eps, scale, gate, gate_rows)
     dev, rt, bt = _device(dx), dx.dtype, block.dtype
     f = "float32"
     st = (_lib or lib()).n3d_residual_norm_grad(
-        dev, cfg, _matrix(block, rows, cols, bt, dev), _matrix(r, rows, cols, rt, dev), _flat(post_w, cols, f, dev),
+        dev, cfg, _matrix(block, sh, bt, dev), _matrix(r, sh, rt, dev), _flat(post_w, cols, f, dev),
         _flat(post_b, cols, f, dev), _flat(gate, gates, f, dev), _flat(pre_w, cols, f, dev),
-        _matrix(dy, rows, cols, bt, dev), _matrix(dr, rows, cols, rt, dev), _matrix(dx, rows, cols, rt, dev),
-        _matrix(dblock, rows, cols, bt, dev), _flat(dgate, gates, f, dev), _flat(dpost_w, cols, f, dev),
+        _matrix(dy, sh, bt, dev), _matrix(dr, sh, rt, dev), _matrix(dx, sh, rt, dev),
+        _matrix(dblock, sh, bt, dev), _flat(dgate, gates, f, dev), _flat(dpost_w, cols, f, dev),
         _flat(dpost_b, cols, f, dev), _flat(dpre_w, cols, f, dev), _flat(dpre_b, cols, f, dev), *_space(workspace, dev),
         stream)
     if st:
@@ -850,13 +856,14 @@ def attention_forward(q, k, v, out, lse=None, q_len=None, k_len=None, scale: flo
     q_len, k_len: int32 [seqs]; left, right: the window around key row i + q_offset, negative for no limit."""
     cfg = _attn_config(q, k, scale, left, right, q_offset)
     dev, dt = _device(q), q.dtype
-    b, nq, hq, hd = q.shape
-    _, nk, hk, _ = k.shape
+    qs, ks = q.shape, k.shape
+    b, nq, hq, hd = qs
+    if ks[0] != b or ks[3] != hd:
+        _refuse(k, (b, ks[1], ks[2], hd), dt, dev)
     st = (_lib or lib()).n3d_attention_forward(
-        dev, cfg, _pack_heads(*_heads(q, b, nq, hq, hd, dt, dev)), _pack_heads(*_heads(k, b, nk, hk, hd, dt, dev)),
-        _pack_heads(*_heads(v, b, nk, hk, hd, dt, dev)), _flat(q_len, b, "int32", dev), _flat(k_len, b, "int32", dev),
-        _pack_heads(*_heads(out, b, nq, hq, hd, dt, dev)), _flat(lse, b * hq * nq, "float32", dev),
-        *_space(workspace, dev), stream)
+        dev, cfg, _pack_heads(*_heads(q, qs, dt, dev)), _pack_heads(*_heads(k, ks, dt, dev)),
+        _pack_heads(*_heads(v, ks, dt, dev)), _flat(q_len, b, "int32", dev), _flat(k_len, b, "int32", dev),
+        _pack_heads(*_heads(out, qs, dt, dev)), _flat(lse, b * hq * nq, "float32", dev), *_space(workspace, dev), stream)
     if st:
         _check(st)
 
@@ -867,10 +874,12 @@ def attention_backward(q, k, v, out, lse, dout, dq, dk, dv, q_len=None, k_len=No
     `workspace`: a tensor of at least attention_workspace bytes."""
     cfg = _attn_config(q, k, scale, left, right, q_offset)
     dev, dt = _device(q), q.dtype
-    b, nq, hq, hd = q.shape
-    _, nk, hk, _ = k.shape
-    qs = [_pack_heads(*_heads(t, b, nq, hq, hd, dt, dev)) for t in (q, out, dout, dq)]
-    ks = [_pack_heads(*_heads(t, b, nk, hk, hd, dt, dev)) for t in (k, v, dk, dv)]
+    shape, other = q.shape, k.shape
+    b, nq, hq, hd = shape
+    if other[0] != b or other[3] != hd:
+        _refuse(k, (b, other[1], other[2], hd), dt, dev)
+    qs = [_pack_heads(*_heads(t, shape, dt, dev)) for t in (q, out, dout, dq)]
+    ks = [_pack_heads(*_heads(t, other, dt, dev)) for t in (k, v, dk, dv)]
     st = (_lib or lib()).n3d_attention_backward(
         dev, cfg, qs[0], ks[0], ks[1], qs[1], _flat(lse, b * hq * nq, "float32", dev), qs[2],
         _flat(q_len, b, "int32", dev), _flat(k_len, b, "int32", dev), qs[3], ks[2], ks[3], *_space(workspace, dev),
