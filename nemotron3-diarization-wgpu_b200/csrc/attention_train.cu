@@ -1,5 +1,7 @@
 // Attention with its gradient on the fp32 units (n3d_attention_forward, _backward), for
-// fp32 tensors and for tensors whose pointers or strides are not whole 16-byte words.
+// tensors that the tensor-core kernels do not take: 16-bit ones whose pointers or strides
+// are not whole 16-byte words, or that are broadcast, and fp32 ones of at most 64 query and
+// key rows (forward only; the rule and its figures are in attention_train_tc.cu).
 //
 // With S = scale q k^T and lse from the forward pass, P = exp(S - lse) is computed again:
 //   D = sum_d dout out,  dP = dout v^T,  dS = P (dP - D)
@@ -17,7 +19,8 @@
 // Bound: fp32 FMA issue and shared-memory reads about equally: 256 threads as 16 x 16
 // hold 4 x 4 scores (rows 4 ty + i, columns tx + 16 j) and 4 x head_dim / 16 accumulators
 // each; one 16-byte shared read feeds 8 FMAs.  Row padding of 16 bytes keeps the column
-// reads free of bank conflicts.
+// reads free of bank conflicts.  Measured on a B200 in fp32: 8 x 256 rows, 8 heads of 64, forward
+// 49 us, gradient 155 us (11 and 12 TFLOP/s); tensor cores take 25 and 43.
 
 #include <climits>
 
