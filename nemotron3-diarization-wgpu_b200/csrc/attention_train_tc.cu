@@ -79,8 +79,8 @@ struct Cfg {
     static constexpr bool PAIR = PARTS == 2;
     // column blocks in softmax at a time (an fp32 forward pass of head_dim 128 has TMEM for one)
     static constexpr int NWG = SMALL || (PAIR && HD == 128 && MODE == FORWARD) ? 1 : 2;
-    static constexpr int CHUNK = 16;                        // columns a thread has in registers at a time (gradients)
-    static constexpr int NBUF = MODE == FORWARD ? 2 : NWG;  // score buffers
+    static constexpr bool ROW_TMEM = !PAIR && (MODE == GRAD_Q || (MODE == FORWARD && HD == 128));
+    static constexpr int NBUF = MODE != FORWARD ? NWG : PAIR || HD == 64 ? 2 : ROW_TMEM ? 3 : 4;  // score buffers
     static constexpr int SOFTMAX = 3;                       // first softmax warp
     static constexpr int THREADS = 32 * SOFTMAX + 128 * NWG, PER_SM = SMALL ? 2 : 1;
     static constexpr int RTILE = ROWS * HD * 2 * PARTS, CTILE = COLS * HD * 2 * PARTS;  // bytes
@@ -105,10 +105,9 @@ struct Cfg {
     // pairs: the accumulators are added up after them (see the head of the file); dk and dv
     // of head_dim 128 are added up in the output tensors, for which there is no TMEM
     static constexpr bool SUM = PAIR, SUM_OUT = PAIR && HD == 128 && MODE == GRAD_KV;
+    static constexpr uint32_t ROWT = ACC + (SUM && !SUM_OUT ? 2 : 1) * NACC * HD;  // first column of the row tiles
     static constexpr uint32_t TMEM_COLS = SMALL ? 256 : 512;
-    static_assert(COLS % CHUNK == 0, "whole chunks");
-    static_assert(NBUF % NWG == 0, "a score buffer belongs to one softmax group");
-    static_assert(ACC + (SUM && !SUM_OUT ? 2 : 1) * NACC * HD <= TMEM_COLS && PER_SM * TMEM_COLS <= 512, "TMEM");
+    static_assert(ROWT + (ROW_TMEM ? (GRAD ? 2 : 1) * HD / 2 : 0) <= TMEM_COLS && PER_SM * TMEM_COLS <= 512, "TMEM");
     static_assert(NST >= 1 && (SMEM + 1024) * PER_SM <= 228 * 1024, "shared memory");
 };
 
@@ -198,44 +197,23 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t* v) {
     static_assert(N == 8 || N == 16, "8 or 16 columns");
     N == 8 ? tmem_st8(taddr, v) : tmem_st16(taddr, v);
 }
-// N columns at each of two places of this thread's lane: both loads, one wait.
-template <int N>
+// 16 columns at each of two places of this thread's lane: both loads, one wait.
 __device__ __forceinline__ void tmem_ld_pair(uint32_t a, uint32_t b, float* x, float* y) {
-    static_assert(N == 16 || N == 32, "16 or 32 columns");
-    uint32_t r[2 * N];
+    uint32_t r[32];
 #pragma unroll
     for (int h = 0; h < 2; h++)
-        if constexpr (N == 16)
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                : "=r"(r[N * h + 0]), "=r"(r[N * h + 1]), "=r"(r[N * h + 2]), "=r"(r[N * h + 3]), "=r"(r[N * h + 4]),
-                  "=r"(r[N * h + 5]), "=r"(r[N * h + 6]), "=r"(r[N * h + 7]), "=r"(r[N * h + 8]), "=r"(r[N * h + 9]),
-                  "=r"(r[N * h + 10]), "=r"(r[N * h + 11]), "=r"(r[N * h + 12]), "=r"(r[N * h + 13]),
-                  "=r"(r[N * h + 14]), "=r"(r[N * h + 15])
-                : "r"(h ? b : a));
-        else
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-                "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                : "=r"(r[N * h + 0]), "=r"(r[N * h + 1]), "=r"(r[N * h + 2]), "=r"(r[N * h + 3]), "=r"(r[N * h + 4]),
-                  "=r"(r[N * h + 5]), "=r"(r[N * h + 6]), "=r"(r[N * h + 7]), "=r"(r[N * h + 8]), "=r"(r[N * h + 9]),
-                  "=r"(r[N * h + 10]), "=r"(r[N * h + 11]), "=r"(r[N * h + 12]), "=r"(r[N * h + 13]),
-                  "=r"(r[N * h + 14]), "=r"(r[N * h + 15]), "=r"(r[N * h + 16]), "=r"(r[N * h + 17]),
-                  "=r"(r[N * h + 18]), "=r"(r[N * h + 19]), "=r"(r[N * h + 20]), "=r"(r[N * h + 21]),
-                  "=r"(r[N * h + 22]), "=r"(r[N * h + 23]), "=r"(r[N * h + 24]), "=r"(r[N * h + 25]),
-                  "=r"(r[N * h + 26]), "=r"(r[N * h + 27]), "=r"(r[N * h + 28]), "=r"(r[N * h + 29]),
-                  "=r"(r[N * h + 30]), "=r"(r[N * h + 31])
-                : "r"(h ? b : a));
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[16 * h + 0]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]), "=r"(r[16 * h + 4]),
+              "=r"(r[16 * h + 5]), "=r"(r[16 * h + 6]), "=r"(r[16 * h + 7]), "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]),
+              "=r"(r[16 * h + 10]), "=r"(r[16 * h + 11]), "=r"(r[16 * h + 12]), "=r"(r[16 * h + 13]),
+              "=r"(r[16 * h + 14]), "=r"(r[16 * h + 15])
+            : "r"(h ? b : a));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
     reg_fence16(r);
     reg_fence16(r + 16);
-    if constexpr (N == 32) {
-        reg_fence16(r + 32);
-        reg_fence16(r + 48);
-    }
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] = __uint_as_float(r[i]), y[i] = __uint_as_float(r[N + i]);
+    for (int i = 0; i < 16; i++) x[i] = __uint_as_float(r[i]), y[i] = __uint_as_float(r[16 + i]);
 }
 __device__ __forceinline__ float max3f(float a, float b, float c) {
     float r;
@@ -309,19 +287,20 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
     uint64_t* c_full = r_free + 2;         // NST: the column tiles of block g landed (stage g % NST)
     uint64_t* c_empty = c_full + 4;        // NST: block g's second products completed
     uint64_t* t_full = c_empty + 4;        // NBUF: T of block g completed (buffer g % NBUF)
-    uint64_t* p_full = t_full + 2;         // NBUF: weights of block g written
-    uint64_t* acc_done = p_full + 2;       // NBUF: second products of block g completed
-    uint64_t* acc_free = acc_done + 2;     // NWG (pairs): the accumulator is added to its sum (4 warps)
+    uint64_t* p_full = t_full + 4;         // NBUF: weights of block g written
+    uint64_t* acc_done = p_full + 4;       // NBUF: second products of block g completed
+    uint64_t* acc_free = acc_done + 4;     // NWG (pairs): the accumulator is added to its sum (4 warps)
     uint64_t* all_done = acc_free + 2;     // 1: phase n = the last product of loaded item n completed
     uint64_t* acc_read = all_done + 1;     // 1: phase n = its accumulators are read (every softmax warp)
-    uint64_t* item_full = acc_read + 1;    // 2: item k is known (slot k % 2)
+    uint64_t* rows_in = acc_read + 1;      // 1: phase n = its row tiles are in TMEM (every softmax warp)
+    uint64_t* item_full = rows_in + 1;     // 2: item k is known (slot k % 2)
     uint64_t* item_empty = item_full + 2;  // 2: item k was read by every other warp
     uint64_t* answered = item_empty + 2;   // 1: the scheduler's answer arrived
-    static_assert(NST <= 4 && NBUF <= 2 && NWG <= 2 && C::RB <= 2, "barriers");
-    Item* items = reinterpret_cast<Item*>(bars + 32);  // 2
-    uint8_t* answer = reinterpret_cast<uint8_t*>(bars + 44);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46);
-    float* joins = reinterpret_cast<float*>(bars + 48);  // 2 x JOIN
+    static_assert(NST <= 4 && NBUF <= 4 && NWG <= 2 && C::RB <= 2, "barriers");
+    Item* items = reinterpret_cast<Item*>(bars + 36);  // 2
+    uint8_t* answer = reinterpret_cast<uint8_t*>(bars + 48);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 50);
+    float* joins = reinterpret_cast<float*>(bars + 52);  // 2 x JOIN
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0 && lane == 0) {
@@ -332,6 +311,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         for (int i = 0; i < NWG; i++) mbar_init(&acc_free[i], 4);
         mbar_init(all_done, 1);
         mbar_init(acc_read, 4 * NWG);
+        mbar_init(rows_in, 4 * NWG);
         for (int i = 0; i < 2; i++) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 2 + 4 * NWG);
         mbar_init(answered, 1);
         mbar_fence_init();
@@ -482,9 +462,11 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             if (it.nblk == 0) continue;
             uint8_t* rows1 = rows + n % C::RB * C::ROW_BYTES;
             uint8_t* rows2 = rows1 + C::RTILE;
-            // (phase n / RB; the next needs this item's outputs)
-            ok = __all_sync(0xffffffffu, mbar_wait(&r_full[n % C::RB], (n / C::RB) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-            if (!PAIR && ok && it.r0 + ROWS > it.row_len && it.row_len < row_cap) {
+            // (in TMEM phase n, in shared memory phase n / RB; the next needs this item's outputs)
+            ok = __all_sync(0xffffffffu,
+                            C::ROW_TMEM ? mbar_wait(rows_in, n & 1, err, DEV_TIMEOUT_ATTN_TRAIN)
+                                        : mbar_wait(&r_full[n % C::RB], (n / C::RB) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            if (!PAIR && !C::ROW_TMEM && ok && it.r0 + ROWS > it.row_len && it.row_len < row_cap) {
                 clear(rows1, it.row_len - it.r0, ROWS);
                 if (C::GRAD) clear(rows2, it.row_len - it.r0, ROWS);
                 fence_async_smem();
@@ -525,8 +507,12 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                                                     (kk % 4) * 32;
                                 const uint32_t co = b + i * C::CTILE + (PAIR && c == 1 ? CPART : 0) + (kk / 4) * BOX +
                                                     (kk % 4) * 32;
-                                umma_f16(t + 64 * i, desc_k_sw128(ro), desc_k_sw128(co),
-                                         i == 0 && args.negate ? t_neg : t_desc, kk + c != 0);
+                                const uint32_t desc = i == 0 && args.negate ? t_neg : t_desc;
+                                if constexpr (C::ROW_TMEM)
+                                    umma_f16_ts(t + 64 * i, tmem + C::ROWT + i * HD / 2 + kk * 8, desc_k_sw128(co), desc,
+                                                kk + c != 0);
+                                else
+                                    umma_f16(t + 64 * i, desc_k_sw128(ro), desc_k_sw128(co), desc, kk + c != 0);
                             }
                     umma_commit(&t_full[g % NBUF]);
                 }
@@ -619,6 +605,32 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             auto out_row = [&](const HeadsView& t) {
                 return static_cast<float*>(t.p) + (long long)seq * t.seq + (long long)head * t.head + (long long)row * t.row;
             };
+
+            // The row tiles go to TMEM as the A operands of T; what they held for the item before was read by
+            // products that its all_done covers.  Rows past the length are zeros there.
+            if (C::ROW_TMEM && nblk > 0) {
+                // (phase n / RB; the next needs this item's outputs)
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(&r_full[n % C::RB], (n / C::RB) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+#pragma unroll 1
+                for (int i = wg; i < (C::GRAD ? 2 : 1) * HD / 64; i += NWG) {  // 64 elements: 32 columns
+                    const uint8_t* from = rows1 + i * 2 * BOX + r * 128;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(from + (((4 * h + j) ^ (r & 7)) << 4));
+                            w[4 * j] = live ? x.x : 0, w[4 * j + 1] = live ? x.y : 0;
+                            w[4 * j + 2] = live ? x.z : 0, w[4 * j + 3] = live ? x.w : 0;
+                        }
+                        tmem_st16(lb + C::ROWT + i * 32 + h * 16, w);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(rows_in);
+            }
 
             // dq, 16-bit: does the row see keys of one block only?  Then D is taken from that block (below)
             const bool single = MODE == GRAD_Q && !PAIR && live && hi > lo && (hi - 1) / COLS == lo / COLS;
@@ -778,7 +790,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
 #pragma unroll 1
                             for (int h = 0; h < COLS; h += 16) {
                                 float s[16], u[16];
-                                tmem_ld_pair<16>(t + h, t + 64 + h, s, u);
+                                tmem_ld_pair(t + h, t + 64 + h, s, u);
 #pragma unroll
                                 for (int c = 0; c < 16; c++) {
                                     const int cc = c0 + h + c;
@@ -793,11 +805,11 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                         }
                     }
                     auto weights = [&](auto masked) {
-                        constexpr int CH = C::CHUNK;
+                        constexpr int CH = 16;  // columns in registers at a time
 #pragma unroll
                         for (int h = 0; h < COLS; h += CH) {  // the weights go over scores that are read already
                             float s[CH], u[CH];
-                            tmem_ld_pair<CH>(t + h, t + 64 + h, s, u);
+                            tmem_ld_pair(t + h, t + 64 + h, s, u);
                             uint32_t pw[CH / 2 * PARTS], dw[CH / 2 * PARTS];  // pairs: h, then l
 #pragma unroll
                             for (int c = 0; c < CH; c += 4) {
