@@ -302,7 +302,10 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 50);
     float* joins = reinterpret_cast<float*>(bars + 52);  // 2 x JOIN
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // The reduction tells the compiler that a value is the same in the warp, which keeps what the issuing warps
+    // derive from it in uniform registers, where MMAs take their operands from.
+    auto uniform = [](int x) { return (int)__reduce_max_sync(0xffffffffu, x); };
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < C::RB; i++) mbar_init(&r_full[i], 1), mbar_init(&r_free[i], 4 * NWG);
         for (int i = 0; i < NST; i++) mbar_init(&c_full[i], 1), mbar_init(&c_empty[i], 1);
@@ -320,7 +323,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
     griddep_wait();
     griddep_launch_dependents();
 
@@ -342,6 +345,13 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_empty[k & 1]);
         return it.valid != 0;
+    };
+    // the same for an issuing warp
+    auto next_uniform = [&](int k, Item& it) {
+        const bool more = next_item(k, it);
+        it.r0 = uniform(it.r0), it.row_len = uniform(it.row_len), it.col_len = uniform(it.col_len);
+        it.c_begin = uniform(it.c_begin), it.per_head = uniform(it.per_head), it.nblk = uniform(it.nblk);
+        return (bool)__all_sync(0xffffffffu, more);
     };
 
     // Every role walks the same items; g counts the column blocks and n the items with any, over all of them:
@@ -458,7 +468,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         const uint32_t t_desc = idesc<T>(COLS, false, false), t_neg = idesc<T>(COLS, false, true);
         bool ok = true;
         Item it;
-        for (int k = 0, gt = 0, n = 0; ok && next_item(k, it); k++) {
+        for (int k = 0, gt = 0, n = 0; ok && next_uniform(k, it); k++) {
             if (it.nblk == 0) continue;
             uint8_t* rows1 = rows + n % C::RB * C::ROW_BYTES;
             uint8_t* rows2 = rows1 + C::RTILE;
@@ -529,7 +539,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         bool ok = true;
         Item it;
         int added[2] = {0, 0};  // pairs: sums of each accumulator taken so far
-        for (int k = 0, gt = 0, n = 0; ok && next_item(k, it); k++) {
+        for (int k = 0, gt = 0, n = 0; ok && next_uniform(k, it); k++) {
             if (it.nblk == 0) continue;
             // the accumulators of the item before (phase n - 1; the next needs this item's products)
             if (n > 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_read, (n - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
