@@ -81,6 +81,9 @@ struct Cfg {
     static constexpr int NWG = SMALL || (PAIR && HD == 128 && MODE == FORWARD) ? 1 : 2;
     static constexpr bool ROW_TMEM = !PAIR && (MODE == GRAD_Q || (MODE == FORWARD && HD == 128));
     static constexpr int NBUF = MODE != FORWARD ? NWG : PAIR || HD == 64 ? 2 : ROW_TMEM ? 3 : 4;  // score buffers
+    // gradients whose weights all lie over T2: T1 of the buffer's next block need not wait for the products that
+    // read them
+    static constexpr bool EARLY = GRAD && !(PAIR && MODE == GRAD_KV);
     static constexpr int SOFTMAX = 3;                       // first softmax warp
     static constexpr int THREADS = 32 * SOFTMAX + 128 * NWG, PER_SM = SMALL ? 2 : 1;
     static constexpr int RTILE = ROWS * HD * 2 * PARTS, CTILE = COLS * HD * 2 * PARTS;  // bytes
@@ -495,35 +498,46 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     fence_async_smem();
                     __syncwarp();
                 }
-                // T of block g overwrites the weights of block g - NBUF, which its second products have read
-                // (phase g / NBUF - 1; the next needs this T)
+                const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
+                const uint32_t t = tmem + (g % NBUF) * C::TBUF;
+                // T1 (i = 0) or T2.  Pairs: l h + h l + h h, the small products first (the accumulator truncates);
+                // the dropped l l is 2^-22 of the product
+                auto product = [&](int i) {
+#pragma unroll
+                    for (int c = 0; c < (PAIR ? 3 : 1); c++)
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; kk++) {
+                            const uint32_t ro = (i ? r2 : r1) + (PAIR && c == 0 ? RPART : 0) + (kk / 4) * 2 * BOX + (kk % 4) * 32;
+                            const uint32_t co = b + i * C::CTILE + (PAIR && c == 1 ? CPART : 0) + (kk / 4) * BOX + (kk % 4) * 32;
+                            const uint32_t desc = i == 0 && args.negate ? t_neg : t_desc;
+                            if constexpr (C::ROW_TMEM)
+                                umma_f16_ts(t + 64 * i, tmem + C::ROWT + i * HD / 2 + kk * 8, desc_k_sw128(co), desc, kk + c != 0);
+                            else
+                                umma_f16(t + 64 * i, desc_k_sw128(ro), desc_k_sw128(co), desc, kk + c != 0);
+                        }
+                };
+                // T1 overwrites scores of block g - NBUF that the softmax has read once its weights are written
+                // (p_full, phase g / NBUF - 1; the next needs this T)
+                if (C::EARLY && g >= NBUF) {
+                    ok = __all_sync(0xffffffffu,
+                                    mbar_wait(&p_full[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                    if (!ok) break;
+                }
+                if (C::EARLY) {
+                    tc_fence_after();
+                    if (elect_one()) product(0);
+                    __syncwarp();
+                }
+                // What is left overwrites the weights, which its second products have read (phase g / NBUF - 1 of
+                // their barrier; the next needs this T)
                 if (g >= NBUF)
                     ok = __all_sync(0xffffffffu,
                                     mbar_wait(&acc_done[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t r1 = smem_u32(rows1), r2 = smem_u32(rows2), b = smem_u32(st);
-                    const uint32_t t = tmem + (g % NBUF) * C::TBUF;
-                    // pairs: l h + h l + h h, the small products first (the accumulator truncates); the
-                    // dropped l l is 2^-22 of the product
-#pragma unroll
-                    for (int i = 0; i < (C::GRAD ? 2 : 1); i++)
-#pragma unroll
-                        for (int c = 0; c < (PAIR ? 3 : 1); c++)
-#pragma unroll
-                            for (int kk = 0; kk < HD / 16; kk++) {
-                                const uint32_t ro = (i ? r2 : r1) + (PAIR && c == 0 ? RPART : 0) + (kk / 4) * 2 * BOX +
-                                                    (kk % 4) * 32;
-                                const uint32_t co = b + i * C::CTILE + (PAIR && c == 1 ? CPART : 0) + (kk / 4) * BOX +
-                                                    (kk % 4) * 32;
-                                const uint32_t desc = i == 0 && args.negate ? t_neg : t_desc;
-                                if constexpr (C::ROW_TMEM)
-                                    umma_f16_ts(t + 64 * i, tmem + C::ROWT + i * HD / 2 + kk * 8, desc_k_sw128(co), desc,
-                                                kk + c != 0);
-                                else
-                                    umma_f16(t + 64 * i, desc_k_sw128(ro), desc_k_sw128(co), desc, kk + c != 0);
-                            }
+                    if (!C::EARLY) product(0);
+                    if (C::GRAD) product(1);
                     umma_commit(&t_full[g % NBUF]);
                 }
                 __syncwarp();
@@ -534,8 +548,8 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
     } else if (warp == 2) {
         // ---- second products: P v (forward); dS k, or dS^T q and P^T dout
         constexpr uint32_t acc_desc = idesc<T>(HD, true);
-        // where the weights of columns 16 kk.. are; a pair's h and l are side by side
-        auto weight_col = [](int kk) { return PAIR ? 16 * kk : 8 * kk; };
+        // where the weights of columns 16 kk.. are; a pair's h and l, or dkv's dS and P, are side by side
+        auto weight_col = [](int kk) { return PAIR || MODE == GRAD_KV ? 16 * kk : 8 * kk; };
         bool ok = true;
         Item it;
         int added[2] = {0, 0};  // pairs: sums of each accumulator taken so far
@@ -574,7 +588,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                                             kk + c != 0 || !first);
                     };
                     second(acc, t + (C::GRAD ? 64 : 0), b + (MODE == FORWARD ? C::CTILE : 0));
-                    if (MODE == GRAD_KV) second(acc + HD, t, b + C::CTILE);
+                    if (MODE == GRAD_KV) second(acc + HD, PAIR ? t : t + 64 + 8, b + C::CTILE);
                     umma_commit(&acc_done[g % NBUF]);
                     umma_commit(&c_empty[g % NST]);
                     if (gi == it.nblk - 1) umma_commit(all_done);
@@ -816,17 +830,28 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     }
                     auto weights = [&](auto masked) {
                         constexpr int CH = 16;  // columns in registers at a time
+                        // dkv: the statistics (-lse log2 e, -D) that are read before the wait for the scores, as many
+                        // as registers hold.  2 x 4096 rows, 16 heads of 128: gradient 904 us with both, 914 with none;
+                        // of 64 with both 677, with one 682, with none 700, but both spill there and fp16 takes
+                        // 154 us for 64 windows of 384 rows, 151 with one or none.
+                        constexpr int AHEAD = MODE != GRAD_KV || PAIR ? 0 : C::SMALL ? 1 : 2;
 #pragma unroll
                         for (int h = 0; h < COLS; h += CH) {  // the weights go over scores that are read already
                             float s[CH], u[CH];
+                            float4 sl[CH / 4], sd[CH / 4];
+#pragma unroll
+                            for (int c = 0; c < CH / 4; c++) {
+                                if (AHEAD > 0) sl[c] = st[h / 4 + c];
+                                if (AHEAD > 1) sd[c] = st[16 + h / 4 + c];
+                            }
                             tmem_ld_pair(t + h, t + 64 + h, s, u);
-                            uint32_t pw[CH / 2 * PARTS], dw[CH / 2 * PARTS];  // pairs: h, then l
+                            uint32_t w[CH * PARTS], *dw = w, *pw = w + CH / 2 * PARTS;  // pairs: h, then l
 #pragma unroll
                             for (int c = 0; c < CH; c += 4) {
                                 float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
                                 if (MODE == GRAD_KV) {
-                                    nl = st[(h + c) / 4];
-                                    nd = st[16 + (h + c) / 4];
+                                    nl = AHEAD > 0 ? sl[c / 4] : st[(h + c) / 4];
+                                    nd = AHEAD > 1 ? sd[c / 4] : st[16 + (h + c) / 4];
                                 }
 #pragma unroll
                                 for (int e = 0; e < 4; e += 2) {
@@ -856,8 +881,12 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                                     }
                                 }
                             }
-                            if (MODE == GRAD_KV) tmem_st<CH / 2 * PARTS>(t + h / 2 * PARTS, pw);
-                            tmem_st<CH / 2 * PARTS>(t + 64 + h / 2 * PARTS, dw);
+                            if constexpr (MODE == GRAD_KV && !PAIR) {
+                                tmem_st16(t + 64 + h, w);  // both over T2
+                            } else {
+                                if (MODE == GRAD_KV) tmem_st<CH / 2 * PARTS>(t + h / 2 * PARTS, pw);
+                                tmem_st<CH / 2 * PARTS>(t + 64 + h / 2 * PARTS, dw);
+                            }
                         }
                     };
                     if (full)
