@@ -246,6 +246,13 @@ __device__ __forceinline__ float pair_ds_scale(float norm, float v_max) {
     return 0.5f * split_scale_of(norm * v_max * (HD == 64 ? 8.0f : 11.3137085f));
 }
 
+// Both waits, tested one behind the other before either's result is used: a wait that passes at once costs the issuing
+// warps 110 - 170 clocks, which two in a row would pay twice for every block.
+__device__ __forceinline__ bool wait_both(uint64_t* a, uint32_t phase_a, uint64_t* b, uint32_t phase_b, int* err) {
+    const bool pa = mbar_try_wait(a, phase_a), pb = mbar_try_wait(b, phase_b);
+    return (pa || mbar_wait(a, phase_a, err, DEV_TIMEOUT_ATTN_TRAIN)) && (pb || mbar_wait(b, phase_b, err, DEV_TIMEOUT_ATTN_TRAIN));
+}
+
 struct TcMaps {
     CUtensorMap q, k, v, dout;       // loads, 64-row boxes
     CUtensorMap out, dq, dk, dv;     // stores, 32-row boxes
@@ -487,8 +494,15 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             }
             for (int gi = 0; ok && gi < it.nblk; gi++) {
                 const int g = gt + gi;
-                // the column tiles of block g (phase g / NST; the next needs this block's second product)
-                ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                // The column tiles of block g (phase g / NST; the next needs this block's second product), and the
+                // score buffer.  T overwrites the weights of block g - NBUF, which its second products have read
+                // (acc_done, phase g / NBUF - 1; the next needs this T).  EARLY: T1 overwrites scores that the softmax
+                // has read once its weights are written (p_full, the same phase), and only T2 waits for the products.
+                uint64_t* c_bar = &c_full[g % NST];
+                uint64_t* t_bar = C::EARLY ? &p_full[g % NBUF] : &acc_done[g % NBUF];
+                const uint32_t c_phase = (g / NST) & 1, t_phase = (g / NBUF - 1) & 1;
+                ok = __all_sync(0xffffffffu, g >= NBUF ? wait_both(c_bar, c_phase, t_bar, t_phase, err)
+                                                       : mbar_wait(c_bar, c_phase, err, DEV_TIMEOUT_ATTN_TRAIN));
                 if (!ok) break;
                 uint8_t* st = ring + (g % NST) * C::STAGE;
                 const int c0 = col0(it, gi);
@@ -516,24 +530,14 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                                 umma_f16(t + 64 * i, desc_k_sw128(ro), desc_k_sw128(co), desc, kk + c != 0);
                         }
                 };
-                // T1 overwrites scores of block g - NBUF that the softmax has read once its weights are written
-                // (p_full, phase g / NBUF - 1; the next needs this T)
-                if (C::EARLY && g >= NBUF) {
-                    ok = __all_sync(0xffffffffu,
-                                    mbar_wait(&p_full[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-                    if (!ok) break;
-                }
                 if (C::EARLY) {
                     tc_fence_after();
                     if (elect_one()) product(0);
                     __syncwarp();
+                    if (g >= NBUF)
+                        ok = __all_sync(0xffffffffu, mbar_wait(&acc_done[g % NBUF], t_phase, err, DEV_TIMEOUT_ATTN_TRAIN));
+                    if (!ok) break;
                 }
-                // What is left overwrites the weights, which its second products have read (phase g / NBUF - 1 of
-                // their barrier; the next needs this T)
-                if (g >= NBUF)
-                    ok = __all_sync(0xffffffffu,
-                                    mbar_wait(&acc_done[g % NBUF], (g / NBUF - 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
-                if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
                     if (!C::EARLY) product(0);
@@ -561,8 +565,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 const int g = gt + gi;
                 // the column tiles (as above) and the weights of block g (phase g / NBUF; the next needs T of
                 // block g + NBUF, hence this product)
-                ok = __all_sync(0xffffffffu, mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN) &&
-                                                 mbar_wait(&p_full[g % NBUF], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                ok = __all_sync(0xffffffffu, wait_both(&c_full[g % NST], (g / NST) & 1, &p_full[g % NBUF], (g / NBUF) & 1, err));
                 // which accumulator, and the block's number there: a pair's starts afresh every second one,
                 // once the softmax group has added it up (the next addition needs this product)
                 const int which = MODE == FORWARD ? g % NWG : 0, m = MODE == FORWARD ? gi / NWG : gi;
