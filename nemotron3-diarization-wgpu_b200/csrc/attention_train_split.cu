@@ -8,8 +8,8 @@
 //
 // Bound: latency (four lines of a thread are in flight) before memory: two reads of each
 // operand and one write of the same size.  Measured on a B200, cold: q, k and v of 8 x 501 rows,
-// 8 heads of 64 (25 MB) 12 us for the magnitudes and 14 us for the split; with dout and the
-// statistics 14 and 21 us.
+// 8 heads of 64 (25 MB) 13 us for the magnitudes and 16 us for the split; with dout and the
+// statistics 16 and 22 us.
 
 #include <cuda_fp16.h>
 

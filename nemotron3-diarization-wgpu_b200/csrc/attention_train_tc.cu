@@ -5,18 +5,20 @@
 //   dq       rows = queries, columns = keys:  T1 = q k^T, T2 = dout v^T;   dq += dS k
 //   dkv      rows = keys, columns = queries:  T1 = k q^T, T2 = v dout^T;   dk += dS^T q, dv += P^T dout
 //
-// A block owns 128 rows (TMEM lanes, one softmax thread each) and walks blocks of 64
-// columns.  Both operands of T1 and T2 are K-major tiles in shared memory; the weights (P,
-// dS) go back to TMEM as the 16-bit A operand of the second product, over the scores they
-// came from, and its B operand is the same column tile read with the token index as K
-// (MN-major), so no tile is stored twice or transposed.  Nothing of size rows x columns
-// leaves the SM.
-//   warp 0      TMA: the row tiles once, the column tiles through a ring of stages
-//   warp 1      TMEM owner; issues T of block g once the second products of block g - NBUF, which read
-//               the weights in the same columns, have completed
-//   warp 2      issues the second products (with both kinds on one thread, which issues an MMA of 64
-//               columns every ~55 clocks, that thread was the bottleneck; a thread for each of the
-//               four products of dkv gains nothing more: the MMAs then wait for one another)
+// A block works on items of 128 rows of a head (TMEM lanes, one softmax thread each) and walks
+// blocks of 64 columns.  When an item's loads are under way it takes the next one over from
+// the grid by cluster launch control, so that launch, set-up and epilogue overlap (windows of
+// 384 rows: forward 97 us with a block per item, 75 so).  The column tiles are K-major
+// operands of T1 and T2 in shared memory; the weights (P, dS) go back to TMEM as the 16-bit
+// A operand of the second product, over scores that are read, and its B operand is the same
+// column tile read with the token index as K (MN-major), so no tile is stored twice or
+// transposed.  The row tiles are T's A operands: in TMEM where they fit and pay (ROW_TMEM),
+// else in shared memory.  Nothing of size rows x columns leaves the SM.
+//   warp 0      items; TMA: the row tiles, the column tiles through a ring of stages
+//   warp 1      TMEM owner; issues T of block g once its score buffer is free (see EARLY)
+//   warp 2      issues the second products (with both kinds on one thread the gradient of 2 x 4096 rows,
+//               16 heads of 128, took 1092 us against 946; a thread for each of the four products of
+//               dkv gains nothing more)
 //   warps 3..   softmax groups of 4 warps, one thread per row; NWG column blocks are in work at a time
 // head_dim 64: one group and two blocks per SM, which interleave (256 TMEM columns each);
 // head_dim 128: one block per SM with two groups on alternating column blocks (forward:
@@ -39,12 +41,14 @@
 // of each first, and is then added to a sum that is rounded to nearest (more TMEM, or the
 // output tensor).
 //
-// Bound: the MMAs of T at head_dim 128 (75 clocks each instead of 32: N = 64 with both operands
-// in shared memory; tensor pipe 37 - 48 % busy), at head_dim 64 the chain from T over the
-// softmax to the second product, two blocks of which interleave on an SM.  Measured on a B200:
-// 128 windows of 384 rows, 8 heads of 64, bf16, forward 75 us and gradient 268 us (515 and 505
-// executed TFLOP/s); 2 x 4096 rows, 16 heads of 128, 312 and 958 us (880 and 1000); the same
-// causal with 4 key heads 175 and 548 us.
+// Bound, from clock stamps in every role: at head_dim 128 in forward and dq the thread that
+// issues T, whose block of 8 or 16 MMAs takes 300 - 570 clocks and each wait, passed at once,
+// another 110 - 170 (tensor pipe 46 - 48 % busy); in dkv the chain of a score buffer, softmax 1500 -
+// 1800, second products 500 - 800, T2 450.  At head_dim 64 the softmax threads: in forward they work
+// without a pause, in the gradients they wait for T (750 of 1850 clocks in dq, 850 of 2900 in dkv) while
+// the SM's other block computes.  Measured on a B200: 128 windows of 384 rows, 8 heads of 64, bf16,
+// forward 74 us and gradient 253 us (520 and 535 executed TFLOP/s); 2 x 4096 rows, 16 heads of 128, 255
+// and 873 us (1080 and 1100); the same causal with 4 key heads 136 and 497 us.
 //
 // Rows past a sequence's length: TMA fills what lies past the tensor with zeros, and the
 // T warp overwrites what lies past the length with zeros before a tile is used, so
@@ -79,8 +83,12 @@ struct Cfg {
     static constexpr bool PAIR = PARTS == 2;
     // column blocks in softmax at a time (an fp32 forward pass of head_dim 128 has TMEM for one)
     static constexpr int NWG = SMALL || (PAIR && HD == 128 && MODE == FORWARD) ? 1 : 2;
+    // Row tiles as TMEM operands.  2 x 4096 rows, 16 heads of 128, us with and without: forward 265 and 272, gradient
+    // (dq) 931 and 959; 128 windows of 384 rows, 8 heads of 64: gradient 262 and 268, but forward 78.7 and
+    // 75.7 (the copy is on the path of every item of six blocks).  dkv's accumulators leave no room, nor do pairs.
     static constexpr bool ROW_TMEM = !PAIR && (MODE == GRAD_Q || (MODE == FORWARD && HD == 128));
-    static constexpr int NBUF = MODE != FORWARD ? NWG : PAIR || HD == 64 ? 2 : ROW_TMEM ? 3 : 4;  // score buffers
+    // score buffers: as many as TMEM holds (forward of 128: a third took 312 us to 265, with the row tiles' move)
+    static constexpr int NBUF = MODE != FORWARD ? NWG : ROW_TMEM ? 3 : 2;
     // gradients whose weights all lie over T2: T1 of the buffer's next block need not wait for the products that
     // read them
     static constexpr bool EARLY = GRAD && !(PAIR && MODE == GRAD_KV);
@@ -1189,9 +1197,9 @@ bool attention_tc_fits(const AttnArgs& a, int dtype, bool backward) {
 }
 
 // The split's two launches and its blocks of one per SM cost more than they save where all of a head is
-// one tile of the fp32 units: forward, 32 sequences x 8 heads of 64 rows take 35 us against 18 there, 128 of
-// 32 rows 91 against 52; 8 of 128 rows 21 against 20, 8 of 256 rows 31 against 49.  The gradient is at
-// least even everywhere (1 x 64 rows 21 us against 41, 128 x 32 rows 188 against 174).
+// one tile of the fp32 units: forward, 32 sequences x 8 heads of 64 x 64 rows take 27 us against 18 there, 128 of
+// 32 rows 65 against 52; 8 of 128 rows 18 against 20, 8 of 256 rows 25 against 49.  The gradient pays
+// everywhere (1 x 16 rows 28 us against 30, 128 x 32 rows 116 against 175, 8 x 256 rows 43 against 155).
 bool attention_split_pays(size_t q_rows, size_t k_rows, bool backward) {
     return q_rows > 0 && k_rows > 0 && (backward || q_rows > 64 || k_rows > 64);
 }

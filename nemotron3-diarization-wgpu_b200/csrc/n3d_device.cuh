@@ -19,6 +19,7 @@ enum DevError : int {
     DEV_BAD_SHAPE = 4,
     // 5: the attention kernel's waits (attention_tc.cu)
     DEV_TIMEOUT_PROBE = 6,  // the wait self-test (n3d_selftest_wait_timeout)
+    // 7: the waits of attention with its gradient (attention_train_tc.cu)
 };
 
 // ~2 s of wall time, far above any legitimate wait in these kernels.

@@ -14,17 +14,17 @@
 // Bound: memory (r, dr, block, dy read once, dx, dblock written once); what costs time is
 // the latency of two or three sums over each row, so that many rows must be in work.  A row
 // has one thread for every 8 columns (16 beyond 4096), and a slot of threads takes a
-// contiguous range of rows, two at a time: their sums share the barriers, and the weights
+// contiguous range of rows, two at a time (one beyond 4096): their sums share the barriers, and the weights
 // are read and the column sums (weights, biases, gate; in shared memory, where each thread
 // alone adds to its columns) updated once for both.  One row at a time with the column sums
-// in registers, up to 40 a thread, took 176 us for 8191 x 4096 in bf16; two take 123.  Slots of
+// in registers, up to 40 a thread, took 176 us for 8191 x 4096 in bf16; two take 124.  Slots of
 // a block are added at the end, blocks by a second kernel, in a fixed order.  A gate row's
 // gradient is complete when its rows lie in one slot; at the borders of slots partial sums
 // go to the workspace and the second kernel adds them.
 //
-// Measured on a B200: 48128 x 512, fp32 stream and bf16 blocks, LayerNorms and a gate 110 us
-// (4.0 TB/s); fp32 throughout without a gate 103 us (5.7 TB/s); 8191 x 4096 in bf16, RMS norms
-// and gates 123 us (3.3 TB/s; one row's 512 threads and their barriers fill an SM).
+// Measured on a B200: 48128 x 512, fp32 stream and bf16 blocks, LayerNorms and a gate 111 us
+// (4.0 TB/s); fp32 throughout without a gate 104 us (5.7 TB/s); 8191 x 4096 in bf16, RMS norms
+// and gates 124 us (3.2 TB/s; the registers of 512 threads, one pair of rows, fill an SM).
 
 #include <algorithm>
 #include <climits>
