@@ -163,14 +163,15 @@ def lengths(b, n, seed):
 
 
 def run(b, nq, nk, hq, hk, hd, dtype, left=-1, right=-1, off=0, ragged=False, layout="rows", scale=0.0, seed=0, std=1.0,
-        do_std=0.1, check=True):
+        do_std=0.1, v_std=1.0, check=True):
     """Forward and backward on the GPU, checked against 64 bits; returns the outputs."""
     import torch
 
     dt = getattr(torch, dtype)
     g = torch.Generator().manual_seed(seed)
     rnd = lambda n, h: torch.randn(b, n, h, hd, generator=g).to(dt)
-    host = [(rnd(nq, hq) * std).to(dt), (rnd(nk, hk) * std).to(dt), rnd(nk, hk), (rnd(nq, hq) * do_std).to(dt)]
+    host = [(rnd(nq, hq) * std).to(dt), (rnd(nk, hk) * std).to(dt), (rnd(nk, hk) * v_std).to(dt),
+            (rnd(nq, hq) * do_std).to(dt)]
     ql, kl = (lengths(b, nq, seed + 1), lengths(b, nk, seed + 2)) if ragged else ([nq] * b, [nk] * b)
     if ragged:  # what stands past the lengths is never read
         for s in range(b):
@@ -263,6 +264,14 @@ def test_peaked_and_flat_rows_and_small_gradients(dtype):
     run(1, 130, 200, 1, 1, 64, dtype, scale=1e-3, seed=9)              # all keys alike
     run(1, 130, 200, 1, 1, 64, dtype, scale=-0.2, seed=10)             # a negative scale
     run(1, 130, 200, 1, 1, 128, dtype, do_std=2e-3, seed=11)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,v_std", [(64, 380.0), (128, 260.0)])
+def test_large_values(dtype, hd, v_std):
+    # rows of v of norms about 3000, inside the 4096 that fp16 gradients are held to; outputs stay far from its largest
+    run(1, 130, 200, 2, 1, hd, dtype, -1, 0, 70, do_std=0.02, v_std=v_std, seed=15)
 
 
 @pytest.mark.gpu
