@@ -106,6 +106,11 @@ __global__ void __launch_bounds__(GradCfg<TPR, EPT>::THREADS, GradCfg<TPR, EPT>:
             }
         };
 
+        // With an RMS norm (or none) before and none behind, only the second sum below is taken.  A sum's words may be
+        // written again only past another barrier of the row, so that sum then takes its own words and those of
+        // the first one in turn.
+        const bool alone = a.pre != N3D_NORM_LAYER && !post;
+        bool turn = false;
         long long row = begin;
         while (row < end) {
             if (row == gate_end) {
@@ -183,7 +188,8 @@ __global__ void __launch_bounds__(GradCfg<TPR, EPT>::THREADS, GradCfg<TPR, EPT>:
                             s2[3 * q + 1] += b[q][i] * b[q][i];
                             s2[3 * q + 2] += g[q][i] * h[q][i];
                         }
-            row_sums<TPR>(s2, sums[local][3 * R], local);
+            row_sums<TPR>(s2, sums[local][turn ? 0 : 3 * R], local);
+            turn = alone && !turn;
             float rstd_b[R], s3[2 * R] = {};
             const float* gate = a.rows_per_gate ? a.gate + gate_row * C : nullptr;
 #pragma unroll
