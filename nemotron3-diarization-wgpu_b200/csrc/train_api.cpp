@@ -137,6 +137,13 @@ n3d::ResidualArgs residual_args(const n3d_residual_config& cfg) {
     a.rows_per_gate = (long long)std::min(cfg.rows_per_gate, std::max<size_t>(cfg.rows, 1));
     return a;
 }
+// The weights that the configuration uses; the others are not read, whatever the caller passed.
+void set_weights(n3d::ResidualArgs& a, const float* post_w, const float* post_b, const float* gate, const float* pre_w,
+                 const float* pre_b) {
+    if (a.post != N3D_NORM_NONE) a.post_w = post_w, a.post_b = post_b;
+    if (a.pre != N3D_NORM_NONE) a.pre_w = pre_w, a.pre_b = pre_b;
+    if (a.rows_per_gate) a.gate = gate;
+}
 struct ResidualWorkspace {
     size_t sums, gate_parts;  // floats
 };
@@ -311,15 +318,14 @@ n3d_status n3d_residual_norm(int device, const n3d_residual_config* cfg, const n
         check_in_place(*r, *x, cfg->rows, "n3d_residual_norm: in place, r and x must have the same stride");
         if (pre) check_in_place(*y, *block, cfg->rows, "n3d_residual_norm: in place, y and block must have the same stride");
         n3d::ResidualArgs a = residual_args(*cfg);
-        a.post_w = d_post_w, a.post_b = d_post_b, a.pre_w = d_pre_w, a.pre_b = d_pre_b;
-        a.gate = d_gate;
+        set_weights(a, d_post_w, d_post_b, d_gate, d_pre_w, d_pre_b);
         a.x = x->d_data, a.ld_x = x->row_stride;
         a.block = block->d_data, a.ld_block = block->row_stride;
         a.r_out = r->d_data, a.ld_r_out = r->row_stride;
         if (pre) a.y = y->d_data, a.ld_y = y->row_stride;
         a.wide = cfg->cols % 4 == 0 && wide_rows(x, cfg->residual_dtype) && wide_rows(r, cfg->residual_dtype) &&
                  wide_rows(block, cfg->block_dtype) && wide_rows(pre ? y : nullptr, cfg->block_dtype) &&
-                 wide_weights({d_post_w, d_post_b, d_gate, d_pre_w, d_pre_b});
+                 wide_weights({a.post_w, a.post_b, a.gate, a.pre_w, a.pre_b});
         if (cfg->rows == 0) return;
         DeviceGuard g(device);
         check_record(train_error(device));
@@ -371,8 +377,7 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config* cfg, co
             return;
         }
         n3d::ResidualArgs a = residual_args(*cfg);
-        a.post_w = d_post_w, a.post_b = d_post_b, a.pre_w = d_pre_w;
-        a.gate = d_gate;
+        set_weights(a, d_post_w, d_post_b, d_gate, d_pre_w, nullptr);
         a.block = block->d_data, a.ld_block = block->row_stride;
         if (pre) a.r = r->d_data, a.ld_r = r->row_stride, a.dy = dy->d_data, a.ld_dy = dy->row_stride;
         if (dr) a.dr = dr->d_data, a.ld_dr = dr->row_stride;
@@ -383,7 +388,7 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config* cfg, co
         a.gate_parts = a.sums + w.sums;
         a.wide = cols % 4 == 0 && wide_rows(block, bt) && wide_rows(dx, rt) && wide_rows(dblock, bt) &&
                  wide_rows(pre ? r : nullptr, rt) && wide_rows(pre ? dy : nullptr, bt) && wide_rows(dr, rt) &&
-                 wide_weights({d_post_w, d_post_b, d_gate, d_pre_w, d_dgate});
+                 wide_weights({a.post_w, a.post_b, a.gate, a.pre_w, d_dgate});
         a.slots = n3d::residual_split(a.rows, a.cols, a.wide).slots;
         n3d::launch_residual_norm_grad((cudaStream_t)stream, a, rt, bt);
     });

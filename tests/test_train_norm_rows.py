@@ -106,3 +106,28 @@ def test_forward_of_the_plain_pairs(rows, cols, rt, bt, post, pre):
     if pre != "none":
         h, s = hat64(r64, pre)
         close(y, y64, row(p["pre_w"][None]) * mag / s * (1 + row(h) ** 2) + row(p["pre_b"][None]), 150, bt, "y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [512, 7])
+@pytest.mark.parametrize("post,pre", [("none", "rms"), ("none", "layer"), ("rms", "none"), ("layer", "none"), ("none", "none")])
+def test_weights_of_a_norm_that_is_not_used_are_not_read(cols, post, pre):
+    import torch
+
+    t, _ = make(37, cols, "float32", "bfloat16", 0, cols)
+    d = {n: v.cuda() for n, v in t.items()}
+    bad = torch.full((cols,), math.nan, device="cuda")
+    used = {n: d[n] for k, p in ((post, "post"), (pre, "pre")) if k != "none" for n in (p + "_w", p + "_b")}
+    unused = {n: bad for k, p in ((post, "post"), (pre, "pre")) if k == "none" for n in (p + "_w", p + "_b")}
+    space = torch.empty(n3d.residual_norm_workspace(37, cols), dtype=torch.uint8, device="cuda")
+    with_pre = pre != "none"
+    got = []
+    for extra in ({}, unused):
+        kw = dict(post=post, pre=pre, **used, **extra)
+        r, y, dx, db = (torch.full_like(d[n], math.nan) for n in ("x", "block", "x", "block"))
+        n3d.residual_norm(d["x"], d["block"], r, y if with_pre else None, **kw)
+        n3d.residual_norm_grad(d["block"], d["r"] if with_pre else None, d["dy"] if with_pre else None, d["dr"], dx, db,
+                               workspace=space, **kw)
+        got.append([r, dx, db] + [y] * with_pre)
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and not a.isnan().any()
