@@ -623,7 +623,9 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             s_v = split_scale_of(v_max);
             if (C::GRAD) s_do = split_scale_of(args.maxima[3]);
         }
-        const float k2 = PAIR ? args.k2 / s_q / s_k : args.k2;
+        // Held normal: with tiny q and k the quotient would be 0, and 0 times the -inf of a masked score NaN.  (Raw
+        // scores stay below 2^37, so such scores are 0 next to 1 either way.)
+        const float k2 = PAIR ? fmaxf(args.k2 / s_q / s_k, 1.17549435e-38f) : args.k2;
         const float dp_unit = PAIR ? 1.0f / s_do / s_v : 1.0f;  // T2 times this is dP
         constexpr float P_LOG2 = !F16 ? 0.0f : MODE == FORWARD ? 7.0f : MODE == GRAD_KV ? (PAIR ? 15.0f : 10.0f) : 0.0f;
         constexpr float P_SCALE = PAIR ? 32768.0f : 1024.0f;  // 2^P_LOG2 of dkv
