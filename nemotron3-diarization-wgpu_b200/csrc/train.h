@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cstdint>
 
 #include "../../include/n3d.h"
@@ -72,7 +73,8 @@ struct AttnArgs {
     int left, right, offset;      // kNoLimit where unlimited
     const int32_t *q_len, *k_len;  // null: all rows
 };
-constexpr int kNoLimit = 1 << 30;
+constexpr int kNoLimit = INT_MAX;
+constexpr int kMaxReach = 1 << 30;  // of left, right and offset: their sums stay inside 32 bits where that matters
 
 // The rows of one sequence and which keys a query row sees.
 struct AttnMask {

@@ -167,8 +167,8 @@ void check_attn(const n3d_attn_config* cfg) {
     arg_check(cfg->seqs <= (size_t)INT_MAX && cfg->q_rows <= (size_t)1 << 30 && cfg->k_rows <= (size_t)1 << 30,
               "attention: seqs beyond 2^31 or rows beyond 2^30");
     arg_check(std::isfinite(cfg->scale), "attention: scale is not finite");
-    arg_check(cfg->left <= n3d::kNoLimit && cfg->right <= n3d::kNoLimit && cfg->q_offset <= n3d::kNoLimit &&
-                  cfg->q_offset >= -n3d::kNoLimit,
+    arg_check(cfg->left <= n3d::kMaxReach && cfg->right <= n3d::kMaxReach && cfg->q_offset <= n3d::kMaxReach &&
+                  cfg->q_offset >= -n3d::kMaxReach,
               "attention: left, right or q_offset beyond 2^30");
 }
 // The tensors every attention call has; fills their views.
