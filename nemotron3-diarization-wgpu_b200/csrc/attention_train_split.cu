@@ -1,15 +1,17 @@
-// fp32 operands of the training attention for the tensor cores: the largest magnitude of
-// q, k, v (and dout), then each as two fp16 arrays of x s (h = x s rounded to 11 bits, l the
-// rest; s the power of two that brings the largest magnitude to at most 2^15), as the
-// library's other fp32 products (n3d_device.cuh).  Rows past the lengths become zeros.
+// fp32 operands of the training attention for the tensor cores: each row of q, k, v (and dout) as
+// two fp16 arrays of x s (h = x s rounded to 11 bits, l the rest), as the library's other fp32
+// products (n3d_device.cuh), with a power of two s for every row: the one that brings its largest
+// magnitude into [2^14, 2^15).  The main kernel takes the rows' units 1 / s where it has a row or
+// a column of scores in hand.  (One s for a whole tensor would leave a row 2^-20 the size of the
+// largest with 20 bits, one of 2^-40 with none, and let a sequence's result depend on what else is in
+// the batch.)  Rows past the lengths become zeros.
 //
-// For the gradient the same pass takes, per query row, -lse log2 e, -D = -(dout . out) and
-// |dout row|, in fp32 from the unsplit tensors, and the largest |dout row| of each head.
+// For the gradient the same pass takes, per query row, -lse log2 e and -D = -(dout . out), in
+// fp32 from the unsplit tensors.
 //
-// Bound: latency (four lines of a thread are in flight) before memory: two reads of each
+// Bound: latency (four lines of a thread are in flight) before memory: one read of each
 // operand and one write of the same size.  Measured on a B200, cold: q, k and v of 8 x 501 rows,
-// 8 heads of 64 (25 MB) 13 us for the magnitudes and 16 us for the split; with dout and the
-// statistics 16 and 22 us.
+// 8 heads of 64 (25 MB) 18 us, with dout and the statistics 24; of 2 x 4096 rows, 16 heads (101 MB) 60 and 88.
 
 #include <cuda_fp16.h>
 
@@ -24,7 +26,8 @@ namespace n3d {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int ILP = 4;  // lines of a thread in flight
+constexpr int ILP = 4;       // lines of a thread in flight
+constexpr int BLOCKS = 296;  // at most, of each operand
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Operand {
@@ -41,8 +44,8 @@ struct SplitArgs {
     int o_wide;
     const float* lse;
     AttnSplitSpace sp;
-    int heads_total;  // seqs * q_heads
-    int q_tiles, backward;
+    int q_tiles, k_tiles;  // blocks of 128 query rows, of 64 key rows
+    int backward;
 };
 
 // Line i of an operand: sequence * heads + head, sequence, row; whether the row is inside its length.
@@ -64,77 +67,22 @@ __device__ __forceinline__ float4 line_load(const HeadsView& t, const Line& l, i
     return wide ? *reinterpret_cast<const float4*>(x) : make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// blockIdx.y: the operand.  HD / 4 threads a line, ILP lines a thread.  Infinities and NaN
-// do not count: they make their own products NaN whatever the scale.
-template <int HD>
-__global__ void __launch_bounds__(THREADS) attention_absmax_kernel(const __grid_constant__ SplitArgs a) {
-    constexpr int TPL = HD / 4, LINES = THREADS / TPL;
-    __shared__ float part[THREADS / 32];
-    griddep_wait();
-    griddep_launch_dependents();
-    const Operand& p = a.op[blockIdx.y];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x % TPL * 4;
-    if (a.backward && blockIdx.y == 3)
-        for (int i = blockIdx.x * THREADS + threadIdx.x; i < a.heads_total; i += gridDim.x * THREADS)
-            a.sp.head_norm[i] = 0.0f;
-    float m = 0.0f;
-    for (long long first = (long long)blockIdx.x * LINES * ILP; first < p.lines; first += (long long)gridDim.x * LINES * ILP) {
-        float4 v[ILP];
-#pragma unroll
-        for (int j = 0; j < ILP; j++) {
-            v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const long long i = first + j * LINES + threadIdx.x / TPL;
-            if (i < p.lines) {
-                const Line l = line_of(p, (int)i);
-                if (l.live) v[j] = line_load(p.t, l, p.heads, c, p.wide);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < ILP; j++) {
-            const float x[4] = {fabsf(v[j].x), fabsf(v[j].y), fabsf(v[j].z), fabsf(v[j].w)};
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (x[e] < INFINITY) m = fmaxf(m, x[e]);
-        }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) part[warp] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < THREADS / 32; i++) m = fmaxf(m, part[i]);
-        a.sp.partial[blockIdx.y * kSplitBlocks + blockIdx.x] = m;
-    }
+// The power of two that brings m into [2^14, 2^15), at most 2^126 so that its inverse is normal too; 1 for m = 0.
+__device__ __forceinline__ float row_scale(float m) {
+    if (!(m > 0.0f)) return 1.0f;
+    return __int_as_float(min(253, 268 - (__float_as_int(m) >> 23)) << 23);
 }
 
+// blockIdx.y: the operand.  HD / 4 threads a line, ILP lines a thread.
 template <int HD>
 __global__ void __launch_bounds__(THREADS) attention_split_kernel(const __grid_constant__ SplitArgs a) {
     constexpr int TPL = HD / 4, LINES = THREADS / TPL;
-    __shared__ float part[THREADS / 32];
     griddep_wait();
     griddep_launch_dependents();
-    const Operand& p = a.op[blockIdx.y];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x % TPL * 4;
-    float m = 0.0f;
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += THREADS) m = fmaxf(m, a.sp.partial[blockIdx.y * kSplitBlocks + i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) part[warp] = m;
-    __syncthreads();
-    m = part[0];
-    for (int i = 1; i < THREADS / 32; i++) m = fmaxf(m, part[i]);
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.sp.maxima[blockIdx.y] = m;
-    const float s = split_scale_of(m);
-    const bool stats = a.backward && blockIdx.y == 3;
-    // the largest |dout row| of the head that this thread is at: a maximum of non-negative floats, the same
-    // in any order
-    int norm_head = 0;
-    float norm = 0.0f;
-    auto keep_norm = [&](int next) {
-        if (norm > 0.0f) atomicMax(reinterpret_cast<int*>(a.sp.head_norm + norm_head), __float_as_int(norm));
-        norm_head = next;
-        norm = 0.0f;
-    };
+    const int which = blockIdx.y;
+    const Operand& p = a.op[which];
+    const bool keys = which == 1 || which == 2, stats = a.backward && which == 3;
+    const int c = threadIdx.x % TPL * 4;
     for (long long first = (long long)blockIdx.x * LINES * ILP; first < p.lines; first += (long long)gridDim.x * LINES * ILP) {
         float4 v[ILP], o[ILP];
         Line l[ILP];
@@ -152,45 +100,42 @@ __global__ void __launch_bounds__(THREADS) attention_split_kernel(const __grid_c
 #pragma unroll
         for (int j = 0; j < ILP; j++) {
             const bool inside = at[j] < p.lines;
-            uint2 h, lo;
             const float x[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-            split2x4(x, s, h, lo);
-            if (inside) {
-                __half* out = p.out + at[j] * HD + c;
-                *reinterpret_cast<uint2*>(out) = h;
-                *reinterpret_cast<uint2*>(out + (long long)p.lines * HD) = lo;
-            }
-            if (stats) {
-                float dot = x[0] * o[j].x + x[1] * o[j].y + x[2] * o[j].z + x[3] * o[j].w;
-                float norm2 = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
+            // the row's largest magnitude; infinities and NaN do not count: their products are NaN whatever the scale
+            float m = 0.0f;
 #pragma unroll
-                for (int k = TPL / 2; k > 0; k >>= 1) {
-                    dot += __shfl_xor_sync(0xffffffffu, dot, k);
-                    norm2 += __shfl_xor_sync(0xffffffffu, norm2, k);
-                }
-                if (inside && c == 0) {
-                    const int row = l[j].row;
-                    float* const tiles = a.sp.stats + (long long)l[j].sh * a.q_tiles * 2 * kSplitStat;
-                    float* st = tiles + row / 64 * kSplitStat + row % 64;
-                    const float lse = l[j].live ? a.lse[(long long)l[j].sh * p.rows + row] : -INFINITY;
-                    st[0] = lse == -INFINITY ? -INFINITY : -lse * LOG2E;
-                    st[64] = -dot;
-                    st[128] = sqrtf(norm2);
-                    if (l[j].sh != norm_head) keep_norm(l[j].sh);
-                    if (norm2 > 0.0f) norm = fmaxf(norm, sqrtf(norm2));
-                    // the rows of the last block of 64 that do not exist belong to it too
-                    if (row == p.rows - 1)
-                        for (int r = p.rows; r % 64 != 0; r++) {
-                            float* e = tiles + r / 64 * kSplitStat + r % 64;
-                            e[0] = -INFINITY;
-                            e[64] = 0.0f;
-                            e[128] = 0.0f;
-                        }
+            for (int e = 0; e < 4; e++)
+                if (fabsf(x[e]) < INFINITY) m = fmaxf(m, fabsf(x[e]));
+            float dot = x[0] * o[j].x + x[1] * o[j].y + x[2] * o[j].z + x[3] * o[j].w;
+#pragma unroll
+            for (int k = TPL / 2; k > 0; k >>= 1) {
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+                if (stats) dot += __shfl_xor_sync(0xffffffffu, dot, k);
+            }
+            const float s = row_scale(m);
+            if (!inside) continue;
+            uint2 h, lo;
+            split2x4(x, s, h, lo);
+            __half* out = p.out + at[j] * HD + c;
+            *reinterpret_cast<uint2*>(out) = h;
+            *reinterpret_cast<uint2*>(out + (long long)p.lines * HD) = lo;
+            if (c != 0) continue;
+            // what the row's block of 64 holds of it; the rows of the last block that do not exist belong to the last row
+            const int row = l[j].row, end = row == p.rows - 1 ? (row / 64 + 1) * 64 : row + 1;
+            float* const blocks = keys ? a.sp.key_stats + (long long)l[j].sh * a.k_tiles * kKeyStat
+                                       : a.sp.stats + (long long)l[j].sh * a.q_tiles * 2 * kSplitStat;
+            float* const st = blocks + row / 64 * (keys ? kKeyStat : kSplitStat) + row % 64;
+            const int unit = keys ? (which - 1) * 64 : which == 0 ? 128 : 192;
+            for (int r = 0; r < end - row; r++) st[unit + r] = r == 0 ? 1.0f / s : 1.0f;
+            if (stats) {
+                const float lse = l[j].live ? a.lse[(long long)l[j].sh * p.rows + row] : -INFINITY;
+                for (int r = 0; r < end - row; r++) {
+                    st[r] = r > 0 || lse == -INFINITY ? -INFINITY : -lse * LOG2E;
+                    st[64 + r] = r > 0 ? 0.0f : -dot;
                 }
             }
         }
     }
-    if (stats) keep_norm(0);
 }
 
 }  // namespace
@@ -205,16 +150,12 @@ size_t attn_split_space(void* base, size_t seqs, size_t q_heads, size_t k_heads,
     };
     AttnSplitSpace s{};
     const size_t q = seqs * q_heads * q_rows * head_dim * 4, k = seqs * k_heads * k_rows * head_dim * 4;
-    s.maxima = static_cast<float*>(take(4 * sizeof(float)));
-    s.partial = static_cast<float*>(take(4 * kSplitBlocks * sizeof(float)));
     s.q = take(q);
     s.k = take(k);
     s.v = take(k);
-    if (backward) {
-        s.dout = take(q);
-        s.head_norm = static_cast<float*>(take(seqs * q_heads * sizeof(float)));
-        s.stats = static_cast<float*>(take(seqs * q_heads * ((q_rows + 127) / 128) * 2 * kSplitStat * sizeof(float)));
-    }
+    s.stats = static_cast<float*>(take(seqs * q_heads * ((q_rows + 127) / 128) * 2 * kSplitStat * sizeof(float)));
+    s.key_stats = static_cast<float*>(take(seqs * k_heads * ((k_rows + 63) / 64) * kKeyStat * sizeof(float)));
+    if (backward) s.dout = take(q);
     if (out) *out = s;
     return at;
 }
@@ -245,18 +186,12 @@ void launch_attention_split(cudaStream_t s, const AttnArgs& a, const AttnSplitSp
     t.o_wide = wide(a.o);
     t.lse = a.lse;
     t.sp = sp;
-    t.heads_total = a.seqs * a.q_heads;
     t.q_tiles = (a.q_rows + 127) / 128;
+    t.k_tiles = (a.k_rows + 63) / 64;
     t.backward = backward;
     const long long per = (long long)THREADS / (a.head_dim / 4) * ILP;
-    const dim3 grid((unsigned)std::clamp<long long>((most + per - 1) / per, 1, kSplitBlocks), backward ? 4 : 3);
-    if (a.head_dim == 64) {
-        launch_pdl(attention_absmax_kernel<64>, grid, dim3(THREADS), 0, s, t);
-        launch_pdl(attention_split_kernel<64>, grid, dim3(THREADS), 0, s, t);
-    } else {
-        launch_pdl(attention_absmax_kernel<128>, grid, dim3(THREADS), 0, s, t);
-        launch_pdl(attention_split_kernel<128>, grid, dim3(THREADS), 0, s, t);
-    }
+    const dim3 grid((unsigned)std::clamp<long long>((most + per - 1) / per, 1, BLOCKS), backward ? 4 : 3);
+    launch_pdl(a.head_dim == 64 ? attention_split_kernel<64> : attention_split_kernel<128>, grid, dim3(THREADS), 0, s, t);
 }
 
 }  // namespace n3d

@@ -34,12 +34,17 @@
 // two, so that small weights and gradients keep fp16's precision; |dS| <= 2 P |dout row|
 // |v row| then stays inside fp16 while |v row| < 4096.
 //
-// fp32: every operand is a pair h + l of fp16 arrays (attention_train_split.cu), P and dS are split
-// in the softmax, and each product is l h + h l + h h.  The tensor cores' fp32 accumulators
-// truncate: about 2^-26 of the accumulator per MMA, always towards zero, which 12 MMAs a block
-// carry to 1.5e-5 at 4096 rows.  So an accumulator takes two blocks, the small products
-// of each first, and is then added to a sum that is rounded to nearest (more TMEM, or the
-// output tensor).
+// fp32: every operand is a pair h + l of fp16 arrays (attention_train_split.cu), each row of it in a unit
+// of its own, a power of two; the weights are split in the softmax, and each product is l h + h l + h h.
+// Scores and T2 are multiplied by the units of their row and column; a weight by the unit of the column
+// that the second product multiplies it with, and then by a power of two of its own row that
+// brings the row's largest weight of the block into [64, 128).  So each row of each operand, and each row of
+// weights, keeps 22 bits however small it is beside others, and no sequence depends on the others of its batch.
+// The tensor cores' fp32 accumulators truncate: about 2^-26 of the accumulator per MMA, always
+// towards zero, which 12 MMAs a block carry to 1.5e-5 at 4096 rows.  So an accumulator takes two blocks, the
+// small products of each first, and is then added to a sum that is rounded to nearest (more
+// TMEM, or the output tensor), which also takes it out of its row's unit.  The second block of two keeps the
+// first one's unit unless its own weights do not fit there.
 //
 // Bound, from clock stamps in every role: at head_dim 128 in forward and dq the thread that
 // issues T, whose block of 8 or 16 MMAs takes 300 - 570 clocks and each wait, passed at once,
@@ -87,22 +92,28 @@ struct Cfg {
     // (dq) 931 and 959; 128 windows of 384 rows, 8 heads of 64: gradient 262 and 268, but forward 78.7 and
     // 75.7 (the copy is on the path of every item of six blocks).  dkv's accumulators leave no room, nor do pairs.
     static constexpr bool ROW_TMEM = !PAIR && (MODE == GRAD_Q || (MODE == FORWARD && HD == 128));
-    // score buffers: as many as TMEM holds (forward of 128: a third took 312 us to 265, with the row tiles' move)
-    static constexpr int NBUF = MODE != FORWARD ? NWG : ROW_TMEM ? 3 : 2;
+    // Score buffers, as many as TMEM holds where that pays.  Forward of 128: a third took 312 us to 265, with the
+    // row tiles' move; forward of pairs, 2 x 4096 rows, 16 heads of 64: two 852 us, three 766, four 693 (of 128:
+    // no change); dq of pairs, 64 heads of 501 rows of 64: a third takes the gradient from 109 to 107.
+    static constexpr int NBUF = PAIR && HD == 64 && MODE != GRAD_KV ? (MODE == FORWARD ? 4 : 3) : MODE != FORWARD ? NWG : ROW_TMEM ? 3 : 2;
     // gradients whose weights all lie over T2: T1 of the buffer's next block need not wait for the products that
     // read them
     static constexpr bool EARLY = GRAD && !(PAIR && MODE == GRAD_KV);
     static constexpr int SOFTMAX = 3;                       // first softmax warp
     static constexpr int THREADS = 32 * SOFTMAX + 128 * NWG, PER_SM = SMALL ? 2 : 1;
     static constexpr int RTILE = ROWS * HD * 2 * PARTS, CTILE = COLS * HD * 2 * PARTS;  // bytes
-    static constexpr int STATS = MODE == GRAD_KV ? 512 : 0;               // 64 x (-lse log2 e), 64 x (-D)
+    // 64 x (-lse log2 e), 64 x (-D), pairs: the units of q and dout; pairs otherwise: those of k and v
+    static constexpr int STATS = MODE == GRAD_KV ? (PAIR ? kSplitStat : 128) * 4 : PAIR ? kKeyStat * 4 : 0;
     static constexpr int STAT_LD = PARTS == 1 ? 128 : kSplitStat;         // floats of a block of 64 rows
     static constexpr int STAGE = 2 * CTILE + 1024 * (STATS > 0);
     static constexpr int ROW_BYTES = (GRAD ? 2 : 1) * RTILE;
     // floats of the groups' row statistics (double-buffered by item)
-    static constexpr int JOIN = MODE == FORWARD && NWG > 1 ? (4 + 2 * PAIR) * 128 : 4;
+    static constexpr int JOIN = MODE == FORWARD ? (NWG > 1 ? (4 + 4 * PAIR) * 128 : 4) : PAIR ? 2 * 128 : 4;
+    // pairs, gradients: the rows' units of the weights, from the group of an even block to that of the next
+    // (double-buffered by pair of blocks)
+    static constexpr int UNITS = PAIR && GRAD ? 4 * 128 : 0;
     // barriers, items, the TMEM slot, the statistics, and slack to align the tiles to 1024 bytes
-    static constexpr int REST = 704 + 2 * JOIN * 4 + 1024;
+    static constexpr int REST = 704 + 2 * JOIN * 4 + UNITS * 4 + 1024;
     static constexpr int ROOM = 226 * 1024 / PER_SM - REST;
     // Row tiles of two items, so that the next one's load during this one's work, where that leaves enough
     // stages.  Gradient of 64 windows of 384 rows of 64: 155 us with two and two, 174 with one and four;
@@ -247,11 +258,27 @@ __device__ __forceinline__ float row_lse(float l, float m, float k2, float shift
     const double t = (double)m * (double)k2 + ((double)((bits >> 23) - 127) - (double)shift) + (double)log2f(mantissa);
     return (float)(t * 0.6931471805599453);
 }
-// Pairs: the power of two that keeps |dS| times it within 2^15, from |dS| <= 2 |dout row| |v row| and
-// |v row| <= sqrt(head_dim) max|v|.
-template <int HD>
-__device__ __forceinline__ float pair_ds_scale(float norm, float v_max) {
-    return 0.5f * split_scale_of(norm * v_max * (HD == 64 ? 8.0f : 11.3137085f));
+// Four floats of shared memory, not moved ahead of what stands before it (which would hold registers).
+__device__ __forceinline__ float4 lds4(const float4* p) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(p)));
+    return v;
+}
+// Pairs: the power of two that brings a row's largest weight w into [64, 128); 1 if there is none.  (Held below
+// 2^126, so that its inverse is normal too.)
+__device__ __forceinline__ float weight_unit(float w) {
+    return w > 0.0f && w < INFINITY ? __int_as_float(min(253, 260 - (__float_as_int(w) >> 23)) << 23) : 1.0f;
+}
+constexpr float MAX_WEIGHT = 32768.0f;  // that a row's unit may bring a weight to
+// The largest of sixteen magnitudes and m.
+__device__ __forceinline__ float max16(const float* x, float m) {
+    float a = fabsf(x[0]), b = fabsf(x[1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 4) {
+        a = max3f(a, fabsf(x[i]), fabsf(x[i + 1]));
+        if (i + 2 < 16) b = max3f(b, fabsf(x[i + 2]), fabsf(x[i + 3]));
+    }
+    return max3f(m, a, b);
 }
 
 // Both waits, tested one behind the other before either's result is used: a wait that passes at once costs the issuing
@@ -272,10 +299,10 @@ struct TcArgs {
     int ascending;     // which end of a one-sided window is open: 1 if keys before the query
     float k2, factor;  // |scale| log2 e; the scale of dq and dk
     int negate;        // scale < 0
-    float* stats;      // [seqs * q_heads][q tiles][2][-lse log2 e: 64 | -D: 64 (| pairs: |dout row|: 64)]
-    float* norms;      // [seqs * q_heads][q tiles]: the largest |dout row|; pairs: [seqs * q_heads]
-    const float* maxima;  // pairs: the largest |q|, |k|, |v|, |dout|
-    int q_tiles;
+    float* stats;      // [seqs * q_heads][q tiles][2][-lse log2 e: 64 | -D: 64 (| pairs: units of q: 64 | of dout: 64)]
+    float* norms;      // [seqs * q_heads][q tiles]: the largest |dout row|
+    const float* key_stats;  // pairs: [seqs * k_heads][k tiles][units of k: 64 | of v: 64]
+    int q_tiles, k_tiles;    // of 128 query rows, of 64 key rows
 };
 
 // T: the type of the MMA operands; tensors are of type T (PARTS 1) or fp32 (PARTS 2, T = fp16).
@@ -314,11 +341,13 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
     uint64_t* item_full = rows_in + 1;     // 2: item k is known (slot k % 2)
     uint64_t* item_empty = item_full + 2;  // 2: item k was read by every other warp
     uint64_t* answered = item_empty + 2;   // 1: the scheduler's answer arrived
+    uint64_t* unit_set = answered + 1;     // 2 (pairs, gradients): the units of pair of blocks x are known (slot x % 2)
     static_assert(NST <= 4 && NBUF <= 4 && NWG <= 2 && C::RB <= 2, "barriers");
     Item* items = reinterpret_cast<Item*>(bars + 36);  // 2
     uint8_t* answer = reinterpret_cast<uint8_t*>(bars + 48);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 50);
     float* joins = reinterpret_cast<float*>(bars + 52);  // 2 x JOIN
+    float* units = joins + 2 * C::JOIN;                  // UNITS
 
     // The reduction tells the compiler that a value is the same in the warp, which keeps what the issuing warps
     // derive from it in uniform registers, where MMAs take their operands from.
@@ -335,6 +364,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         mbar_init(rows_in, 4 * NWG);
         for (int i = 0; i < 2; i++) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 2 + 4 * NWG);
         mbar_init(answered, 1);
+        for (int i = 0; i < 2; i++) mbar_init(&unit_set[i], 4);
         mbar_fence_init();
     }
     if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -456,6 +486,10 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                             bulk_load(st + 2 * C::CTILE,
                                       args.stats + (((long long)it.seq * a.q_heads + ch) * args.q_tiles * 2 + c0 / COLS) *
                                                        C::STAT_LD,
+                                      C::STATS, cb);
+                        else if (PAIR)
+                            bulk_load(st + 2 * C::CTILE,
+                                      args.key_stats + (((long long)it.seq * a.k_heads + ch) * args.k_tiles + c0 / COLS) * kKeyStat,
                                       C::STATS, cb);
                     }
                     if (ok) gt += it.nblk;
@@ -614,21 +648,11 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
         const int wg = (warp - C::SOFTMAX) / 4;
         const int qd = warp & 3, r = qd * 32 + lane;
         const uint32_t lb = tmem + (static_cast<uint32_t>(qd * 32) << 16);
-        // pairs: the powers of two that q, k, v and dout were multiplied by
-        float s_q = 1.0f, s_k = 1.0f, s_v = 1.0f, s_do = 1.0f, v_max = 0.0f;
-        if (PAIR) {
-            s_q = split_scale_of(args.maxima[0]);
-            s_k = split_scale_of(args.maxima[1]);
-            v_max = args.maxima[2];
-            s_v = split_scale_of(v_max);
-            if (C::GRAD) s_do = split_scale_of(args.maxima[3]);
-        }
-        // Held normal: with tiny q and k the quotient would be 0, and 0 times the -inf of a masked score NaN.  (Raw
-        // scores stay below 2^37, so such scores are 0 next to 1 either way.)
-        const float k2 = PAIR ? fmaxf(args.k2 / s_q / s_k, 1.17549435e-38f) : args.k2;
-        const float dp_unit = PAIR ? 1.0f / s_do / s_v : 1.0f;  // T2 times this is dP
-        constexpr float P_LOG2 = !F16 ? 0.0f : MODE == FORWARD ? 7.0f : MODE == GRAD_KV ? (PAIR ? 15.0f : 10.0f) : 0.0f;
-        constexpr float P_SCALE = PAIR ? 32768.0f : 1024.0f;  // 2^P_LOG2 of dkv
+        // (pairs: the scores are in units of log2 once they are read)
+        const float k2 = PAIR ? 1.0f : args.k2;
+        constexpr float P_LOG2 = !F16 || PAIR ? 0.0f : MODE == FORWARD ? 7.0f : MODE == GRAD_KV ? 10.0f : 0.0f;
+        constexpr float P_SCALE = 1024.0f;  // 2^P_LOG2 of dkv
+        int pairs = 0;  // pairs, gradients: pairs of blocks of the items before
         bool ok = true;
         Item it;
         for (int k = 0, gt = 0, n = 0; next_item(k, it); k++) {
@@ -673,12 +697,21 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             const bool single = MODE == GRAD_Q && !PAIR && live && hi > lo && (hi - 1) / COLS == lo / COLS;
             // dq: this row's -lse log2 e, -D and fp16 scale; dkv: the fp16 scale of the head group
             float nlse = 0.0f, ndot = 0.0f, ds_scale = 1.0f;
-            if (MODE == GRAD_Q && PAIR) {
+            // pairs: this row's factors of T1 and T2
+            float row1 = 0.0f, row2 = 0.0f;
+            if (PAIR && MODE == GRAD_KV) {
+                const float* st =
+                    args.key_stats + (((long long)seq * a.k_heads + head) * args.k_tiles + row / 64) * kKeyStat + row % 64;
+                if (live) row1 = args.k2 * st[0], row2 = st[64];
+            } else if (PAIR) {
                 const float* st =
                     args.stats + ((((long long)seq * a.q_heads + head) * args.q_tiles + r0 / ROWS) * 2 + r / 64) * C::STAT_LD + r % 64;
-                nlse = live ? st[0] : -INFINITY;
-                ndot = live ? st[64] : 0.0f;
-                ds_scale = pair_ds_scale<HD>(live ? st[128] : 0.0f, v_max);
+                if (live) row1 = args.k2 * st[128];
+                if (MODE == GRAD_Q) {
+                    nlse = live ? st[0] : -INFINITY;
+                    ndot = live ? st[64] : 0.0f;
+                    row2 = live ? st[192] : 0.0f;
+                }
             } else if (MODE == GRAD_Q) {
                 const long long sqh = (long long)seq * a.q_heads + head;
                 float norm2 = 0.0f;
@@ -720,36 +753,83 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     }
                 }
             }
-            if (MODE == GRAD_KV && F16) {
-                // the largest |dout row| of the head group: a pair has one for each head, otherwise one for each tile
+            if (MODE == GRAD_KV && F16 && !PAIR) {
+                // the largest |dout row| of the head group, from one for each tile
                 float m = 0.0f;
-                const int per = PAIR ? 1 : args.q_tiles;
-                const float* n = args.norms + ((long long)seq * a.q_heads + head * group) * per;
-                for (int i = lane; i < group * per; i += 32) m = fmaxf(m, n[i]);
+                const float* n = args.norms + ((long long)seq * a.q_heads + head * group) * args.q_tiles;
+                for (int i = lane; i < group * args.q_tiles; i += 32) m = fmaxf(m, n[i]);
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                ds_scale = PAIR ? pair_ds_scale<HD>(m, v_max) : 8.0f * inverse_power(m);
+                ds_scale = 8.0f * inverse_power(m);
             }
 
             float m = -INFINITY, l = 0.0f;  // forward: running maximum (raw scores) and sum (times 2^P_LOG2)
             float m_sum = -INFINITY;        // pairs, forward: the maximum that the summed accumulators refer to
             auto sum_factor = [&](float to) { return m_sum == to ? 1.0f : ex2_approx((m_sum - to) * k2); };
+            // pairs: the units of this row's weights (dkv: of dS and of P) in the accumulators; 0: all were 0 so far
+            float unit1 = 0.0f, unit2 = 0.0f;
+            // the unit after a block whose largest weight is `top`: a first block (of two) takes its own, a second one the
+            // first one's if its weights fit there.  Returns what the accumulator is to be multiplied by.
+            auto new_unit = [&](float& unit, float top, bool first) {
+                const float before = unit;
+                if (first || before == 0.0f) {
+                    unit = top > 0.0f ? weight_unit(top) : 0.0f;
+                    return 1.0f;
+                }
+                if (!(top * before > MAX_WEIGHT)) return 1.0f;
+                unit = weight_unit(top);
+                return unit / before;
+            };
+            auto used = [](float unit) { return unit == 0.0f ? 1.0f : unit; };
+            // multiplies `n` columns of an accumulator of this warp's rows
+            auto scale_acc = [&](uint32_t acc, int n, float by) {
+                const uint64_t c2 = pack2(by, by);
+#pragma unroll 1
+                for (int cb = 0; cb < n; cb += 16) {
+                    float o[16];
+                    uint32_t u[16];
+                    tmem_ld16(acc + cb, o);
+#pragma unroll
+                    for (int d = 0; d < 16; d += 2) {
+                        unpack2(mul2(pack2(o[d], o[d + 1]), c2), o[d], o[d + 1]);
+                        u[d] = __float_as_uint(o[d]), u[d + 1] = __float_as_uint(o[d + 1]);
+                    }
+                    tmem_st16(acc + cb, u);
+                }
+            };
             for (int gi = NWG == 1 ? 0 : (wg + gt) & 1; gi < nblk; gi += NWG) {
                 const int g = gt + gi, buf = g % NBUF, c0 = col0(it, gi);
                 const uint32_t t = lb + buf * C::TBUF;
                 const bool full = c0 >= it.full_lo && c0 + COLS <= it.full_hi;
                 // T of block g (phase g / NBUF of its buffer: the next needs this block's weights).  After an
                 // expired wait the loop keeps running (results unused).
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(&t_full[buf], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                // Column statistics came by bulk copy: this thread's own wait makes them visible.
+                uint64_t *t_bar = &t_full[buf], *c_bar = &c_full[g % NST];
+                ok = __all_sync(0xffffffffu, ok && (C::STATS > 0 ? wait_both(t_bar, (g / NBUF) & 1, c_bar, (g / NST) & 1, err)
+                                                                 : mbar_wait(t_bar, (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN)));
                 tc_fence_after();
+                const int nth = MODE == FORWARD ? gi / NWG : gi;  // the block's number in its accumulator
+                const float4* st = reinterpret_cast<const float4*>(ring + (g % NST) * C::STAGE + 2 * C::CTILE);
                 if constexpr (MODE == FORWARD) {
                     float s[64];
                     tmem_ld32(t, s);
                     tmem_ld32(t + 32, s + 32);
+                    // Pairs: the units of the columns; the row's factor, which may be 0, before -inf takes a score's place
+                    const float kf = !PAIR ? args.k2 : full ? row1 : 1.0f;
+                    if constexpr (PAIR) {
+#pragma unroll
+                        for (int c = 0; c < 64; c += 4) {
+                            const float4 kk = lds4(st + c / 4);
+                            unpack2(mul2(pack2(s[c], s[c + 1]), pack2(kk.x, kk.y)), s[c], s[c + 1]);
+                            unpack2(mul2(pack2(s[c + 2], s[c + 3]), pack2(kk.z, kk.w)), s[c + 2], s[c + 3]);
+                        }
+                    }
                     if (!full) {
 #pragma unroll
-                        for (int c = 0; c < 64; c++)
+                        for (int c = 0; c < 64; c++) {
+                            if (PAIR) s[c] *= row1;
                             if (c0 + c < lo || c0 + c >= hi) s[c] = -INFINITY;
+                        }
                     }
                     float mx[8];
 #pragma unroll
@@ -758,65 +838,71 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     for (int c = 16; c < 64; c += 16)
 #pragma unroll
                         for (int i = 0; i < 8; i++) mx[i] = max3f(mx[i], s[c + i], s[c + 8 + i]);
-                    const float mb = max3f(max3f(mx[0], mx[1], mx[2]), max3f(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+                    const float mb = max3f(max3f(mx[0], mx[1], mx[2]), max3f(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) *
+                                     (PAIR ? kf : 1.0f);
                     // (an unseen block leaves mb = -inf: no raise, and the exponents below stay -inf)
                     const bool raise = mb > m && (mb - m) * k2 > RESCALE_LOG2;
                     const float corr = raise ? ex2_approx((m - mb) * k2) : 1.0f;  // 0 from m = -inf
                     if (raise) m = mb;
                     const float off = m == -INFINITY ? 0.0f : P_LOG2 - m * k2;
-                    const uint64_t k22 = pack2(k2, k2), off2 = pack2(off, off);
+                    const uint64_t k22 = pack2(kf, kf), off2 = pack2(off, off);
                     uint64_t sum2[4] = {0, 0, 0, 0};
-                    // 16 words of weights at a time, over scores that are in registers (pairs: 16 columns, 8 words of
-                    // h and 8 of l)
-                    constexpr int CW = 32 / PARTS;
+                    float acc_by = corr;  // what the accumulator is multiplied by
+                    if constexpr (PAIR) {
+                        float top = 0.0f, tops[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int i = 0; i < 64; i += CW) {
-                        uint32_t w[16];
+                        for (int c = 0; c < 64; c += 4) {
+                            const float4 vv = lds4(st + 16 + c / 4);
 #pragma unroll
-                        for (int c = i; c < i + CW; c += 2) {
-                            float x, y;
-                            unpack2(fma2(pack2(s[c], s[c + 1]), k22, off2), x, y);
-                            x = ex2_approx(x);
-                            y = ex2_approx(y);
-                            sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], pack2(x, y));
-                            const int j = (c - i) / 2;
-                            if constexpr (PAIR)
-                                split2x2(x, y, 1.0f, w[j], w[8 + j]);
-                            else
-                                w[j] = pack_pair<T>(x, y);
+                            for (int e = c; e < c + 4; e += 2) {
+                                float x, y;
+                                unpack2(fma2(pack2(s[e], s[e + 1]), k22, off2), x, y);
+                                const uint64_t p2 = pack2(ex2_approx(x), ex2_approx(y));
+                                sum2[(e >> 1) & 3] = add2(sum2[(e >> 1) & 3], p2);
+                                unpack2(mul2(p2, e == c ? pack2(vv.x, vv.y) : pack2(vv.z, vv.w)), s[e], s[e + 1]);
+                                tops[(e >> 1) & 3] = max3f(tops[(e >> 1) & 3], s[e], s[e + 1]);
+                            }
                         }
-                        tmem_st16(t + i / CW * 16, w);
+                        top = fmaxf(max3f(tops[0], tops[1], tops[2]), tops[3]);
+                        acc_by *= new_unit(unit1, top, nth % 2 == 0);
+                        const float by = used(unit1);
+#pragma unroll
+                        for (int i = 0; i < 64; i += 16) {  // 8 words of h and 8 of l
+                            uint32_t w[16];
+#pragma unroll
+                            for (int c = 0; c < 16; c += 2) split2x2(s[i + c], s[i + c + 1], by, w[c / 2], w[8 + c / 2]);
+                            tmem_st16(t + i, w);
+                        }
+                    } else {
+                        // 16 words of weights at a time, over scores that are in registers
+#pragma unroll
+                        for (int i = 0; i < 64; i += 32) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int c = i; c < i + 32; c += 2) {
+                                float x, y;
+                                unpack2(fma2(pack2(s[c], s[c + 1]), k22, off2), x, y);
+                                x = ex2_approx(x);
+                                y = ex2_approx(y);
+                                sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], pack2(x, y));
+                                w[(c - i) / 2] = pack_pair<T>(x, y);
+                            }
+                            tmem_st16(t + i / 2, w);
+                        }
                     }
                     float sa, sb;
                     unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sa, sb);
                     l = l * corr + (sa + sb);
-                    if (gi >= NWG && !(C::SUM && gi / NWG % 2 == 0) && __any_sync(0xffffffffu, raise)) {
+                    if (nth > 0 && !(C::SUM && nth % 2 == 0) && __any_sync(0xffffffffu, acc_by != 1.0f)) {
                         // this group's previous product (its phase: the buffer's next product needs P of
                         // this or a later block of the group)
                         ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_done[(g - NWG) % NBUF], ((g - NWG) / NBUF) & 1, err,
                                                                      DEV_TIMEOUT_ATTN_TRAIN));
                         tc_fence_after();
-                        const uint32_t acc = lb + C::ACC + wg * HD;
-                        const uint64_t c2 = pack2(corr, corr);
-#pragma unroll 1
-                        for (int cb = 0; cb < HD; cb += 16) {
-                            float o[16];
-                            uint32_t u[16];
-                            tmem_ld16(acc + cb, o);
-#pragma unroll
-                            for (int d = 0; d < 16; d += 2) {
-                                unpack2(mul2(pack2(o[d], o[d + 1]), c2), o[d], o[d + 1]);
-                                u[d] = __float_as_uint(o[d]), u[d + 1] = __float_as_uint(o[d + 1]);
-                            }
-                            tmem_st16(acc + cb, u);
-                        }
+                        scale_acc(lb + C::ACC + wg * HD, HD, acc_by);
                     }
                 } else {
-                    const float4* st = reinterpret_cast<const float4*>(ring + (g % NST) * C::STAGE + 2 * C::CTILE);
-                    const uint64_t k22 = pack2(k2, k2), scale2 = pack2(ds_scale, ds_scale), unit2 = pack2(dp_unit, dp_unit);
-                    if (MODE == GRAD_KV)  // the statistics came by bulk copy: this thread's own wait makes them visible
-                        ok = __all_sync(0xffffffffu,
-                                        ok && mbar_wait(&c_full[g % NST], (g / NST) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                    const uint64_t k22 = pack2(k2, k2), scale2 = pack2(ds_scale, ds_scale);
                     // A row of few keys has large P, and dP - D cancels: with D from the rounded output, dS would
                     // keep that rounding (a row with one key has dS = 0).  Where the row's keys are all here,
                     // D = sum P dP, for dkv too.
@@ -847,7 +933,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                         // as registers hold.  2 x 4096 rows, 16 heads of 128: gradient 904 us with both, 914 with none;
                         // of 64 with both 677, with one 682, with none 700, but both spill there and fp16 takes
                         // 154 us for 64 windows of 384 rows, 151 with one or none.
-                        constexpr int AHEAD = MODE != GRAD_KV || PAIR ? 0 : C::SMALL ? 1 : 2;
+                        constexpr int AHEAD = MODE != GRAD_KV ? 0 : C::SMALL ? 1 : 2;
 #pragma unroll
                         for (int h = 0; h < COLS; h += CH) {  // the weights go over scores that are read already
                             float s[CH], u[CH];
@@ -858,7 +944,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                                 if (AHEAD > 1) sd[c] = st[16 + h / 4 + c];
                             }
                             tmem_ld_pair(t + h, t + 64 + h, s, u);
-                            uint32_t w[CH * PARTS], *dw = w, *pw = w + CH / 2 * PARTS;  // pairs: h, then l
+                            uint32_t w[CH], *dw = w, *pw = w + CH / 2;
 #pragma unroll
                             for (int c = 0; c < CH; c += 4) {
                                 float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
@@ -877,35 +963,127 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                                     y = ex2_approx(y);
                                     if (masked && (cc < lo || cc >= hi)) x = 0.0f;
                                     if (masked && (cc + 1 < lo || cc + 1 >= hi)) y = 0.0f;
-                                    const uint64_t u2 = pack2(u[c + e], u[c + e + 1]);
-                                    uint64_t g2 = mul2(pack2(x, y), PAIR ? fma2(u2, unit2, d2) : add2(u2, d2));
+                                    uint64_t g2 = mul2(pack2(x, y), add2(pack2(u[c + e], u[c + e + 1]), d2));
                                     if (F16) g2 = mul2(g2, scale2);
                                     unpack2(g2, gx, gy);
                                     if (masked && x == 0.0f) gx = 0.0f;
                                     if (masked && y == 0.0f) gy = 0.0f;
                                     const int i = (c + e) / 2;
-                                    if constexpr (PAIR) {
-                                        if (MODE == GRAD_KV) split2x2(x, y, P_SCALE, pw[i], pw[CH / 2 + i]);
-                                        split2x2(gx, gy, 1.0f, dw[i], dw[CH / 2 + i]);
-                                    } else {
-                                        if (MODE == GRAD_KV)
-                                            pw[i] = F16 ? pack_pair<T>(x * P_SCALE, y * P_SCALE) : pack_pair<T>(x, y);
-                                        dw[i] = pack_pair<T>(gx, gy);
-                                    }
+                                    if (MODE == GRAD_KV)
+                                        pw[i] = F16 ? pack_pair<T>(x * P_SCALE, y * P_SCALE) : pack_pair<T>(x, y);
+                                    dw[i] = pack_pair<T>(gx, gy);
                                 }
                             }
-                            if constexpr (MODE == GRAD_KV && !PAIR) {
+                            if constexpr (MODE == GRAD_KV)
                                 tmem_st16(t + 64 + h, w);  // both over T2
-                            } else {
-                                if (MODE == GRAD_KV) tmem_st<CH / 2 * PARTS>(t + h / 2 * PARTS, pw);
-                                tmem_st<CH / 2 * PARTS>(t + 64 + h / 2 * PARTS, dw);
-                            }
+                            else
+                                tmem_st8(t + 64 + h / 2, dw);
                         }
                     };
-                    if (full)
-                        weights(std::false_type());
+                    // Pairs: dS (and P) times the units of their columns, first as they are, for their largest, then
+                    // in the row's unit as h and l; meanwhile they are in TMEM, over T2 and over the scores.
+                    auto pair_weights = [&](auto masked) {
+                        constexpr int CH = 16;
+                        constexpr bool KV = MODE == GRAD_KV;
+                        const uint64_t row12 = pack2(row1, row1), row22 = pack2(row2, row2);
+                        float top1 = 0.0f, top2 = 0.0f;
+#pragma unroll
+                        for (int h = 0; h < COLS; h += CH) {
+                            float s[CH], u[CH];
+                            tmem_ld_pair(t + h, t + 64 + h, s, u);
+#pragma unroll
+                            for (int c = 0; c < CH; c += 4) {
+                                // units of the columns of T1 and T2 (k and v, or q and dout)
+                                const float4 a4 = lds4(st + (KV ? 32 : 0) + (h + c) / 4), b4 = lds4(st + (KV ? 48 : 16) + (h + c) / 4);
+                                float4 nl = make_float4(nlse, nlse, nlse, nlse), nd = make_float4(ndot, ndot, ndot, ndot);
+                                if (KV) nl = lds4(st + (h + c) / 4), nd = lds4(st + 16 + (h + c) / 4);
+#pragma unroll
+                                for (int e = 0; e < 4; e += 2) {
+                                    const uint64_t n2 = e == 0 ? pack2(nl.x, nl.y) : pack2(nl.z, nl.w);
+                                    const uint64_t d2 = e == 0 ? pack2(nd.x, nd.y) : pack2(nd.z, nd.w);
+                                    const uint64_t a2 = e == 0 ? pack2(a4.x, a4.y) : pack2(a4.z, a4.w);
+                                    const uint64_t b2 = e == 0 ? pack2(b4.x, b4.y) : pack2(b4.z, b4.w);
+                                    const int i = c + e, cc = c0 + h + i;
+                                    float x, y, gx, gy;
+                                    unpack2(fma2(mul2(pack2(s[i], s[i + 1]), a2), row12, n2), x, y);
+                                    x = ex2_approx(x);
+                                    y = ex2_approx(y);
+                                    if (masked && (cc < lo || cc >= hi)) x = 0.0f;
+                                    if (masked && (cc + 1 < lo || cc + 1 >= hi)) y = 0.0f;
+                                    const uint64_t g2 = mul2(pack2(x, y), fma2(mul2(pack2(u[i], u[i + 1]), b2), row22, d2));
+                                    unpack2(mul2(g2, a2), gx, gy);
+                                    if (masked && x == 0.0f) gx = 0.0f;
+                                    if (masked && y == 0.0f) gy = 0.0f;
+                                    if (KV) unpack2(mul2(pack2(x, y), b2), s[i], s[i + 1]);
+                                    u[i] = gx, u[i + 1] = gy;
+                                }
+                            }
+                            uint32_t w[CH];
+                            if (KV) {
+                                top2 = max16(s, top2);
+#pragma unroll
+                                for (int c = 0; c < CH; c++) w[c] = __float_as_uint(s[c]);
+                                tmem_st16(t + h, w);
+                            }
+                            top1 = max16(u, top1);
+#pragma unroll
+                            for (int c = 0; c < CH; c++) w[c] = __float_as_uint(u[c]);
+                            tmem_st16(t + 64 + h, w);
+                        }
+                        // The row's units: an even block's go to the group of the next one, which goes on with them.
+                        // (unit_set: phase x / 2 of its slot for pair x.  The slot is set again two pairs on, by a block at least
+                        // four on; its T2 waits for the products of a block three before it or two, hence for this pair's
+                        // second one's weights.)
+                        const int x = pairs + gi / 2;
+                        float* const xu = units + (x & 1) * 256;
+                        float by1 = 1.0f, by2 = 1.0f;
+                        if (gi % 2 == 0) {
+                            new_unit(unit1, top1, true);
+                            if (KV) new_unit(unit2, top2, true);
+                            if (gi + 1 < nblk) {
+                                xu[r] = unit1;
+                                if (KV) xu[128 + r] = unit2;
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&unit_set[x & 1]);
+                            }
+                        } else {
+                            ok = __all_sync(0xffffffffu, ok && mbar_wait(&unit_set[x & 1], (x >> 1) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+                            unit1 = xu[r];
+                            by1 = new_unit(unit1, top1, false);
+                            if (KV) unit2 = xu[128 + r], by2 = new_unit(unit2, top2, false);
+                            if (__any_sync(0xffffffffu, by1 != 1.0f || by2 != 1.0f)) {
+                                // the even block's product (its phase: the next product of its buffer follows this block's)
+                                ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_done[(g - 1) % NBUF], ((g - 1) / NBUF) & 1, err,
+                                                                             DEV_TIMEOUT_ATTN_TRAIN));
+                                tc_fence_after();
+                                scale_acc(lb + C::ACC, HD, by1);
+                                if (KV) scale_acc(lb + C::ACC + HD, HD, by2);
+                            }
+                        }
+                        const float u1 = used(unit1), u2 = used(unit2);
+                        tmem_wait_st();  // what is read again
+#pragma unroll
+                        for (int h = 0; h < COLS; h += CH) {
+                            float d[CH];
+                            uint32_t w[CH];
+                            if constexpr (KV) {
+                                float p[CH];
+                                tmem_ld_pair(t + h, t + 64 + h, p, d);
+#pragma unroll
+                                for (int c = 0; c < CH; c += 2) split2x2(p[c], p[c + 1], u2, w[c / 2], w[8 + c / 2]);
+                                tmem_st16(t + h, w);
+                            } else {
+                                tmem_ld16(t + 64 + h, d);
+                            }
+#pragma unroll
+                            for (int c = 0; c < CH; c += 2) split2x2(d[c], d[c + 1], u1, w[c / 2], w[8 + c / 2]);
+                            tmem_st16(t + 64 + h, w);
+                        }
+                    };
+                    if constexpr (PAIR)
+                        full ? pair_weights(std::false_type()) : pair_weights(std::true_type());
                     else
-                        weights(std::true_type());
+                        full ? weights(std::false_type()) : weights(std::true_type());
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -913,19 +1091,21 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 if (lane == 0) mbar_arrive(&p_full[buf]);
 
                 // pairs: after every second product into an accumulator, if another follows, add it to the sum
-                const int nth = MODE == FORWARD ? gi / NWG : gi;
                 if (C::SUM && nth % 2 == 1 && gi + (MODE == FORWARD ? NWG : 1) < nblk) {
                     // (its phase: the buffer's next product needs weights of this group)
                     ok = __all_sync(0xffffffffu,
                                     ok && mbar_wait(&acc_done[buf], (g / NBUF) & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
                     tc_fence_after();
                     const float f = MODE == FORWARD ? sum_factor(m) : 1.0f;
+                    const float to1 = 1.0f / used(unit1), to2 = 1.0f / used(unit2);  // exact
                     const uint32_t from = lb + C::ACC + (MODE == FORWARD ? wg * HD : 0);
                     constexpr int WIDTH = MODE == GRAD_KV ? 2 * HD : HD;
 #pragma unroll 1
                     for (int cb = 0; cb < WIDTH; cb += 16) {
                         float o[16], u[16];
                         tmem_ld16(from + cb, o);
+#pragma unroll
+                        for (int d = 0; d < 16; d++) o[d] *= cb < HD ? to1 : to2;
                         if constexpr (C::SUM_OUT) {
                             if (live) {
                                 float* to = out_row(cb < HD ? a.dk : a.dv) + cb % HD;
@@ -973,18 +1153,28 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             // ---- the accumulators, once every product has completed (phase n; the next needs acc_read)
             if (nblk > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(all_done, n & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
             tc_fence_after();
-            if (C::SUM_OUT) asm volatile("bar.sync 1, 256;" ::: "memory");  // the sums in the outputs are written
-            float f0 = 0.0f, f1 = 0.0f;  // what the accumulator(s) are multiplied by
+            if (PAIR && MODE != FORWARD) {
+                // the last block's group knows the accumulators' units (and SUM_OUT: the sums in the outputs are written)
+                if (((wg + gt + nblk - 1) & 1) == 0) {
+                    join[r] = 1.0f / used(unit1);
+                    join[128 + r] = 1.0f / used(unit2);
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                pairs += nblk / 2;
+            }
+            float f0 = 0.0f, f1 = 0.0f, fv = 1.0f;  // what the accumulator(s) are multiplied by
             float g0 = 0.0f, g1 = 0.0f;  // and their sums
             if (MODE == FORWARD) {
                 float lse;
                 if (NWG == 1) {
-                    f0 = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN;
+                    g0 = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN;
+                    f0 = g0 / used(unit1);
+                    g0 *= sum_factor(m);
                     lse = row_lse(l, m, k2, P_LOG2);
                 } else {
                     join[wg * 128 + r] = m;
                     join[256 + wg * 128 + r] = l;
-                    if (C::SUM) join[512 + wg * 128 + r] = sum_factor(m);
+                    if (C::SUM) join[512 + wg * 128 + r] = sum_factor(m), join[768 + wg * 128 + r] = 1.0f / used(unit1);
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     const float m0 = join[r], m1 = join[128 + r], l0 = join[256 + r], l1 = join[256 + 128 + r];
                     const float mm = fmaxf(m0, m1);
@@ -999,17 +1189,20 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 }
                 if (a.lse && wg == 0 && row < a.q_rows)
                     a.lse[((long long)seq * a.q_heads + head) * a.q_rows + row] = live ? lse : -INFINITY;
-                f0 /= s_v;
-                f1 /= s_v;
-                if (C::SUM) {
-                    g0 = f0 * (NWG == 1 ? sum_factor(m) : join[512 + r]);
+                if (C::SUM && NWG > 1) {
+                    g0 = f0 * join[512 + r];
                     g1 = f1 * join[512 + 128 + r];
+                    f0 *= join[768 + r];
+                    f1 *= join[768 + 128 + r];
                 }
+            } else if (PAIR) {
+                g0 = args.factor;
+                f0 = g0 * join[r];
+                fv = join[128 + r];  // of dv
             } else {
-                f0 = args.factor / ds_scale / (MODE == GRAD_Q ? s_k : s_q);
-                g0 = f0;
+                f0 = args.factor / ds_scale;
+                if (F16) fv = 1.0f / P_SCALE;
             }
-            const float fv = F16 ? 1.0f / P_SCALE / s_do : 1.0f;  // of dv
             // 64 columns of an accumulator (plus what belongs to it) to this row's staging: a row of 64
             // elements, its 16-byte words swizzled by the row
             constexpr int EL = PAIR ? 4 : 2, WORDS = 64 * EL / 16, ROW = 64 * EL;
@@ -1089,7 +1282,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 uint8_t* box = rows1 + i * ROWS * ROW;
                 const int d = 64 * (i % PER);
                 const bool is_dv = MODE == GRAD_KV && i >= PER;
-                stage_box(acc + 64 * i, is_dv ? fv : f0, is_dv ? fv : g0,
+                stage_box(acc + 64 * i, is_dv ? fv : f0, is_dv ? 1.0f : g0,
                           C::SUM_OUT ? out_row(is_dv ? a.dv : a.dk) + d : nullptr, box);
                 send_box(MODE == FORWARD ? &maps.out : MODE == GRAD_Q ? &maps.dq : i < PER ? &maps.dk : &maps.dv,
                          MODE == FORWARD ? a.o : MODE == GRAD_Q ? a.dq : i < PER ? a.dk : a.dv, box, d);
@@ -1159,13 +1352,13 @@ void launch(cudaStream_t s, const AttnArgs& a, const AttnSplitSpace* sp) {
     t.factor = a.scale;
     t.negate = a.scale < 0.0f;
     t.q_tiles = (a.q_rows + ROWS - 1) / ROWS;
+    t.k_tiles = (a.k_rows + COLS - 1) / COLS;
     if (PARTS == 1) {
         t.stats = a.row_dot;
         t.norms = a.row_dot + (size_t)a.seqs * a.q_heads * t.q_tiles * 256;
     } else {
         t.stats = p.stats;
-        t.norms = p.head_norm;
-        t.maxima = p.maxima;
+        t.key_stats = p.key_stats;
     }
     launch_pdl(attention_train_tc_kernel<T, HD, MODE, PARTS>, dim3((unsigned)blocks), dim3(C::THREADS), C::SMEM, s, m, t);
 }
@@ -1198,10 +1391,11 @@ bool attention_tc_fits(const AttnArgs& a, int dtype, bool backward) {
     return f && (!backward || (q_side(a.dout) && q_side(a.dq) && k_side(a.dk) && k_side(a.dv)));
 }
 
-// The split's two launches and its blocks of one per SM cost more than they save where all of a head is
-// one tile of the fp32 units: forward, 32 sequences x 8 heads of 64 x 64 rows take 27 us against 18 there, 128 of
-// 32 rows 65 against 52; 8 of 128 rows 18 against 20, 8 of 256 rows 25 against 49.  The gradient pays
-// everywhere (1 x 16 rows 28 us against 30, 128 x 32 rows 116 against 175, 8 x 256 rows 43 against 155).
+// The split's launch and its blocks of one per SM cost more than they save where all of a head is
+// one tile of the fp32 units: forward, 32 sequences x 8 heads of 64 x 64 rows take 24 us against 18 there, 128 of
+// 32 rows 65 against 52; of 65 rows 29 against 52, 8 of 128 rows 18 against 20, 8 of 256 rows 23 against 49.
+// The gradient pays everywhere (1 x 16 rows 25 us against 30, 128 x 32 rows 133 against 175, 8 x 256 rows 43
+// against 155).
 bool attention_split_pays(size_t q_rows, size_t k_rows, bool backward) {
     return q_rows > 0 && k_rows > 0 && (backward || q_rows > 64 || k_rows > 64);
 }

@@ -412,13 +412,6 @@ __device__ __forceinline__ void split2x2(float a, float b, float s, uint32_t& h,
     unpack2(fma2(pack2(ha, hb), pack2(-1.0f, -1.0f), pack2(as, bs)), la, lb);
     l = f16x2_rn(la, lb);
 }
-// The scale of a tensor whose largest magnitude is m: the largest power of two with
-// m s <= 2^15, within 2^-100 .. 2^100; 1 for m = 0.
-__device__ __forceinline__ float split_scale_of(float m) {
-    if (!(m > 0.0f)) return 1.0f;
-    const float s = fminf(fmaxf(32768.0f / m, 7.888609052210118e-31f), 1.2676506002282294e30f);
-    return __uint_as_float(__float_as_uint(s) & 0x7f800000u);
-}
 // Four consecutive elements: h and l as 4 fp16 each (8 bytes).
 __device__ __forceinline__ void split2x4(const float* x, float s, uint2& h, uint2& l) {
     split2x2(x[0], x[1], s, h.x, l.x);

@@ -115,15 +115,13 @@ struct AttnMask {
 inline size_t attn_workspace_floats(size_t seqs, size_t q_heads, size_t q_rows) {
     return seqs * q_heads * ((q_rows + 127) / 128) * (2 * 128 + 1);
 }
-// Workspace of fp32 tensors on the tensor cores (attention_train_split.cu): the largest
-// magnitudes, the statistics, and each operand as two fp16 arrays [part][seqs][heads][rows][hd].
-constexpr int kSplitBlocks = 296;  // blocks that look for a tensor's largest magnitude
-constexpr int kSplitStat = 192;    // floats per 64 query rows: -lse log2 e | -D | |dout row|
+// Workspace of fp32 tensors on the tensor cores (attention_train_split.cu): what belongs to
+// each row, and each operand as two fp16 arrays [part][seqs][heads][rows][hd].
+constexpr int kSplitStat = 256;  // floats per 64 query rows: -lse log2 e | -D | unit of q | unit of dout
+constexpr int kKeyStat = 128;    // floats per 64 key rows: unit of k | unit of v
 struct AttnSplitSpace {
-    float* maxima;     // [4]: q, k, v, dout
-    float* partial;    // [4][kSplitBlocks]
-    float* head_norm;  // [seqs * q_heads]: the largest |dout row|
     float* stats;      // [seqs * q_heads][q tiles of 128][2][kSplitStat]
+    float* key_stats;  // [seqs * k_heads][k tiles of 64][kKeyStat]
     void *q, *k, *v, *dout;
 };
 // Lays the workspace out at `base` (may be null) and returns its size in bytes.
