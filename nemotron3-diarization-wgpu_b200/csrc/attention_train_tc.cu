@@ -1151,7 +1151,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                 continue;
             }
             // ---- the accumulators, once every product has completed (phase n; the next needs acc_read)
-            if (nblk > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(all_done, n & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(all_done, n & 1, err, DEV_TIMEOUT_ATTN_TRAIN));
             tc_fence_after();
             if (PAIR && MODE != FORWARD) {
                 // the last block's group knows the accumulators' units (and SUM_OUT: the sums in the outputs are written)
@@ -1172,13 +1172,16 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     g0 *= sum_factor(m);
                     lse = row_lse(l, m, k2, P_LOG2);
                 } else {
-                    join[wg * 128 + r] = m;
-                    join[256 + wg * 128 + r] = l;
-                    if (C::SUM) join[512 + wg * 128 + r] = sum_factor(m), join[768 + wg * 128 + r] = 1.0f / used(unit1);
+                    // Joined by the groups' parts in the item, not their numbers: the group of the first block depends on
+                    // the items this block of threads had before, and the join is not symmetric in its roundings.
+                    const int part = (wg + gt) & 1;
+                    join[part * 128 + r] = m;
+                    join[256 + part * 128 + r] = l;
+                    if (C::SUM) join[512 + part * 128 + r] = sum_factor(m), join[768 + part * 128 + r] = 1.0f / used(unit1);
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     const float m0 = join[r], m1 = join[128 + r], l0 = join[256 + r], l1 = join[256 + 128 + r];
                     const float mm = fmaxf(m0, m1);
-                    // a group that saw nothing has m = -inf and l = 0
+                    // (what saw nothing has m = -inf and l = 0)
                     const float e0 = l0 == 0.0f ? 0.0f : ex2_approx((m0 - mm) * k2);
                     const float e1 = l1 == 0.0f ? 0.0f : ex2_approx((m1 - mm) * k2);
                     const float sum = l0 * e0 + l1 * e1;
@@ -1207,16 +1210,18 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
             // elements, its 16-byte words swizzled by the row
             constexpr int EL = PAIR ? 4 : 2, WORDS = 64 * EL / 16, ROW = 64 * EL;
             // (second: the other group's accumulator; summed: what was added up before)
-            // blocks of each accumulator: the groups of the forward pass take turns, from the group of block gt
-            const int mine0 = MODE == FORWARD && NWG > 1 ? (nblk + 1 - (gt & 1)) / 2 : nblk;
-            const bool have = mine0 > 0, second = MODE == FORWARD && NWG > 1 && nblk > mine0;
-            const bool summed = C::SUM && mine0 > 2, summed2 = C::SUM && second && nblk - mine0 > 2;
-            auto stage_box = [&](uint32_t acc, float f, float gs, const float* sum_row, uint8_t* box) {
-                const uint32_t acc2 = acc + HD, sum = acc + C::NACC * HD;
+            // The groups of the forward pass take turns, from the group of block gt, whose accumulator comes first.
+            constexpr bool TURNS = MODE == FORWARD && NWG > 1;
+            const int lead = TURNS ? (gt & 1) * HD : 0;
+            const bool second = TURNS && nblk > 1;
+            const bool summed = C::SUM && (TURNS ? nblk > 4 : nblk > 2), summed2 = C::SUM && TURNS && nblk > 5;
+            auto stage_box = [&](uint32_t col, float f, float gs, const float* sum_row, uint8_t* box) {
+                const uint32_t acc = col + lead, acc2 = col + HD - lead;
+                const uint32_t sum = acc + C::NACC * HD, sum2 = acc2 + C::NACC * HD;
 #pragma unroll 1
                 for (int cb = 0; cb < 64; cb += 16) {
                     float o[16], o2[16], u[16], u2[16];
-                    if (have) tmem_ld16(acc + cb, o);
+                    tmem_ld16(acc + cb, o);
                     if (second) tmem_ld16(acc2 + cb, o2);
                     if (C::SUM_OUT) {
 #pragma unroll
@@ -1224,13 +1229,13 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     } else if (summed) {
                         tmem_ld16(sum + cb, u);
                     }
-                    if (summed2) tmem_ld16(sum + HD + cb, u2);
+                    if (summed2) tmem_ld16(sum2 + cb, u2);
                     uint32_t w[4 * EL];
 #pragma unroll
                     for (int d = 0; d < 16; d += 2) {
                         float x = 0.0f, y = 0.0f;
-                        if (live && nblk > 0) {
-                            if (have) x = o[d] * f, y = o[d + 1] * f;
+                        if (live) {
+                            x = o[d] * f, y = o[d + 1] * f;
                             if (summed) x += u[d] * gs, y += u[d + 1] * gs;
                             if (second) x += o2[d] * f1, y += o2[d + 1] * f1;
                             if (summed2) x += u2[d] * g1, y += u2[d + 1] * g1;
