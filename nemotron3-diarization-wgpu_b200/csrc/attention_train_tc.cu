@@ -78,6 +78,7 @@ constexpr int ROWS = 128, COLS = 64;
 constexpr int BOX = 64 * 128;  // a TMA box: 64 rows of 64 elements
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_LOG2 = 8.0f;  // forward: raise the running maximum when exponents would exceed 2^8
+constexpr float FAR = 32768.0f;  // exponents whose rounding, 2^-9, is no longer small
 constexpr int DEV_TIMEOUT_ATTN_TRAIN = 7;
 
 // PARTS: 1 for 16-bit tensors, 2 for fp32 tensors as fp16 pairs h + l.
@@ -844,8 +845,17 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     const bool raise = mb > m && (mb - m) * k2 > RESCALE_LOG2;
                     const float corr = raise ? ex2_approx((m - mb) * k2) : 1.0f;  // 0 from m = -inf
                     if (raise) m = mb;
-                    const float off = m == -INFINITY ? 0.0f : P_LOG2 - m * k2;
-                    const uint64_t k22 = pack2(kf, kf), off2 = pack2(off, off);
+                    float off = m == -INFINITY ? 0.0f : P_LOG2 - m * k2, ks = kf;
+                    // Huge scores: off is rounded by up to 2^-24 of it, by which every weight of the row would be off: in
+                    // fp16 they would pass 2^16, or vanish.  There the maximum is subtracted first.  (bf16 holds any such
+                    // factor and the row sum takes it out again; the test alone cost 2 % of 128 windows of 384 rows.)
+                    if ((F16 || PAIR) && fabsf(off) > FAR) {
+#pragma unroll
+                        for (int c = 0; c < 64; c++) s[c] = PAIR ? __fmul_rn(s[c], kf) - m : s[c] - m;
+                        off = P_LOG2;
+                        if (PAIR) ks = 1.0f;
+                    }
+                    const uint64_t k22 = pack2(ks, ks), off2 = pack2(off, off);
                     uint64_t sum2[4] = {0, 0, 0, 0};
                     float acc_by = corr;  // what the accumulator is multiplied by
                     if constexpr (PAIR) {

@@ -168,3 +168,36 @@ def test_fp32_weights_that_grow_along_the_row():
     run_by_row(t[0], t[1], t[2] * g.flip(1), t[3] * g.flip(1))
     run_by_row(t[0], t[1] * g.clamp(max=3.0), t[2], t[3])
     run_by_row(t[0] * g.clamp(max=3.0), t[1], t[2], t[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [60, 200])
+@pytest.mark.parametrize("size", [1.0, 1e2, 3e3])
+def test_the_largest_of_huge_scores_takes_all(dtype, hd, n, size):
+    """Every query is a large multiple of one key's row, the others are small beside it: scores of up to 1e8, of which the
+    largest leads by far more than their rounding.  Then P is 1 there and 0 elsewhere, exactly, and out is v's row.  (In
+    bf16 a row's weights keep a common factor that is no power of two, and are rounded with it.)"""
+    import torch
+
+    dt = getattr(torch, dtype)
+    pick = torch.arange(n).flip(0)
+    k = torch.sign(normal(91, 1, n, 1, hd))  # rows of the same norm, far from parallel
+    q = (k[:, pick] * size).to(dt)
+    k = (k * size).to(dt)
+    if size == 1.0:  # scores of 8 and 11: scaled to 8e6 and more in the call
+        scale = 1e6 * hd ** -0.5
+    else:
+        scale = hd ** -0.5
+    v = normal(92, 1, n, 1, hd).to(dt)
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    out, lse = torch.empty_like(q), torch.empty(1, 1, n, device="cuda")
+    space = torch.empty(max(16, n3d.attention_workspace(q, k, False)), dtype=torch.uint8, device="cuda")
+    n3d.attention_forward(q, k, v, out, lse, scale=scale, workspace=space)
+    torch.cuda.synchronize()
+    want = v[:, pick.cuda()].double()
+    # fp32: v's row in 22 bits, divided by a sum of 1; 16 bits: one rounding of what the type holds
+    assert ((out.double() - want).abs() <= 4 * E * want.abs().amax(3, keepdim=True)).all()
+    top = (q.double() * k[:, pick.cuda()].double()).sum(3).transpose(1, 2) * scale
+    assert ((lse.double() - top).abs() <= 16 * E * top).all()
