@@ -497,7 +497,9 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config *cfg, co
  * rounded to the type before the second product (sums stay fp32); fp32 tensors keep fp32
  * accuracy in every row, whatever the sizes of other rows, heads and sequences.  In fp16
  * the rows of v are to have norms below 4096 where a gradient is taken: beyond, the
- * gradient of a probability may pass fp16's largest value and dq, dk become infinite. */
+ * gradient of a probability may pass fp16's largest value and dq, dk become infinite.
+ * The gradient takes its probabilities from lse, which is rounded to fp32: with scores of
+ * 1e5 and more they are off by that rounding (at 1e6 by some per cent), but never above 1. */
 typedef struct n3d_attn_config {
     size_t seqs, q_rows, k_rows;
     size_t head_dim; /* 64 or 128 */

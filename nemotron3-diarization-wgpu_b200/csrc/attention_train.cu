@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(THREADS) attention_train_kernel(const __grid_c
                         const float lse = MODE == GRAD_KV ? col_lse[cc] : row_lse[4 * ty + i];
                         const float dot = MODE == GRAD_KV ? col_dot[cc] : row_dot[4 * ty + i];
                         const bool seen = c >= lo && c < hi;
-                        const float p = seen ? exp2f(t1[i][j] * k2 - lse) : 0.0f;
+                        // (held at 1 where the statistics' rounding passes the exponent's: huge scores)
+                        const float p = seen ? exp2f(fminf(t1[i][j] * k2 - lse, 0.0f)) : 0.0f;
                         if (MODE == GRAD_KV) w2[(4 * ty + i) * S::LP + cc] = p;
                         w1[(4 * ty + i) * S::LP + cc] = seen ? p * (t2[i][j] - dot) : 0.0f;
                     }

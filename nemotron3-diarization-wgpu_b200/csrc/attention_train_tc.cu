@@ -265,6 +265,14 @@ __device__ __forceinline__ float4 lds4(const float4* p) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(p)));
     return v;
 }
+// -lse log2 e of a row for the gradient.  Beyond 2^18 its rounding (here, and lse's own) matters: at 2^30 P would come out as
+// any power of two up to 2^128, and the gradients infinite.  There it is moved by a little more than that
+// rounding, so that P <= 1.  (Holding each exponent at 0 instead, as pairs do, took the gradient of 64 windows of
+// 377 rows of 64 in fp16 from 162 us to 167, a test for such rows to 165.)
+__device__ __forceinline__ float row_nlse(float lse) {
+    const float n = -lse * LOG2E;
+    return fabsf(n) > 262144.0f ? n - fabsf(n) * 2.384185791015625e-7f : n;  // 2^-22
+}
 // Pairs: the power of two that brings a row's largest weight w into [64, 128); 1 if there is none.  (Held below
 // 2^126, so that its inverse is normal too.)
 __device__ __forceinline__ float weight_unit(float w) {
@@ -735,7 +743,7 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                     }
                     ndot = -dot;
                     const float l = a.lse[sqh * a.q_rows + row];
-                    if (l != -INFINITY) nlse = -l * LOG2E;
+                    if (l != -INFINITY) nlse = row_nlse(l);
                 }
                 const float norm = sqrtf(norm2);
                 if (F16) ds_scale = 8.0f * inverse_power(norm);
@@ -1016,8 +1024,8 @@ __global__ void __launch_bounds__(Cfg<HD, MODE, PARTS>::THREADS, Cfg<HD, MODE, P
                                     const int i = c + e, cc = c0 + h + i;
                                     float x, y, gx, gy;
                                     unpack2(fma2(mul2(pack2(s[i], s[i + 1]), a2), row12, n2), x, y);
-                                    x = ex2_approx(x);
-                                    y = ex2_approx(y);
+                                    x = ex2_approx(fminf(x, 0.0f));  // (row_nlse: huge scores)
+                                    y = ex2_approx(fminf(y, 0.0f));
                                     if (masked && (cc < lo || cc >= hi)) x = 0.0f;
                                     if (masked && (cc + 1 < lo || cc + 1 >= hi)) y = 0.0f;
                                     const uint64_t g2 = mul2(pack2(x, y), fma2(mul2(pack2(u[i], u[i + 1]), b2), row22, d2));

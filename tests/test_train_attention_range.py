@@ -135,7 +135,7 @@ def test_fp32_sizes_that_differ(hd, which, by):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("which", ["v", "dout"])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
 @pytest.mark.parametrize("n", [150, 333])
 def test_fp32_one_row_a_billion_times_the_others(hd, which, n):
     """Rows that a window keeps apart from it are as good as without it."""
@@ -201,3 +201,37 @@ def test_the_largest_of_huge_scores_takes_all(dtype, hd, n, size):
     assert ((out.double() - want).abs() <= 4 * E * want.abs().amax(3, keepdim=True)).all()
     top = (q.double() * k[:, pick.cuda()].double()).sum(3).transpose(1, 2) * scale
     assert ((lse.double() - top).abs() <= 16 * E * top).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("layout", ["rows", "odd"])
+def test_gradients_of_huge_scores_stay_in_bounds(dtype, hd, layout):
+    """One query and one key row with a score of about 1e9, whose row statistics are rounded by about 64.  P <= 1 bounds every
+    gradient: |dS| <= 2 |dout row| |v row|; and rows of dq that do not see the pair are what they are without it."""
+    import torch
+
+    n = 200
+    t = [normal(81 + i, 1, n, 1, hd).to(getattr(torch, dtype)) for i in range(4)]
+    t[3] *= 0.1
+    got = []
+    for size in (1.0, 1e4):
+        q, k, v, do = (x.clone() for x in t)
+        q[0, 150] *= size
+        k[0, 70] = q[0, 150]
+        if layout == "odd":
+            q, k, v, do = (torch.nn.functional.pad(x.cuda().reshape(-1), (1, 0))[1:].view(x.shape) for x in (q, k, v, do))
+        q, k, v, do = (x.cuda() for x in (q, k, v, do))
+        out, dq, dk, dv = (torch.empty_like(x) for x in (q, q, k, v))
+        lse = torch.empty(1, 1, n, device="cuda")
+        space = torch.empty(n3d.attention_workspace(q, k), dtype=torch.uint8, device="cuda")
+        n3d.attention_forward(q, k, v, out, lse, right=0, workspace=space)
+        n3d.attention_backward(q, k, v, out, lse, do, dq, dk, dv, right=0, workspace=space)
+        torch.cuda.synchronize()
+        got.append((dq, dk, dv))
+    norm = lambda x: x.double().norm(dim=3).cpu()
+    ds = 2.1 * norm(do).max() * norm(v).max() * hd ** -0.5
+    assert norm(dq).max() <= ds * norm(k).sum() and norm(dk).max() <= ds * norm(q).sum()
+    assert norm(dv).max() <= 1.1 * norm(do).sum()
+    assert torch.equal(got[0][0][:, :70], got[1][0][:, :70])
