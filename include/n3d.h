@@ -492,6 +492,7 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config *cfg, co
  * A row that sees no key has out = 0 and lse = -inf, and no gradient passes it.  Rows at
  * or past q_len and k_len are not read: they may hold anything.  q_len and k_len are
  * int32 [seqs] device arrays, values outside 0..rows are clamped; NULL means all rows.
+ * No output overlaps an input or another output.
  *
  * bf16 and fp16 products run on the tensor cores with probabilities and their gradients
  * rounded to the type before the second product (sums stay fp32); fp32 tensors keep fp32

@@ -197,6 +197,11 @@ void check_workspace(size_t need, const void* p, size_t bytes) {
               "attention: a 16-byte aligned workspace of n3d_attention_workspace bytes is wanted");
 }
 
+// An output that stands where tensors do that other blocks, or later launches, still read or write.
+void check_apart(const n3d_heads* out, std::initializer_list<const n3d_heads*> others, const char* what) {
+    for (const n3d_heads* t : others) arg_check(!out->d_data || out->d_data != t->d_data, what);
+}
+
 void check_sizes(size_t seqs, size_t rows) {
     arg_check(seqs <= (size_t)INT_MAX && rows <= (size_t)INT_MAX, "seqs or rows beyond 2^31");
 }
@@ -411,6 +416,7 @@ n3d_status n3d_attention_forward(int device, const n3d_attn_config* cfg, const n
     return guarded([&] {
         check_attn(cfg);
         n3d::AttnArgs a = attn_args(*cfg, q, k, v, out, true, d_q_len, d_k_len);
+        check_apart(out, {k, v}, "n3d_attention_forward: out stands where keys or values do");
         check_workspace(n3d_attention_workspace(cfg, q->heads, k->heads, 0), d_workspace, workspace_bytes);
         a.lse = d_lse;
         a.row_dot = static_cast<float*>(d_workspace);
@@ -438,6 +444,10 @@ n3d_status n3d_attention_backward(int device, const n3d_attn_config* cfg, const 
         check_heads(*dv, cfg->seqs, cfg->k_rows, cfg->head_dim, cfg->dtype, true);
         arg_check(dout->heads == q->heads && dq->heads == q->heads && dk->heads == k->heads && dv->heads == k->heads,
                   "n3d_attention_backward: a gradient has other heads than its tensor");
+        const char* apart = "n3d_attention_backward: a gradient stands where an input or another gradient does";
+        check_apart(dq, {q, k, v, dout, dk, dv}, apart);
+        check_apart(dk, {q, v, out, dout, dv}, apart);
+        check_apart(dv, {q, k, out, dout}, apart);
         check_workspace(n3d_attention_workspace(cfg, q->heads, k->heads, 1), d_workspace, workspace_bytes);
         a.dout = view(*dout), a.dq = view(*dq), a.dk = view(*dk), a.dv = view(*dv);
         a.lse = const_cast<float*>(d_lse);
