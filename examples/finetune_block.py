@@ -57,8 +57,9 @@ class Block:
         self.norm_space = e(n3d.residual_norm_workspace(rows, WIDTH, rows), t=torch.uint8)
 
     def step(self, x, prev, target, lens) -> torch.Tensor:
-        """One forward and backward pass; the gradients are in self.grads and self.dx.  x fp32 [rows, 512],
-        prev and target [rows, 512] of the block's type, lens int32 [windows].  Returns the loss."""
+        """One forward and backward pass; the gradients are in self.grads and self.dx, and that of prev, still times
+        self.loss_scale, in self.dprev.  x fp32 [rows, 512], prev and target [rows, 512] of the block's type, lens
+        int32 [windows].  Returns the loss."""
         p, g, rows = self.p, self.grads, self.b * self.s
         st = torch.cuda.current_stream().cuda_stream
         norm1 = dict(gate=p["gate"], gate_rows=rows, pre_w=p["w1"], pre_b=p["b1"], stream=st)

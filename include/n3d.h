@@ -492,13 +492,17 @@ n3d_status n3d_residual_norm_grad(int device, const n3d_residual_config *cfg, co
  * A row that sees no key has out = 0 and lse = -inf, and no gradient passes it.  Rows at
  * or past q_len and k_len are not read: they may hold anything.  q_len and k_len are
  * int32 [seqs] device arrays, values outside 0..rows are clamped; NULL means all rows.
- * No output overlaps an input or another output.
+ * No output overlaps an input or another output.  What the rows inside the lengths hold
+ * is finite: the weight of a pair that a window hides is 0, and 0 times an infinity or NaN
+ * is NaN, so such a value may reach rows that do not see it.
  *
  * bf16 and fp16 products run on the tensor cores with probabilities and their gradients
  * rounded to the type before the second product (sums stay fp32); fp32 tensors keep fp32
  * accuracy in every row, whatever the sizes of other rows, heads and sequences.  In fp16
  * the rows of v are to have norms below 4096 where a gradient is taken: beyond, the
- * gradient of a probability may pass fp16's largest value and dq, dk become infinite.
+ * gradient of a probability may pass fp16's largest value and dq, dk become infinite; and
+ * dk of keys that only rows of small dout see (2^-8 of the largest |dout row| of the heads
+ * and less) is rounded like gradients of that many powers of two more.
  * The gradient takes its probabilities from lse, which is rounded to fp32: with scores of
  * 1e5 and more they are off by that rounding (at 1e6 by some per cent), but never above 1. */
 typedef struct n3d_attn_config {

@@ -31,8 +31,10 @@
 //
 // fp16: P is kept times 2^7 (forward, P <= 2^8 there) or 2^10 (dkv), and dS times 2^3 /
 // |dout row| (dq) or over the largest |dout row| of the head group (dkv), as powers of
-// two, so that small weights and gradients keep fp16's precision; |dS| <= 2 P |dout row|
-// |v row| then stays inside fp16 while |v row| < 4096.
+// two, so that small weights and gradients keep fp16's precision.  dS_j = P_j (1 - P_j) dout . (v_j - o'), o' the
+// mean of the other rows of v by their weights, so |dS| <= |dout row| max |v row| / 2, and times up to 16 /
+// |dout row| it stays below 2^15 while |v row| < 4096.  (In dkv the rows with the least dout lose bits: where
+// P |dout row| |v row| is below 2^-16 of the largest |dout row|, dS is subnormal.)
 //
 // fp32: every operand is a pair h + l of fp16 arrays (attention_train_split.cu), each row of it in a unit
 // of its own, a power of two; the weights are split in the softmax, and each product is l h + h l + h h.

@@ -3,7 +3,7 @@
 // Bound: memory.  Each element of x and block is read once and each of r and y written
 // once; the row stays in registers between its sums (mean, then the squares of the
 // centred values, for each norm), so nothing is read twice.  Rows of up to 1024 columns
-// belong to one warp, whose sums need no barrier; wider rows to a block of 128 to 512
+// belong to one warp, whose sums need no barrier; wider rows to a block of 128 or 256
 // threads with 16 or 32 columns each.  Enough warps are resident to keep loads in flight while
 // others sum.
 //
