@@ -11,7 +11,7 @@
 //
 // Bound: latency (four lines of a thread are in flight) before memory: one read of each
 // operand and one write of the same size.  Measured on a B200, cold: q, k and v of 8 x 501 rows,
-// 8 heads of 64 (25 MB) 18 us, with dout and the statistics 24; of 2 x 4096 rows, 16 heads (101 MB) 60 and 88.
+// 8 heads of 64 (25 MB) 18 - 20 us, with dout and the statistics 24 - 26; of 2 x 4096 rows, 16 heads (101 MB) 60 and 88.
 
 #include <cuda_fp16.h>
 
