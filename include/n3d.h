@@ -439,7 +439,7 @@ n3d_status n3d_rope_plan_make(const n3d_rope_config *cfg, n3d_rope_plan *plan);
  * d_positions[s * rows + r], or first_position + r when d_positions is NULL; positions
  * may be negative.  transpose != 0 applies the transposed rotation, which is the
  * gradient: x then holds dL/dy and y receives dL/dx.  y[t] may be x[t] itself (the same
- * pointer and strides), and must not overlap it otherwise. */
+ * pointer and strides), and must not overlap it otherwise, nor the other tensors. */
 n3d_status n3d_rope(int device, const n3d_rope_plan *plan, int dtype, size_t seqs, size_t rows, size_t count,
                     const n3d_heads *x, const n3d_heads *y, const int32_t *d_positions, long long first_position,
                     int transpose, void *stream);

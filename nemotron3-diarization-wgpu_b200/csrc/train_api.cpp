@@ -290,6 +290,11 @@ n3d_status n3d_rope(int device, const n3d_rope_plan* plan, int dtype, size_t seq
                           "n3d_rope: in place, x and y must have the same strides");
             heads += x[i].heads;
         }
+        if (count == 2) {
+            const char* apart = "n3d_rope: an output stands where the other tensor or the other output does";
+            check_apart(&y[0], {&x[1], &y[1]}, apart);
+            check_apart(&y[1], {&x[0]}, apart);
+        }
         if (seqs == 0 || rows == 0) return;
         if (count == 1) a.x[1] = a.x[0], a.y[1] = a.y[0];
         a.heads0 = (int)x[0].heads;
